@@ -264,6 +264,39 @@ int rg_shard_softmax_finish(int dtype, int index_dtype, int64_t d, int64_t n, in
 int rg_run_noalloc(int op, int dtype, int index_dtype, int64_t d, int64_t n, int64_t b,
                    const void *values, const void *offsets, void *out, uint32_t flags, void *stream);
 
+/* ------------------------------------------------------- segmented scan
+ * This build's extension (the reference has no such operation): a gated
+ * linear recurrence over the packed rows, column by column,
+ *   out[t] = gates[t] * out[t - 1] + values[t]
+ * within each segment.  Before a segment's first row the state is
+ * initial[s] (f32 [B, D]); without `initial` (NULL) the first row's output is
+ * values[t] and its gate is not used.  final_state[s] (f32 [B, D], NULL: not
+ * wanted) is the state after the segment's last row; for a segment without
+ * rows it is initial[s], or 0.  values, gates and out are [N, D] of `dtype`
+ * with 1 <= D <= 65536; states are f32 and are rounded to `dtype` only in out.
+ * Gates must be finite, and products of the gates over neighbouring rows of a
+ * segment must stay in f32's range where its states are not zero (|gate| <= 1
+ * always does).
+ *
+ * rg_scan_workspace_bytes gives the scratch of either call (256-byte aligned;
+ * 0: none) and carry_rows, the rows of `carries` (f32 [carry_rows, D]): the
+ * states that rg_scan records for rg_scan_backward, NULL if no backward pass
+ * follows.  rg_scan_backward takes the forward call's inputs and carries and
+ * the gradients of out and final_state (NULL: zero) and writes the gradients
+ * that are not NULL; grad_initial (f32 [B, D]) needs `initial`.  Written
+ * tensors overlap nothing.  flags: RG_FLAG_NO_VECTORIZE, the same for both
+ * passes.  Results do not depend on timing: equal inputs give equal bits. */
+int rg_scan_workspace_bytes(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, uint32_t flags,
+                            int64_t *bytes, int64_t *carry_rows);
+int rg_scan(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, const void *values, const void *gates,
+            const void *offsets, const float *initial, void *out, float *final_state, float *carries,
+            void *workspace, int64_t workspace_bytes, uint32_t flags, void *stream, rg_report *report);
+int rg_scan_backward(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, const void *values,
+                     const void *gates, const void *offsets, const float *initial, const float *carries,
+                     const void *grad_out, const float *grad_final, void *grad_values, void *grad_gates,
+                     float *grad_initial, void *workspace, int64_t workspace_bytes, uint32_t flags, void *stream,
+                     rg_report *report);
+
 /* ------------------------------------------------------- schedule choice
  * This build's extension (the reference chooses in Python,
  * python/ragged/selection.py:106-126): the scores of the boosted decision

@@ -57,6 +57,8 @@ enum KernelId : int {
   K_OFFSETS_CHECK = 11,
   K_POINTWISE_LOGITS = 12,
   K_POINTWISE_CAST = 13,
+  K_SCAN = 14,
+  K_SCAN_BACKWARD = 15,
 };
 
 // Recording helper for rg_report.

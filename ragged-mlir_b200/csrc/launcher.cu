@@ -210,6 +210,8 @@ const char *rg_kernel_name(int kernel_id) {
     case K_OFFSETS_CHECK: return "offsets_check";
     case K_POINTWISE_LOGITS: return "pointwise_logits";
     case K_POINTWISE_CAST: return "pointwise_cast";
+    case K_SCAN: return "scan";
+    case K_SCAN_BACKWARD: return "scan_backward";
   }
   return "";
 }

@@ -10,12 +10,13 @@ from .cache import Artifact, ArtifactCache, CacheKey
 from .compiler import Compiler
 from .errors import (CacheError, CacheMismatch, CacheMiss, CompilationError, RaggedError, RuntimeUnavailable,
                      SpecializationLimit, ToolchainUnavailable, ValidationError)
-from .model import DIALECT_VERSION, ExecutionReport, Hints, ProgramSpec
+from .layers import CompiledMatmul, CompiledScan
+from .model import DIALECT_VERSION, ExecutionReport, Hints, MatmulSpec, ProgramSpec, ScanSpec
 from .optimizations import Optimizations
 from .runtime import CompiledProgram
 
 __all__ = ["Artifact", "ArtifactCache", "CacheKey", "Compiler", "CompiledProgram", "DIALECT_VERSION",
-           "ExecutionReport", "Hints", "Optimizations", "ProgramSpec", "RaggedError", "ValidationError",
+           "ExecutionReport", "Hints", "MatmulSpec", "Optimizations", "ProgramSpec", "ScanSpec", "RaggedError", "ValidationError",
            "CacheError", "CacheMismatch", "CacheMiss", "CompilationError", "RuntimeUnavailable",
            "SpecializationLimit", "ToolchainUnavailable"]
 

@@ -28,13 +28,15 @@ FLAG_NO_VECTORIZE = 1
 FLAG_IN_PLACE = 2
 FLAG_NO_POINTWISE_FUSION = 4
 MAX_LAUNCHES = 8
+PRODUCTS = {"forward": 0, "grad_values": 1, "grad_weights": 2}
 
 # Every symbol include/ragged_b200.h declares.
 EXPORTED = ("rg_version", "rg_error_string", "rg_last_error", "rg_get_device_info", "rg_workspace_bytes",
             "rg_run", "rg_kernel_name", "rg_check_offsets", "rg_pointwise_workspace_bytes", "rg_run_pointwise",
             "rg_shard_rows", "rg_shard_split", "rg_shard_edge_bytes", "rg_shard_workspace_bytes",
             "rg_shard_segments", "rg_shard_softmax_workspace_bytes", "rg_run_shard_softmax",
-            "rg_shard_softmax_finish", "rg_run_shard", "rg_shard_combine", "rg_run_noalloc", "rg_tree_scores")
+            "rg_shard_softmax_finish", "rg_run_shard", "rg_shard_combine", "rg_run_noalloc", "rg_tree_scores",
+            "rg_scan_workspace_bytes", "rg_scan", "rg_scan_backward")
 
 
 class Report(ctypes.Structure):
@@ -96,6 +98,13 @@ def library(path: Path | None = None):
         lib.rg_run_noalloc.restype = i32
         lib.rg_tree_scores.argtypes = [i64, p, p, p, p, p, p, i64, p, p, i32, p, i32, p, i32, p]
         lib.rg_tree_scores.restype = i32
+        lib.rg_scan_workspace_bytes.argtypes = [i32, i32, i64, i64, i64, u32, ctypes.POINTER(i64), ctypes.POINTER(i64)]
+        lib.rg_scan_workspace_bytes.restype = i32
+        lib.rg_scan.argtypes = [i32, i32, i64, i64, i64, p, p, p, p, p, p, p, p, i64, u32, p, ctypes.POINTER(Report)]
+        lib.rg_scan.restype = i32
+        lib.rg_scan_backward.argtypes = [i32, i32, i64, i64, i64, p, p, p, p, p, p, p, p, p, p, p, i64, u32, p,
+                                         ctypes.POINTER(Report)]
+        lib.rg_scan_backward.restype = i32
         pi64 = ctypes.POINTER(i64)
         lib.rg_shard_rows.argtypes = [i64, i32, i32, pi64, pi64]
         lib.rg_shard_rows.restype = i32
@@ -325,6 +334,35 @@ def check_offsets(index: str, n: int, b: int, offsets_ptr: int, min_len: int | N
     raise_for(library().rg_check_offsets(INDEX[index], n, b, offsets_ptr, -1 if min_len is None else min_len,
                                          -1 if max_len is None else max_len, status_ptr, stream or None,
                                          ctypes.byref(report)), "rg_check_offsets")
+    return report
+
+
+# --------------------------------------------------------- learned operators
+
+def scan_sizes(dtype: str, index: str, d: int, n: int, b: int, flags: int = 0) -> tuple[int, int]:
+    """(scratch bytes, rows of recorded states) of a segmented scan."""
+    nbytes, rows = ctypes.c_int64(0), ctypes.c_int64(0)
+    raise_for(library().rg_scan_workspace_bytes(DTYPES[dtype], INDEX[index], d, n, b, flags, ctypes.byref(nbytes),
+                                                ctypes.byref(rows)), "rg_scan_workspace_bytes")
+    return nbytes.value, rows.value
+
+
+def scan(dtype: str, index: str, d: int, n: int, b: int, pointers: tuple, workspace_ptr: int, workspace_bytes: int,
+         flags: int, stream: int) -> Report:
+    """``pointers``: values, gates, offsets, initial, out, final, carries (0: none)."""
+    report = Report()
+    raise_for(library().rg_scan(DTYPES[dtype], INDEX[index], d, n, b, *pointers, workspace_ptr, workspace_bytes, flags,
+                                stream, ctypes.byref(report)), "rg_scan")
+    return report
+
+
+def scan_backward(dtype: str, index: str, d: int, n: int, b: int, pointers: tuple, workspace_ptr: int,
+                  workspace_bytes: int, flags: int, stream: int) -> Report:
+    """``pointers``: values, gates, offsets, initial, carries, grad_out,
+    grad_final, grad_values, grad_gates, grad_initial (0: none)."""
+    report = Report()
+    raise_for(library().rg_scan_backward(DTYPES[dtype], INDEX[index], d, n, b, *pointers, workspace_ptr,
+                                         workspace_bytes, flags, stream, ctypes.byref(report)), "rg_scan_backward")
     return report
 
 

@@ -36,7 +36,7 @@ import tempfile
 from typing import Any
 
 from .errors import CacheMismatch, CacheMiss, SpecializationLimit, ValidationError
-from .model import DIALECT_VERSION, ProgramSpec, canonical_json
+from .model import DIALECT_VERSION, SPECS, canonical_json
 
 LEDGER_FORMAT = 2
 
@@ -67,8 +67,8 @@ class CacheKey:
             raise ValidationError("a cache key needs the library version")
 
     @classmethod
-    def from_spec(cls, spec: ProgramSpec, *, library_version: str, library_sha256: str) -> "CacheKey":
-        if not isinstance(spec, ProgramSpec):
+    def from_spec(cls, spec, *, library_version: str, library_sha256: str) -> "CacheKey":
+        if not isinstance(spec, SPECS):
             raise ValidationError("spec must be a ProgramSpec")
         return cls(spec.ir_hash, spec.signature, library_version, library_sha256)
 

@@ -22,7 +22,7 @@ from typing import Any
 from . import _native
 from .cache import Artifact, ArtifactCache, CacheKey, CacheMiss
 from .errors import CompilationError, ToolchainUnavailable
-from .model import DIALECT_VERSION, ProgramSpec
+from .model import DIALECT_VERSION, MatmulSpec, ProgramSpec, ScanSpec
 
 _DIGESTS: dict[tuple, str] = {}
 
@@ -30,10 +30,13 @@ _DIGESTS: dict[tuple, str] = {}
 IMPLEMENTED = {"reduce": ("naive", "classified", "rowbalanced"), "softmax": ("naive", "classified", "rowbalanced")}
 
 
-def schedules_for(spec: ProgramSpec) -> list[str]:
+def schedules_for(spec) -> list[str]:
     """Schedules a program of ``spec`` may run: block per segment only for
     the naive strategy (or classification disabled), otherwise the
-    implemented selecting schedules of its family."""
+    implemented selecting schedules of its family.  A scan or a matrix
+    product has one, its own."""
+    if isinstance(spec, (ScanSpec, MatmulSpec)):
+        return [spec.op]
     if spec.strategy == "naive" or not spec.optimizations.classification:
         return ["naive"]
     family = "softmax" if spec.op == "softmax" else "reduce"
@@ -77,27 +80,34 @@ class Compiler:
             raise CompilationError(f"{', '.join(unsupported)} not implemented by libragged_b200 "
                                    "(outside this build's hot path)")
 
-    def compile(self, spec: ProgramSpec, cache: ArtifactCache, *, adaptive: bool = True, **_: Any):
-        """A CompiledProgram for ``spec``; cached manifests are reused."""
+    def compile(self, spec, cache: ArtifactCache, *, adaptive: bool = True, **_: Any):
+        """A CompiledProgram for a ProgramSpec, a CompiledScan for a ScanSpec, a
+        CompiledMatmul for a MatmulSpec; cached manifests are reused."""
         from .runtime import CompiledProgram
         program = self._compile(spec, cache)
+        if not isinstance(program, CompiledProgram):
+            return program
         if not adaptive or not program.selects:
             return program
         naive = self._compile(replace(spec, strategy="naive"), cache)
         return CompiledProgram(spec, program.artifact, cache_hit=program.cache_hit and naive.cache_hit, naive=naive)
 
-    def _compile(self, spec: ProgramSpec, cache: ArtifactCache):
+    def _compile(self, spec, cache: ArtifactCache):
+        from .layers import CompiledMatmul, CompiledScan
         from .runtime import CompiledProgram
-        if not isinstance(spec, ProgramSpec):
-            raise CompilationError("spec must be a ProgramSpec")
-        self._check_supported(spec)
+        kinds = ((ProgramSpec, CompiledProgram), (ScanSpec, CompiledScan), (MatmulSpec, CompiledMatmul))
+        build = next((program for kind, program in kinds if isinstance(spec, kind)), None)
+        if build is None:
+            raise CompilationError("spec must be a ProgramSpec, a ScanSpec or a MatmulSpec")
+        if isinstance(spec, ProgramSpec):
+            self._check_supported(spec)
         tool = self.toolchain(chip=spec.chip)
         key = CacheKey.from_spec(spec, library_version=tool["library_version"],
                                  library_sha256=tool["library_sha256"])
         try:
-            return CompiledProgram(spec, cache.load(key), cache_hit=True)
+            return build(spec, cache.load(key), cache_hit=True)
         except CacheMiss:
             pass
         metadata = {"toolchain": tool, "spec": spec.to_dict(), "schedules": schedules_for(spec)}
         artifact = cache.publish(key, metadata)
-        return CompiledProgram(spec, artifact, cache_hit=False)
+        return build(spec, artifact, cache_hit=False)

@@ -1,0 +1,259 @@
+"""Programs of the learned operators: the segmented scan and the segmented
+matrix product.
+
+``Compiler().compile(ScanSpec(...), cache)`` gives a ``CompiledScan`` and a
+``MatmulSpec`` a ``CompiledMatmul``.  Both follow ``CompiledProgram.run``: CUDA
+tensors on one device, outputs that the caller allocates, the current stream
+unless ``stream`` is given, no synchronisation in validated mode, and
+``mode="checked"`` to validate the offsets on the device first.  ``run``
+records no gradient; ``run_backward`` computes the gradients of a call, and
+``torch_adapter.segment_scan`` / ``segment_matmul`` put both behind autograd.
+
+Neither operation exists in the reference, whose programs end at sums, maxima
+and softmaxes of packed rows.
+"""
+from __future__ import annotations
+
+from contextlib import nullcontext
+import time
+
+from . import _native
+from .cache import Artifact
+from .errors import CacheMismatch, RuntimeUnavailable, ValidationError
+from .model import ExecutionReport, MatmulSpec, ScanSpec, runs_on
+from .runtime import CompiledProgram, _checked_devices, _torch
+from .validation import STATUS_BYTES
+
+
+def scan_chunk_rows(dtype: str, d: int, vectorize: bool = True) -> int:
+    """Rows per recorded state of a scan (the kernels' chunk: 256 threads,
+    tiles of up to 128 bytes of columns, 4 rows a thread of full 16-byte
+    vectors and 8 of narrower ones)."""
+    size = 4 if dtype == "f32" else 2
+    vec = 1
+    while vectorize and 2 * vec * size <= 16 and d % (2 * vec) == 0:
+        vec *= 2
+    lanes = 1
+    while lanes < d // vec and lanes < 32 and 2 * lanes * vec * size <= 128:
+        lanes *= 2
+    return 256 // lanes * (4 if vec * size == 16 else 8)
+
+
+class _LayerProgram:
+    """Checks and launch steps that both programs share."""
+
+    kind: type
+
+    def __init__(self, spec, artifact: Artifact, *, cache_hit: bool = False):
+        if not isinstance(spec, self.kind):
+            raise ValidationError(f"spec must be a {self.kind.__name__}")
+        if artifact.key.ir_hash != spec.ir_hash:
+            raise CacheMismatch("artifact was recorded for a different specialization")
+        self.spec, self.artifact, self.cache_hit = spec, artifact, cache_hit
+        self._digest = artifact.key.digest
+        self._dtypes = None
+        self._sizes: dict[tuple, object] = {}
+
+    schedules = property(lambda self: (self.spec.op,))
+    _check_offsets = CompiledProgram._check_offsets
+    _check_device_status = staticmethod(CompiledProgram._check_device_status)
+
+    def close(self) -> None:
+        """Nothing to unload: kernels live in the shared library."""
+
+    def _cached(self, key, compute):
+        found = self._sizes.get(key)
+        if found is None:
+            if len(self._sizes) >= 256:
+                self._sizes.clear()
+            found = self._sizes[key] = compute()
+        return found
+
+    def _tensors(self, torch, tensors, offsets, mode, gradless):
+        """Checks the offsets and each (name, tensor, shape, dtype)."""
+        if mode not in ("validated", "checked"):
+            raise ValidationError("mode must be validated or checked")
+        if self._dtypes is None:
+            self._dtypes = ({"f32": torch.float32, "bf16": torch.bfloat16}[self.spec.dtype],
+                            {"i32": torch.int32, "i64": torch.int64}[self.spec.offsets_dtype])
+        if not isinstance(offsets, torch.Tensor):
+            raise ValidationError("offsets must be a torch.Tensor")
+        if not offsets.is_cuda:
+            raise RuntimeUnavailable(f"offsets must be on a CUDA device that runs {self.spec.chip} code; "
+                                     "no CPU execution fallback exists")
+        if offsets.dtype != self._dtypes[1]:
+            raise ValidationError("tensor dtype differs from compiled dtype/offsets specialization")
+        if not offsets.is_contiguous():
+            raise ValidationError("offsets must be row-major contiguous")
+        device, recording = offsets.device, gradless and torch.is_grad_enabled()
+        for name, tensor, shape, dtype in tensors:
+            if not isinstance(tensor, torch.Tensor):
+                raise ValidationError(f"{name} must be a torch.Tensor")
+            if not tensor.is_cuda:
+                raise RuntimeUnavailable(f"{name} must be on a CUDA device that runs {self.spec.chip} code; "
+                                         "no CPU execution fallback exists")
+            if tensor.device != device:
+                raise ValidationError(f"{name} must use the CUDA device of offsets")
+            if tensor.dtype != dtype:
+                raise ValidationError(f"{name} must have dtype {dtype}: tensor dtype differs from compiled "
+                                      "dtype/offsets specialization")
+            if tensor.shape != shape:
+                raise ValidationError(f"{name} must have shape {tuple(shape)}")
+            if not tensor.is_contiguous():
+                raise ValidationError(f"{name} must be row-major contiguous")
+            if recording and tensor.requires_grad:
+                raise ValidationError(f"{name} requires a gradient, which run() does not record: use "
+                                      "torch_adapter, or torch.no_grad()")
+
+    def _segments(self, torch, offsets) -> int:
+        if not isinstance(offsets, torch.Tensor) or offsets.ndim != 1 or offsets.numel() < 1:
+            raise ValidationError("offsets must have shape [B+1], including [0] when B=0")
+        return offsets.numel() - 1
+
+    def _rows(self, values, torch, name="values") -> int:
+        if not isinstance(values, torch.Tensor) or values.ndim != 2:
+            raise ValidationError(f"{name} must have shape [N, static D]")
+        return values.shape[0]
+
+    def _launch(self, torch, offsets, n, b, stream, mode, used, work) -> ExecutionReport:
+        """For each (bytes, call) of ``work``: ``call(scratch address, bytes,
+        stream)`` on the execution stream."""
+        started = time.perf_counter()
+        checked = mode == "checked"
+        if b == 0 and n != 0 and not checked:  # checked mode reports it from the device
+            raise ValidationError("B=0 requires N=0; values cannot exist without segments")
+        if self.spec.offsets_dtype == "i32" and n > 2**31 - 1:
+            raise ValidationError("N exceeds the i32 offsets range")
+        device = offsets.device
+        reports, validation, total = [], None, 0
+        with torch.cuda.device(device):
+            if device.index not in _checked_devices:
+                capability = tuple(torch.cuda.get_device_capability(device))
+                if not runs_on(self.spec.chip, capability):
+                    raise RuntimeUnavailable(f"compiled target {self.spec.chip} does not run on the current device "
+                                             f"(sm_{capability[0]}{capability[1]})")
+                _checked_devices.add(device.index)
+            active = stream if stream is not None else torch.cuda.current_stream(device)
+            if not isinstance(active, torch.cuda.Stream) or active.device != device:
+                raise ValidationError("stream must be a torch.cuda.Stream on the values device")
+            if checked:
+                validation = self._check_offsets(offsets, offsets, n, b, active, torch)
+            if b:
+                if stream is not None:
+                    for tensor in used:
+                        tensor.record_stream(active)
+                for nbytes, call in work:
+                    scratch = None
+                    if nbytes:
+                        with torch.cuda.stream(active) if stream is not None else nullcontext():
+                            scratch = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+                    report = call(scratch.data_ptr() if nbytes else 0, nbytes, active.cuda_stream)
+                    reports.append(report)
+                    total = max(total, nbytes)
+                    if checked and nbytes and report.status_offset >= 0:
+                        self._check_device_status(scratch, int(report.status_offset), active, torch)
+        return self._report(started, reports, total, validation)
+
+    def _report(self, started, reports, nbytes, validation) -> ExecutionReport:
+        check, check_ms = validation if validation is not None else (None, None)
+        parts = ([check] if check is not None else []) + reports
+        names = tuple(_native.kernel_name(r.kernel_ids[i]) for r in parts for i in range(r.num_launches))
+        grids = tuple(tuple(r.grid[i]) for r in parts for i in range(r.num_launches))
+        checked_bytes = STATUS_BYTES if check is not None else 0
+        return ExecutionReport(("rows",) if reports else (), (), grids, nbytes + checked_bytes, self._digest, None,
+                               "checked" if check is not None else "validated", names,
+                               (time.perf_counter() - started) * 1000, cache_hit=self.cache_hit,
+                               validation_workspace_bytes=checked_bytes, validation_host_ms=check_ms,
+                               d_tile=int(reports[-1].d_tile) if reports else None,
+                               d_vector=int(reports[-1].d_vector) if reports else 1, selected=self.spec.op)
+
+
+def _address(tensor) -> int:
+    return 0 if tensor is None else tensor.data_ptr()
+
+
+class CompiledScan(_LayerProgram):
+    """out[t] = gates[t] * out[t - 1] + values[t] within each segment."""
+
+    kind = ScanSpec
+
+    def __init__(self, spec, artifact, *, cache_hit: bool = False):
+        super().__init__(spec, artifact, cache_hit=cache_hit)
+        self._flags = 0 if spec.vectorize else _native.FLAG_NO_VECTORIZE
+
+    def carry_rows(self, n: int) -> int:
+        """Rows of the ``carries`` that a call over ``n`` rows records."""
+        rows = scan_chunk_rows(self.spec.dtype, self.spec.feature_dim, self.spec.vectorize)
+        return (n + rows - 1) // rows
+
+    def _scratch(self, n, b) -> int:
+        return self._cached((n, b), lambda: _native.scan_sizes(
+            self.spec.dtype, self.spec.offsets_dtype, self.spec.feature_dim, n, b, self._flags))[0]
+
+    def run(self, values, gates, offsets, out, stream=None, mode: str = "validated", *, initial=None, final=None,
+            carries=None) -> ExecutionReport:
+        """Writes ``out`` [N, D] and, where given, ``final`` (f32 [B, D], the
+        state after each segment) and ``carries`` (f32 [carry_rows(N), D],
+        what ``run_backward`` needs).  ``initial`` (f32 [B, D]) is the state
+        before each segment; without it a segment's first row is its first
+        value.  ``values``, ``gates`` and ``out`` have the program's dtype;
+        outputs overlap nothing."""
+        return self._run(values, gates, offsets, out, initial, final, carries, stream, mode, True)
+
+    def _run(self, values, gates, offsets, out, initial, final, carries, stream, mode, gradless):
+        torch = _torch()
+        spec, d = self.spec, self.spec.feature_dim
+        b, n = self._segments(torch, offsets), self._rows(values, torch)
+        dtype = torch.float32 if spec.dtype == "f32" else torch.bfloat16
+        tensors = [("values", values, (n, d), dtype), ("gates", gates, (n, d), dtype), ("out", out, (n, d), dtype)]
+        if initial is not None:
+            tensors.append(("initial", initial, (b, d), torch.float32))
+        if final is not None:
+            tensors.append(("final", final, (b, d), torch.float32))
+        if carries is not None:
+            tensors.append(("carries", carries, (self.carry_rows(n), d), torch.float32))
+        self._tensors(torch, tensors, offsets, mode, gradless)
+        pointers = (values.data_ptr(), gates.data_ptr(), offsets.data_ptr(), _address(initial), out.data_ptr(),
+                    _address(final), _address(carries))
+
+        def call(scratch, nbytes, on):
+            return _native.scan(spec.dtype, spec.offsets_dtype, d, n, b, pointers, scratch, nbytes, self._flags, on)
+
+        return self._launch(torch, offsets, n, b, stream, mode, [t[1] for t in tensors] + [offsets],
+                            [(self._scratch(n, b), call)])
+
+    def run_backward(self, values, gates, offsets, carries, grad_out, stream=None, *, initial=None, grad_final=None,
+                     grad_values=None, grad_gates=None, grad_initial=None) -> ExecutionReport:
+        """Gradients of a ``run`` that recorded ``carries``, from those of its
+        outputs (``grad_final`` f32 [B, D]; None: zero).  Writes those of
+        ``grad_values``, ``grad_gates`` [N, D] and ``grad_initial`` (f32
+        [B, D], with ``initial``) that are given."""
+        torch = _torch()
+        spec, d = self.spec, self.spec.feature_dim
+        b, n = self._segments(torch, offsets), self._rows(values, torch)
+        dtype = torch.float32 if spec.dtype == "f32" else torch.bfloat16
+        if grad_initial is not None and initial is None:
+            raise ValidationError("grad_initial needs initial")
+        rows = [("values", values, (n, d), dtype), ("gates", gates, (n, d), dtype),
+                ("carries", carries, (self.carry_rows(n), d), torch.float32), ("grad_out", grad_out, (n, d), dtype),
+                ("initial", initial, (b, d), torch.float32), ("grad_final", grad_final, (b, d), torch.float32),
+                ("grad_values", grad_values, (n, d), dtype), ("grad_gates", grad_gates, (n, d), dtype),
+                ("grad_initial", grad_initial, (b, d), torch.float32)]
+        tensors = rows[:4] + [row for row in rows[4:] if row[1] is not None]
+        self._tensors(torch, tensors, offsets, "validated", False)
+        pointers = (values.data_ptr(), gates.data_ptr(), offsets.data_ptr(), _address(initial), carries.data_ptr(),
+                    grad_out.data_ptr(), _address(grad_final), _address(grad_values), _address(grad_gates),
+                    _address(grad_initial))
+
+        def call(scratch, nbytes, on):
+            return _native.scan_backward(spec.dtype, spec.offsets_dtype, d, n, b, pointers, scratch, nbytes,
+                                         self._flags, on)
+
+        return self._launch(torch, offsets, n, b, stream, "validated", [t[1] for t in tensors] + [offsets],
+                            [(self._scratch(n, b), call)])
+
+
+class CompiledMatmul(_LayerProgram):
+    """out[t] = values[t] @ weights[s] for the rows t of segment s."""
+
+    kind = MatmulSpec

@@ -20,6 +20,7 @@ from .errors import ValidationError
 from .optimizations import Optimizations
 
 DIALECT_VERSION = "1"
+MAX_LAYER_DIM = 65536  # widest rows of the learned operators
 
 
 @dataclass(frozen=True)
@@ -152,6 +153,97 @@ class ProgramSpec:
     @property
     def ir_hash(self) -> str:
         return hashlib.sha256(self.canonical_source().encode()).hexdigest()
+
+
+class _LayerSpec:
+    """What the specifications of the learned operators share."""
+
+    def _check(self) -> None:
+        if self.dtype not in ("f32", "bf16"):
+            raise ValidationError("dtype must be f32 or bf16; accumulation is always f32")
+        if self.offsets_dtype not in ("i32", "i64"):
+            raise ValidationError("offsets_dtype must be i32 or i64")
+        if not isinstance(self.hints, Hints):
+            raise ValidationError("hints must be Hints")
+        if self.chip not in CHIPS:
+            raise ValidationError("chip must be sm_100a")
+
+    def _check_dim(self, name: str) -> None:
+        value = getattr(self, name)
+        if type(value) is not int or not 1 <= value <= MAX_LAYER_DIM:
+            raise ValidationError(f"{name} must be a static integer in [1, {MAX_LAYER_DIM}]")
+
+    def to_dict(self) -> dict[str, Any]:
+        return asdict(self)
+
+    @classmethod
+    def from_dict(cls, data: dict[str, Any]):
+        data = dict(data)
+        if data.pop("op", cls.op) != cls.op:
+            raise ValidationError(f"not the description of a {cls.op} program")
+        data["hints"] = Hints(**data.get("hints", {}))
+        return cls(**data)
+
+    def canonical_source(self) -> str:
+        """Stable text naming this specialization (the input of ``ir_hash``)."""
+        return canonical_json({"dialect": DIALECT_VERSION, "spec": self.to_dict()})
+
+    @property
+    def ir_hash(self) -> str:
+        return hashlib.sha256(self.canonical_source().encode()).hexdigest()
+
+
+@dataclass(frozen=True)
+class ScanSpec(_LayerSpec):
+    """A gated linear recurrence over segments, out[t] = gates[t] * out[t - 1]
+    + values[t], over ``feature_dim`` columns.  ``hints`` bound the segment
+    lengths that checked mode accepts; ``vectorize=False`` is for views that
+    are not 16-byte aligned."""
+
+    dtype: str = "f32"
+    feature_dim: int = 128
+    offsets_dtype: str = "i64"
+    hints: Hints = field(default_factory=Hints)
+    vectorize: bool = True
+    chip: str = DEFAULT_CHIP
+    op: str = field(default="scan", init=False)
+
+    def __post_init__(self) -> None:
+        self._check()
+        self._check_dim("feature_dim")
+        if type(self.vectorize) is not bool:
+            raise ValidationError("vectorize must be bool")
+
+    @property
+    def signature(self) -> str:
+        return f"{self.op}:{self.dtype}:D{self.feature_dim}:{self.offsets_dtype}:{self.chip}"
+
+
+@dataclass(frozen=True)
+class MatmulSpec(_LayerSpec):
+    """A matrix product per segment: the rows of segment s times weights[s],
+    ``feature_dim`` columns in and ``out_dim`` columns out.  ``hints`` bound
+    the segment lengths that checked mode accepts."""
+
+    dtype: str = "f32"
+    feature_dim: int = 128
+    out_dim: int = 128
+    offsets_dtype: str = "i64"
+    hints: Hints = field(default_factory=Hints)
+    chip: str = DEFAULT_CHIP
+    op: str = field(default="matmul", init=False)
+
+    def __post_init__(self) -> None:
+        self._check()
+        self._check_dim("feature_dim")
+        self._check_dim("out_dim")
+
+    @property
+    def signature(self) -> str:
+        return f"{self.op}:{self.dtype}:D{self.feature_dim}x{self.out_dim}:{self.offsets_dtype}:{self.chip}"
+
+
+SPECS = (ProgramSpec, ScanSpec, MatmulSpec)
 
 
 @dataclass(frozen=True)

@@ -1,4 +1,4 @@
-"""torch integration: two custom operators over compiled programs, and NJT helpers.
+"""torch integration: custom operators over compiled programs, and NJT helpers.
 
 Importing ``ragged`` never imports torch; ``register_torch_ops()`` defines
 the operators once per process.  Their names and schemas are the
@@ -26,6 +26,7 @@ import threading
 from typing import Any
 
 from .errors import ValidationError
+from .layers import CompiledScan, scan_chunk_rows
 from .runtime import CompiledProgram, _torch
 
 MODES = ("validated", "checked")
@@ -35,6 +36,13 @@ SCHEMAS = {
                       'str mode="validated") -> Tensor',
     "segment_softmax": 'segment_softmax(Tensor values, Tensor offsets, str program, str mode="validated", '
                        'Tensor? mask=None) -> Tensor',
+    # The learned operators (no counterpart in the reference).  `record` keeps
+    # the states that the backward operator needs.
+    "segment_scan": 'segment_scan(Tensor values, Tensor gates, Tensor offsets, Tensor? initial, str program, '
+                    'str mode="validated", bool record=True) -> (Tensor, Tensor, Tensor)',
+    "segment_scan_backward": 'segment_scan_backward(Tensor values, Tensor gates, Tensor offsets, Tensor? initial, '
+                             'Tensor carries, Tensor grad_out, Tensor? grad_final, str program) '
+                             '-> (Tensor, Tensor, Tensor)',
 }
 
 
@@ -46,12 +54,19 @@ class ProgramTable:
         self._programs: dict[str, CompiledProgram] = {}
 
     def enter(self, program) -> str:
-        if program.spec.alias != "none":
+        if getattr(program.spec, "alias", "none") != "none":
             raise ValidationError("functional custom ops require an out-of-place specialization")
         token = program.artifact.key.digest
         with self._lock:
             self._programs[token] = program
         return token
+
+    def vectorizes(self, token: str) -> bool:
+        """Whether the scan program of ``token`` moves full vectors (a token
+        that is not registered, while tracing shapes: yes)."""
+        with self._lock:
+            program = self._programs.get(token)
+        return program is None or getattr(program.spec, "vectorize", True)
 
     def lookup(self, token: str, op: str):
         with self._lock:
@@ -121,6 +136,28 @@ class OpContract:
             raise ValidationError("autograd is outside the supported forward-only contract")
 
 
+    def scan(self, values, gates, offsets, initial) -> None:
+        self.inputs_of("scan", values, offsets)
+        if gates.shape != values.shape or gates.dtype != values.dtype or gates.device != values.device:
+            raise ValidationError("gates must have the shape, dtype and device of values")
+        if initial is not None and (tuple(initial.shape) != (offsets.shape[0] - 1, values.shape[1])
+                                    or initial.dtype != self.torch.float32 or initial.device != values.device):
+            raise ValidationError("initial must be f32 [B, D] on the values device")
+
+    def inputs_of(self, op: str, values, offsets) -> None:
+        """What the learned operators ask of values and offsets."""
+        torch = self.torch
+        if values.ndim != 2 or offsets.ndim != 1:
+            raise ValidationError("expected values[N,D] and offsets[B+1]")
+        torch._check(offsets.shape[0] >= 1)
+        if values.dtype not in (torch.float32, torch.bfloat16):
+            raise ValidationError("values must be f32 or bf16")
+        if offsets.dtype not in (torch.int32, torch.int64):
+            raise ValidationError("offsets must be i32 or i64")
+        if values.device != offsets.device:
+            raise ValidationError("values and offsets must use the same device")
+
+
 def output_shape(op: str, values, offsets) -> tuple:
     """[B, D] for sum and max, [N, D] for softmax."""
     rows = values.shape[0] if op == "softmax" else offsets.shape[0] - 1
@@ -145,9 +182,105 @@ def _call(values, offsets, token: str, op: str, mode: str, mask=None):
     return output
 
 
+def _dense(*tensors):
+    """The tensors, contiguous: a gradient arrives in whatever layout autograd
+    made of it (an expanded sum, a transposed view)."""
+    return tuple(t.contiguous() if t is not None else None for t in tensors)
+
+
+def _scan_shapes(values, offsets, rows: int, record: bool) -> tuple:
+    """Shapes of out, final and carries."""
+    n, d = values.shape
+    return (n, d), (offsets.shape[0] - 1, d), ((n + rows - 1) // rows if record else 0, d)
+
+
+def _scan_call(values, gates, offsets, initial, token: str, mode: str, record: bool):
+    """The real kernel of segment_scan."""
+    torch = _torch()
+    program = _table.lookup(token, "scan")
+    values, gates, initial = _dense(values, gates, initial)
+    out = torch.empty_like(values)
+    state = dict(dtype=torch.float32, device=values.device)
+    final = torch.empty((offsets.shape[0] - 1, values.shape[1]), **state)
+    carries = torch.empty((program.carry_rows(values.shape[0]) if record else 0, values.shape[1]), **state)
+    program._run(values, gates, offsets, out, initial, final, carries if record else None, None, mode, False)
+    return out, final, carries
+
+
+def _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final, token: str):
+    """The real kernel of segment_scan_backward."""
+    torch = _torch()
+    program = _table.lookup(token, "scan")
+    values, gates, initial, grad_out, grad_final = _dense(values, gates, initial, grad_out, grad_final)
+    grad_values, grad_gates = torch.empty_like(values), torch.empty_like(values)
+    grad_initial = torch.empty_like(initial) if initial is not None else carries.new_empty((0,))
+    program.run_backward(values, gates, offsets, carries, grad_out, initial=initial, grad_final=grad_final,
+                         grad_values=grad_values, grad_gates=grad_gates,
+                         grad_initial=grad_initial if initial is not None else None)
+    return grad_values, grad_gates, grad_initial
+
+
+def _first_derivative(torch) -> None:
+    if torch.is_grad_enabled():
+        raise ValidationError("second derivatives are not supported (create_graph)")
+
+
+def _register_scan(torch, library, contract) -> None:
+    def scan_kernel(values, gates, offsets, initial, program, mode="validated", record=True):
+        return _scan_call(values, gates, offsets, initial, program, mode, record)
+
+    def scan_backward_kernel(values, gates, offsets, initial, carries, grad_out, grad_final, program):
+        return _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final, program)
+
+    for key in ("CPU", "CUDA"):
+        library.impl("segment_scan", scan_kernel, key)
+        library.impl("segment_scan_backward", scan_backward_kernel, key)
+
+    @torch.library.register_fake("ragged_mlir::segment_scan", lib=library)
+    def scan_fake(values, gates, offsets, initial, program, mode="validated", record=True):
+        contract.mode(mode)
+        contract.scan(values, gates, offsets, initial)
+        dtype = "f32" if values.dtype == torch.float32 else "bf16"
+        rows = scan_chunk_rows(dtype, int(values.shape[1]), _table.vectorizes(program))
+        out, final, carries = _scan_shapes(values, offsets, rows, record)
+        state = dict(dtype=torch.float32, device=values.device)
+        return (torch.empty(out, dtype=values.dtype, device=values.device), torch.empty(final, **state),
+                torch.empty(carries, **state))
+
+    @torch.library.register_fake("ragged_mlir::segment_scan_backward", lib=library)
+    def scan_backward_fake(values, gates, offsets, initial, carries, grad_out, grad_final, program):
+        grad = torch.empty(values.shape, dtype=values.dtype, device=values.device)
+        state = torch.empty(initial.shape if initial is not None else (0,), dtype=torch.float32, device=values.device)
+        return grad, torch.empty_like(grad), state
+
+    def setup(ctx, inputs, output):
+        values, gates, offsets, initial, program, _, record = inputs
+        ctx.record, ctx.program, ctx.has_initial = record, program, initial is not None
+        ctx.save_for_backward(values, gates, offsets, output[2], *([initial] if initial is not None else []))
+        ctx.mark_non_differentiable(output[2])
+        ctx.set_materialize_grads(False)
+
+    def backward(ctx, grad_out, grad_final, _):
+        if not ctx.record:
+            raise ValidationError("the scan recorded no states (record=False): it has no backward pass")
+        _first_derivative(torch)
+        if grad_out is None and grad_final is None:
+            return (None,) * 7
+        values, gates, offsets, carries, *initial = ctx.saved_tensors
+        if grad_out is None:
+            grad_out = torch.zeros_like(values)
+        grads = torch.ops.ragged_mlir.segment_scan_backward(
+            values, gates, offsets, initial[0] if ctx.has_initial else None, carries, grad_out, grad_final,
+            ctx.program)
+        return grads[0], grads[1], None, grads[2] if ctx.has_initial else None, None, None, None
+
+    torch.library.register_autograd("ragged_mlir::segment_scan", backward, setup_context=setup, lib=library)
+
+
 def register_torch_ops() -> dict[str, Any]:
-    """Define ``ragged_mlir::segment_reduce`` / ``segment_softmax`` (once);
-    returns {"segment_reduce": op, "segment_softmax": op}."""
+    """Define the ``ragged_mlir`` operators (once); returns name -> operator of
+    segment_reduce and segment_softmax, as the reference's function does
+    (``torch.ops.ragged_mlir`` holds them all)."""
     global _library
     with _define_lock:
         if _operators:
@@ -183,6 +316,7 @@ def register_torch_ops() -> dict[str, Any]:
             contract.mask(values, mask)
             return values.new_empty(output_shape("softmax", values, offsets))
 
+        _register_scan(torch, library, contract)
         _library = library
         namespace = torch.ops.ragged_mlir
         _operators.update(segment_reduce=namespace.segment_reduce, segment_softmax=namespace.segment_softmax)
@@ -198,6 +332,23 @@ def segment_softmax(values, offsets, *, program: CompiledProgram, mode: str = "v
     """Segmented softmax of ``program`` through the custom operator."""
     _mask_presence(program, mask)
     return register_torch_ops()["segment_softmax"](values, offsets, register_program(program), mode, mask)
+
+
+def segment_scan(values, gates, offsets, *, program: CompiledScan, initial=None, mode: str = "validated"):
+    """(out [N, D], final f32 [B, D]) of the recurrence out[t] = gates[t] *
+    out[t - 1] + values[t] within each segment, differentiable (once) in
+    values, gates and initial.
+
+    Under a CUDA graph capture of a backward pass, autograd itself must not
+    have an eager graph of the same leaves alive: its accumulation nodes stay
+    on the stream they were first used on, and the capture fails.  Take the
+    gradients with ``torch.autograd.grad``, or drop earlier graphs first."""
+    torch = _torch()
+    register_torch_ops()
+    record = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (values, gates, initial))
+    out, final, _ = torch.ops.ragged_mlir.segment_scan(values, gates, offsets, initial, register_program(program),
+                                                       mode, record)
+    return out, final
 
 
 def bind(program: CompiledProgram, *, mode: str = "validated"):
@@ -242,6 +393,17 @@ def njt_reduce(nt, kind: str, *, program: CompiledProgram, mode: str = "validate
     """Segmented sum or max over the ragged dimension of an NJT: [B, D]."""
     values, offsets = jagged_components(nt)
     return segment_reduce(values, offsets, kind, program=program, mode=mode)
+
+
+def njt_scan(nt, gates, *, program: CompiledScan, initial=None, mode: str = "validated"):
+    """(NJT of the outputs, final) of ``segment_scan`` over the ragged
+    dimension of an NJT; ``gates`` is an NJT on the same offsets."""
+    values, offsets = jagged_components(nt)
+    gate_values, gate_offsets = jagged_components(gates)
+    if gate_offsets is not offsets and gate_offsets.data_ptr() != offsets.data_ptr():
+        raise ValidationError("gates must share the offsets of the values")
+    out, final = segment_scan(values, gate_values, offsets, program=program, initial=initial, mode=mode)
+    return _torch().nested.nested_tensor_from_jagged(out, offsets=offsets), final
 
 
 def njt_softmax(nt, *, program: CompiledProgram, mode: str = "validated", mask=None):
