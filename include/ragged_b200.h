@@ -279,22 +279,21 @@ int rg_run_noalloc(int op, int dtype, int index_dtype, int64_t d, int64_t n, int
  * always does).
  *
  * rg_scan_workspace_bytes gives the scratch of either call (256-byte aligned;
- * 0: none) and carry_rows, the rows of `carries` (f32 [carry_rows, D]): the
- * states that rg_scan records for rg_scan_backward, NULL if no backward pass
+ * 0: none).  carries (f32 [ceil(N / 16), D]) receives
+ * the state before every 16th row for rg_scan_backward, NULL if no backward pass
  * follows.  rg_scan_backward takes the forward call's inputs and carries and
  * the gradients of out and final_state (NULL: zero) and writes the gradients
  * that are not NULL; grad_initial (f32 [B, D]) needs `initial`.  Written
- * tensors overlap nothing.  flags: RG_FLAG_NO_VECTORIZE, the same for both
- * passes.  Results do not depend on timing: equal inputs give equal bits. */
-int rg_scan_workspace_bytes(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, uint32_t flags,
-                            int64_t *bytes, int64_t *carry_rows);
+ * tensors overlap nothing.  Results do not depend on timing: equal inputs give
+ * equal bits. */
+int rg_scan_workspace_bytes(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, int64_t *bytes);
 int rg_scan(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, const void *values, const void *gates,
             const void *offsets, const float *initial, void *out, float *final_state, float *carries,
-            void *workspace, int64_t workspace_bytes, uint32_t flags, void *stream, rg_report *report);
+            void *workspace, int64_t workspace_bytes, void *stream, rg_report *report);
 int rg_scan_backward(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, const void *values,
                      const void *gates, const void *offsets, const float *initial, const float *carries,
                      const void *grad_out, const float *grad_final, void *grad_values, void *grad_gates,
-                     float *grad_initial, void *workspace, int64_t workspace_bytes, uint32_t flags, void *stream,
+                     float *grad_initial, void *workspace, int64_t workspace_bytes, void *stream,
                      rg_report *report);
 
 /* ------------------------------------------------------- schedule choice

@@ -1,6 +1,7 @@
 // Host-side types shared by the launcher and the per-schedule launch code.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -59,6 +60,9 @@ enum KernelId : int {
   K_POINTWISE_CAST = 13,
   K_SCAN = 14,
   K_SCAN_BACKWARD = 15,
+  K_SCAN_FOLD = 16,
+  K_SCAN_FOLD_BACKWARD = 17,
+  K_SCAN_JOIN = 18,
 };
 
 // Recording helper for rg_report.
@@ -74,6 +78,15 @@ Geometry make_geometry(const Problem &p);
 int device_props(DeviceProps *props);  // current device
 int validate(const Problem &p);           // argument checks of rg_run
 int check_device(DeviceProps *props);     // current device must be sm_100
+// Allows `kernel` up to `smem_limit` bytes of dynamic shared memory on the
+// current device, once, and gives the CTAs of `threads` with `smem` bytes that
+// an SM holds (cached per kernel and device).
+int prepare_kernel(const void *kernel, int device, int threads, int smem, int smem_limit, int *per_sm);
+// Tensor map of `rows` rows of `cols` elements (16-byte aligned rows), loaded
+// in boxes; with `swizzle` a box is 128 bytes wide and its 16-byte pieces are
+// permuted within groups of 8 rows as tcgen05's 128-byte swizzle expects.
+int make_tensor_map_2d(CUtensorMap *map, int dtype, const void *base, int64_t rows, int64_t cols, int box_rows,
+                       int box_cols, bool swizzle);
 
 // Per-schedule entry points (launch on stream, record into report).
 int launch_naive(const Problem &p, const Geometry &g, cudaStream_t stream, rg_report *report);

@@ -1,6 +1,7 @@
 // The C ABI (include/ragged_b200.h): argument validation, device queries,
 // geometry, workspace sizing and schedule dispatch.  No exception crosses
 // the boundary; every entry point returns an rg_status.
+#include <atomic>
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
@@ -17,6 +18,14 @@ thread_local std::string g_last_error;
 
 std::mutex g_device_mutex;
 std::vector<DeviceProps> g_devices;  // by ordinal; sm_count == 0 means "not queried"
+
+struct PreparedKernel {
+  const void *kernel;
+  int device, per_sm;
+};
+std::mutex g_prepared_mutex;
+PreparedKernel g_prepared[1024];
+int g_prepared_count = 0;
 }  // namespace
 
 int fail(int status, const std::string &message) {
@@ -88,6 +97,59 @@ int device_props(DeviceProps *props) {
     d.max_threads_per_sm = prop.maxThreadsPerMultiProcessor;
   }
   *props = d;
+  return RG_OK;
+}
+
+int prepare_kernel(const void *kernel, int device, int threads, int smem, int smem_limit, int *per_sm) {
+  std::lock_guard<std::mutex> lock(g_prepared_mutex);
+  for (int i = 0; i < g_prepared_count; ++i) {
+    if (g_prepared[i].kernel == kernel && g_prepared[i].device == device) {
+      *per_sm = g_prepared[i].per_sm;
+      return RG_OK;
+    }
+  }
+  int status = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_limit),
+                          "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
+  if (status) return status;
+  int blocks = 0;
+  status = check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, threads, smem),
+                      "cudaOccupancyMaxActiveBlocksPerMultiprocessor");
+  if (status) return status;
+  if (blocks < 1) return fail(RG_ERR_DEVICE, "a kernel does not fit on this device");
+  if (g_prepared_count < 1024) g_prepared[g_prepared_count++] = {kernel, device, blocks};
+  *per_sm = blocks;
+  return RG_OK;
+}
+
+int make_tensor_map_2d(CUtensorMap *map, int dtype, const void *base, int64_t rows, int64_t cols, int box_rows,
+                       int box_cols, bool swizzle) {
+  using Encode = decltype(&cuTensorMapEncodeTiled);
+  static std::atomic<void *> cached{nullptr};
+  void *entry = cached.load();
+  if (!entry) {
+    cudaDriverEntryPointQueryResult found;
+    const int status = check_cuda(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000,
+                                                                   cudaEnableDefault, &found),
+                                  "cudaGetDriverEntryPointByVersion(cuTensorMapEncodeTiled)");
+    if (status) return status;
+    if (found != cudaDriverEntryPointSuccess || !entry)
+      return fail(RG_ERR_DEVICE, "the CUDA driver has no cuTensorMapEncodeTiled");
+    cached.store(entry);
+  }
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols * elem_bytes(dtype))};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t steps[2] = {1, 1};
+  const CUresult result = reinterpret_cast<Encode>(entry)(
+      map, dtype == RG_DTYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+      const_cast<void *>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (result != CUDA_SUCCESS) {
+    char buffer[96];
+    std::snprintf(buffer, sizeof buffer, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(result));
+    return fail(RG_ERR_CUDA, buffer);
+  }
   return RG_OK;
 }
 
@@ -212,6 +274,9 @@ const char *rg_kernel_name(int kernel_id) {
     case K_POINTWISE_CAST: return "pointwise_cast";
     case K_SCAN: return "scan";
     case K_SCAN_BACKWARD: return "scan_backward";
+    case K_SCAN_FOLD: return "scan_fold";
+    case K_SCAN_FOLD_BACKWARD: return "scan_fold_backward";
+    case K_SCAN_JOIN: return "scan_join";
   }
   return "";
 }

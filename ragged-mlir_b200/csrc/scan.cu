@@ -1,4 +1,5 @@
 // Launch code of the segmented scan (kernels and mathematics: scan.cuh).
+#include <algorithm>
 #include <cstdio>
 #include <cstring>
 
@@ -15,50 +16,41 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
 struct ScanShape {
-  int vec, shift, tiles, rows;
-  int64_t chunks, groups, supers, blocks;
+  int pair;            // elements of 4 bytes of a row (1 where D is odd)
+  int vec;             // of this call: 1 where a tensor is not aligned for pairs
+  int shift, lane_rows, row_shift, tiles;
+  int64_t slabs, blocks;
 };
 
-// Column vectors of up to 16 bytes that divide D; a tile of at most 128 bytes
-// and 32 lanes of them; the rest of the CTA's threads are row groups.
-ScanShape make_shape(int dtype, int64_t d, int64_t n, int64_t b, uint32_t flags) {
-  const int esize = elem_bytes(dtype);
+constexpr int64_t kAloneRows = 256;  // rows up to which walk is the only launch
+
+// 32 lanes, or as many as cover a row, of one vector each.  A lane takes 64
+// rows of a slab where that leaves the GPU's warps two tasks each, and 16 where
+// there are fewer.
+ScanShape make_shape(int dtype, int64_t d, int64_t n, int64_t b, bool aligned_pairs) {
   ScanShape s;
-  s.vec = 1;
-  if (!(flags & RG_FLAG_NO_VECTORIZE))
-    while (2 * s.vec * esize <= 16 && d % (2 * s.vec) == 0) s.vec *= 2;
-  const int64_t cols = d / s.vec;
+  s.pair = dtype == RG_DTYPE_BF16 && d % 2 == 0 ? 2 : 1;
+  s.vec = aligned_pairs ? s.pair : 1;
   s.shift = 0;
-  while ((1 << s.shift) < cols && s.shift < 5 && (2 << s.shift) * s.vec * esize <= 128) ++s.shift;
-  s.tiles = static_cast<int>(ceil_div(cols, int64_t{1} << s.shift));
-  s.rows = (kScanThreads >> s.shift) * scan_rows(esize, s.vec);
-  s.chunks = ceil_div(n, s.rows);
-  s.groups = ceil_div(s.chunks, kScanFan);
-  s.supers = ceil_div(s.groups, kScanFan);
-  // Empty segments are shared out over the CTAs; 4096 of them keep one busy.
-  s.blocks = s.chunks;
-  if (s.blocks < ceil_div(b, 4096)) s.blocks = ceil_div(b, 4096);
+  while ((int64_t{1} << s.shift) * s.vec < d && s.shift < 5) ++s.shift;
+  s.tiles = static_cast<int>(ceil_div(d, (int64_t{1} << s.shift) * s.vec));
+  const int groups = 32 >> s.shift;
+  constexpr int64_t warps = 148 * 24;
+  s.lane_rows = 64;
+  while (s.lane_rows > 16 && (ceil_div(n, s.lane_rows * groups) * s.tiles < 2 * warps || s.lane_rows * groups > 512))
+    s.lane_rows /= 2;
+  s.row_shift = 0;
+  while ((1 << s.row_shift) < s.lane_rows * groups) ++s.row_shift;
+  s.slabs = ceil_div(n, int64_t{1} << s.row_shift);
+  // Empty segments are shared out over the tasks; 1024 of them keep one busy.
+  s.blocks = s.slabs;
+  if (s.blocks < ceil_div(b, 1024)) s.blocks = ceil_div(b, 1024);
   if (s.blocks < 1) s.blocks = 1;
   return s;
 }
 
-struct ScanLayout {
-  int64_t flags, pairs, supers, bytes, cleared;
-};
-
-// Status word at 0, ticket at 8, then flags (cleared before each call), pairs
-// and supergroup states.  A single chunk waits for nothing and needs none.
-ScanLayout make_layout(const ScanShape &s) {
-  ScanLayout l{};
-  if (s.chunks <= 1) return l;
-  const int64_t slots = static_cast<int64_t>(s.tiles) * 2;
-  l.flags = 256;
-  l.cleared = align256(l.flags + (s.chunks + s.groups + s.supers) * slots * 4);
-  l.pairs = l.cleared;
-  l.supers = align256(l.pairs + (s.chunks + s.groups) * s.tiles * kScanCols * 8);
-  l.bytes = align256(l.supers + s.supers * s.tiles * kScanCols * 4);
-  return l;
-}
+// Pairs, then states of each slab.
+int64_t layout_bytes(const ScanShape &s, int64_t n, int64_t d) { return n <= kAloneRows ? 0 : align256(s.slabs * d * 12); }
 
 int check_shape(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b) {
   if (dtype != RG_DTYPE_F32 && dtype != RG_DTYPE_BF16) return fail(RG_ERR_INVALID_ARGUMENT, "dtype must be f32 or bf16");
@@ -110,62 +102,77 @@ int check_ranges(const Range *r, int count) {
   return RG_OK;
 }
 
+// Whether the tensors' alignment (of one element, in `r`) allows pairs.
+bool pairs_aligned(const Range *r, int count) {
+  for (int i = 0; i < count; ++i)
+    if (std::strcmp(r[i].name, "offsets") && r[i].bytes && !aligned(r[i].ptr, r[i].align * 2)) return false;
+  return true;
+}
+
 template <typename T, typename OffT, int VEC, bool BACKWARD>
-int launch(const ScanArgs &p, const ScanShape &s, cudaStream_t stream, rg_report *report) {
-  const int smem = 2 * (s.rows + 1) * 4;
-  const dim3 grid(static_cast<unsigned>(s.blocks * s.tiles), 1, 1);
-  scan_kernel<T, OffT, VEC, BACKWARD><<<grid, kScanThreads, smem, stream>>>(p);
-  record_launch(report, BACKWARD ? K_SCAN_BACKWARD : K_SCAN, grid, kScanThreads, smem);
-  return check_cuda(cudaGetLastError(), "scan_kernel launch");
+int launch(const ScanArgs &p, const ScanShape &s, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
+  const int smem = kScanWarps * scan_marks_words(1 << s.row_shift) * 4;
+  constexpr int usual = kScanWarps * scan_marks_words(64) * 4, limit = kScanWarps * scan_marks_words(512) * 4;
+  auto run = [&](void (*kernel)(ScanArgs), int id, int64_t tasks) {
+    int per_sm = 0;
+    int status = prepare_kernel(reinterpret_cast<const void *>(kernel), dev.device, kScanThreads, usual, limit, &per_sm);
+    if (status) return status;
+    const int64_t ctas = std::min(static_cast<int64_t>(per_sm) * dev.sm_count, ceil_div(tasks, kScanWarps));
+    const dim3 grid(static_cast<unsigned>(ctas), 1, 1);
+    kernel<<<grid, kScanThreads, smem, stream>>>(p);
+    record_launch(report, id, grid, kScanThreads, smem);
+    return check_cuda(cudaGetLastError(), "scan kernel launch");
+  };
+  if (p.pairs) {
+    int status = run(scan_fold_kernel<T, OffT, VEC, BACKWARD>, BACKWARD ? K_SCAN_FOLD_BACKWARD : K_SCAN_FOLD,
+                     s.slabs * s.tiles);
+    if (status) return status;
+    const dim3 grid(static_cast<unsigned>(ceil_div(p.d, 32)), 1, 1);
+    scan_join_kernel<<<grid, kScanJoinWarps * 32, 0, stream>>>(p);
+    record_launch(report, K_SCAN_JOIN, grid, kScanJoinWarps * 32, 0);
+    status = check_cuda(cudaGetLastError(), "scan_join_kernel launch");
+    if (status) return status;
+  }
+  return run(scan_walk_kernel<T, OffT, VEC, BACKWARD>, BACKWARD ? K_SCAN_BACKWARD : K_SCAN, s.blocks * s.tiles);
 }
 
 template <typename OffT, bool BACKWARD>
-int launch_vec(int dtype, const ScanArgs &p, const ScanShape &s, cudaStream_t stream, rg_report *report) {
-  if (dtype == RG_DTYPE_F32) {
-    if (s.vec == 4) return launch<float, OffT, 4, BACKWARD>(p, s, stream, report);
-    if (s.vec == 2) return launch<float, OffT, 2, BACKWARD>(p, s, stream, report);
-    return launch<float, OffT, 1, BACKWARD>(p, s, stream, report);
-  }
-  if (s.vec == 8) return launch<__nv_bfloat16, OffT, 8, BACKWARD>(p, s, stream, report);
-  if (s.vec == 4) return launch<__nv_bfloat16, OffT, 4, BACKWARD>(p, s, stream, report);
-  if (s.vec == 2) return launch<__nv_bfloat16, OffT, 2, BACKWARD>(p, s, stream, report);
-  return launch<__nv_bfloat16, OffT, 1, BACKWARD>(p, s, stream, report);
+int launch_vec(int dtype, const ScanArgs &p, const ScanShape &s, const DeviceProps &dev, cudaStream_t stream,
+               rg_report *report) {
+  if (dtype == RG_DTYPE_F32) return launch<float, OffT, 1, BACKWARD>(p, s, dev, stream, report);
+  if (s.vec == 2) return launch<__nv_bfloat16, OffT, 2, BACKWARD>(p, s, dev, stream, report);
+  return launch<__nv_bfloat16, OffT, 1, BACKWARD>(p, s, dev, stream, report);
 }
 
 template <bool BACKWARD>
-int run_scan(int dtype, int index_dtype, const ScanShape &s, ScanArgs &p, void *workspace, int64_t workspace_bytes,
+int run_scan(int dtype, int index_dtype, bool aligned_pairs, ScanArgs &p, void *workspace, int64_t workspace_bytes,
              cudaStream_t stream, rg_report *report) {
   DeviceProps dev;
   int status = check_device(&dev);
   if (status) return status;
-  if (s.blocks > 2147483647LL / s.tiles) return fail(RG_ERR_INVALID_ARGUMENT, "the call needs more than 2^31 - 1 CTAs");
-  const ScanLayout l = make_layout(s);
+  const ScanShape s = make_shape(dtype, p.d, p.n, p.b, aligned_pairs);
+  if (s.blocks > 2000000000LL / s.tiles) return fail(RG_ERR_INVALID_ARGUMENT, "the call needs more than 2e9 tasks");
+  const int64_t need = layout_bytes(s, p.n, p.d);
   if (report) {
-    report->workspace_bytes = l.bytes;
+    report->workspace_bytes = need;
     report->d_vector = s.vec;
     report->d_tile = 1 << s.shift;
-    report->status_offset = l.bytes ? 0 : -1;
   }
   p.shift = s.shift;
-  p.vec_cols = static_cast<int>(p.d / s.vec);
+  p.lane_rows = s.lane_rows;
+  p.row_shift = s.row_shift;
   p.tiles = s.tiles;
-  p.chunks = s.chunks;
+  p.slabs = s.slabs;
   p.blocks = s.blocks;
-  if (l.bytes) {
-    if (!workspace || workspace_bytes < l.bytes) return fail(RG_ERR_WORKSPACE, "workspace missing or too small");
+  p.per_block = ceil_div(p.b, s.blocks);
+  if (need) {
+    if (!workspace || workspace_bytes < need) return fail(RG_ERR_WORKSPACE, "workspace missing or too small");
     if (!aligned(workspace, 256)) return fail(RG_ERR_WORKSPACE, "workspace must be 256-byte aligned");
-    char *base = static_cast<char *>(workspace);
-    p.status = reinterpret_cast<unsigned long long *>(base);
-    p.ticket = reinterpret_cast<unsigned *>(base + 8);
-    p.flags = reinterpret_cast<unsigned *>(base + l.flags);
-    p.pairs = reinterpret_cast<float2 *>(base + l.pairs);
-    p.supers = reinterpret_cast<float *>(base + l.supers);
-    status = check_cuda(cudaMemsetAsync(base, 0, l.cleared, stream), "cudaMemsetAsync");
-    if (status) return status;
-    if (report) ++report->memsets;
+    p.pairs = static_cast<float2 *>(workspace);
+    p.states = reinterpret_cast<float *>(p.pairs + s.slabs * p.d);
   }
-  if (index_dtype == RG_INDEX_I32) return launch_vec<int32_t, BACKWARD>(dtype, p, s, stream, report);
-  return launch_vec<int64_t, BACKWARD>(dtype, p, s, stream, report);
+  if (index_dtype == RG_INDEX_I32) return launch_vec<int32_t, BACKWARD>(dtype, p, s, dev, stream, report);
+  return launch_vec<int64_t, BACKWARD>(dtype, p, s, dev, stream, report);
 }
 
 void clear_report(rg_report *report) {
@@ -183,37 +190,38 @@ using namespace rgb;
 
 extern "C" {
 
-int rg_scan_workspace_bytes(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, uint32_t flags,
-                            int64_t *bytes, int64_t *carry_rows) {
-  if (!bytes || !carry_rows) return fail(RG_ERR_INVALID_ARGUMENT, "bytes and carry_rows must not be NULL");
+int rg_scan_workspace_bytes(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, int64_t *bytes) {
+  if (!bytes) return fail(RG_ERR_INVALID_ARGUMENT, "bytes is NULL");
   const int status = check_shape(dtype, index_dtype, d, n, b);
   if (status) return status;
-  const ScanShape s = make_shape(dtype, d, n, b, flags);
-  *bytes = make_layout(s).bytes;
-  *carry_rows = s.chunks;
+  // The pairs take the same bytes per column, but the tiles and the slabs that
+  // go by them differ with the alignment of the tensors.
+  const int64_t pairs = layout_bytes(make_shape(dtype, d, n, b, true), n, d);
+  const int64_t singles = layout_bytes(make_shape(dtype, d, n, b, false), n, d);
+  *bytes = pairs > singles ? pairs : singles;
   return RG_OK;
 }
 
 int rg_scan(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, const void *values, const void *gates,
             const void *offsets, const float *initial, void *out, float *final_state, float *carries, void *workspace,
-            int64_t workspace_bytes, uint32_t flags, void *stream, rg_report *report) {
+            int64_t workspace_bytes, void *stream, rg_report *report) {
   clear_report(report);
   int status = check_shape(dtype, index_dtype, d, n, b);
   if (status) return status;
   if (b == 0) return RG_OK;
-  const ScanShape s = make_shape(dtype, d, n, b, flags);
-  const int esize = elem_bytes(dtype), vec = s.vec * esize, state = (s.vec < 4 ? s.vec : 4) * 4;
+  const int esize = elem_bytes(dtype);
   const int isize = index_dtype == RG_INDEX_I32 ? 4 : 8;
   const int64_t full = n * d * esize, states = b * d * 4;
-  const Range ranges[] = {{"values", values, full, vec, false},
-                          {"gates", gates, full, vec, false},
+  const Range ranges[] = {{"values", values, full, esize, false},
+                          {"gates", gates, full, esize, false},
                           {"offsets", offsets, (b + 1) * isize, isize, false},
-                          {"initial", initial, initial ? states : 0, state, false},
-                          {"out", out, full, vec, true},
-                          {"final", final_state, final_state ? states : 0, state, true},
-                          {"carries", carries, carries ? s.chunks * d * 4 : 0, 4, true}};
+                          {"initial", initial, initial ? states : 0, 4, false},
+                          {"out", out, full, esize, true},
+                          {"final", final_state, final_state ? states : 0, 4, true},
+                          {"carries", carries, carries ? ceil_div(n, kScanBatch) * d * 4 : 0, 4, true}};
   status = check_ranges(ranges, 7);
   if (status) return status;
+  const bool pairs = pairs_aligned(ranges, 7);
   ScanArgs p{};
   p.values = values;
   p.gates = gates;
@@ -225,35 +233,35 @@ int rg_scan(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, const v
   p.carries = carries;
   p.out = out;
   p.final_state = final_state;
-  return run_scan<false>(dtype, index_dtype, s, p, workspace, workspace_bytes, static_cast<cudaStream_t>(stream), report);
+  return run_scan<false>(dtype, index_dtype, pairs, p, workspace, workspace_bytes, static_cast<cudaStream_t>(stream), report);
 }
 
 int rg_scan_backward(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, const void *values,
                      const void *gates, const void *offsets, const float *initial, const float *carries,
                      const void *grad_out, const float *grad_final, void *grad_values, void *grad_gates,
-                     float *grad_initial, void *workspace, int64_t workspace_bytes, uint32_t flags, void *stream,
+                     float *grad_initial, void *workspace, int64_t workspace_bytes, void *stream,
                      rg_report *report) {
   clear_report(report);
   int status = check_shape(dtype, index_dtype, d, n, b);
   if (status) return status;
   if (b == 0) return RG_OK;
   if (grad_initial && !initial) return fail(RG_ERR_INVALID_ARGUMENT, "grad_initial needs initial");
-  const ScanShape s = make_shape(dtype, d, n, b, flags);
-  const int esize = elem_bytes(dtype), vec = s.vec * esize, state = (s.vec < 4 ? s.vec : 4) * 4;
+  const int esize = elem_bytes(dtype);
   const int isize = index_dtype == RG_INDEX_I32 ? 4 : 8;
   const int64_t full = n * d * esize, states = b * d * 4;
-  const Range ranges[] = {{"values", values, full, vec, false},
-                          {"gates", gates, full, vec, false},
+  const Range ranges[] = {{"values", values, full, esize, false},
+                          {"gates", gates, full, esize, false},
                           {"offsets", offsets, (b + 1) * isize, isize, false},
-                          {"initial", initial, initial ? states : 0, state, false},
-                          {"carries", carries, s.chunks * d * 4, 4, false},
-                          {"grad_out", grad_out, full, vec, false},
-                          {"grad_final", grad_final, grad_final ? states : 0, state, false},
-                          {"grad_values", grad_values, grad_values ? full : 0, vec, true},
-                          {"grad_gates", grad_gates, grad_gates ? full : 0, vec, true},
-                          {"grad_initial", grad_initial, grad_initial ? states : 0, state, true}};
+                          {"initial", initial, initial ? states : 0, 4, false},
+                          {"carries", carries, ceil_div(n, kScanBatch) * d * 4, 4, false},
+                          {"grad_out", grad_out, full, esize, false},
+                          {"grad_final", grad_final, grad_final ? states : 0, 4, false},
+                          {"grad_values", grad_values, grad_values ? full : 0, esize, true},
+                          {"grad_gates", grad_gates, grad_gates ? full : 0, esize, true},
+                          {"grad_initial", grad_initial, grad_initial ? states : 0, 4, true}};
   status = check_ranges(ranges, 10);
   if (status) return status;
+  const bool pairs = pairs_aligned(ranges, 10);
   ScanArgs p{};
   p.values = values;
   p.gates = gates;
@@ -268,7 +276,7 @@ int rg_scan_backward(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b
   p.grad_values = grad_values;
   p.grad_gates = grad_gates;
   p.grad_initial = grad_initial;
-  return run_scan<true>(dtype, index_dtype, s, p, workspace, workspace_bytes, static_cast<cudaStream_t>(stream), report);
+  return run_scan<true>(dtype, index_dtype, pairs, p, workspace, workspace_bytes, static_cast<cudaStream_t>(stream), report);
 }
 
 }  // extern "C"

@@ -8,21 +8,31 @@
 //
 // Both are first-order recurrences, one forward and one backward in t, whose
 // steps compose: rows r..s act on the state before them as H + A * state with
-// A the product of the gates.  A CTA takes a chunk of rows by a tile of at
-// most 128 bytes of columns, keeps its inputs in registers, and
-//   1. folds (A, H) per thread, warp and chunk and publishes the chunk's pair;
-//   2. gets the state before the chunk from the chunks its segment started
-//      in (the start row is known from the offsets, so no flag is read past it);
-//   3. runs the recurrence over its rows from that state and writes them.
-// Every input is read once and every output written once, which is the bound:
-// the recurrence itself is one FMA an element.
+// A the product of the gates.  Work is cut into slabs of rows by tiles of
+// columns, and every task belongs to one warp: 4 bytes of a row a lane (narrow
+// rows: several row groups side by side), down the rows in batches of 16.  No
+// block barrier, no exchange between lanes; warps hide each other's latency.
 //
-// Step 2 folds a fixed tree (chunks of its group of 16, groups of its
-// supergroup of 16, then the state at the last supergroup's end), so the
-// result does not depend on which CTA came first, and the serial chain is one
-// hop per 256 chunks.  Chunks are handed out by a ticket in dependence order:
-// whoever waits waits on CTAs that already run.  Waits are bounded; one that
-// gives up sets the call's status word and goes on.
+//   fold   (A, H) of each slab.  Only the rows past its last segment start
+//          count, and none where its last row ends a segment.
+//   join   column by column over the slabs: the state before each of them.
+//   walk   the recurrence over a slab's rows from the state before them.
+//
+// Three launches in stream order: nothing waits on anything inside a kernel,
+// the order of all sums is fixed, and equal inputs give equal bits.  Device
+// memory is the bound: walk reads every input once and writes every output
+// once; fold reads again what of the inputs belongs to segments that cross
+// slabs, and walk goes through the slabs from the last one back (forward ones
+// in a backward pass), so that it meets first what fold left in L2.  The
+// arithmetic is one FMA an element, about 10 instructions an element in all.
+//
+// Up to 256 rows walk is the only launch: a lane whose rows go on from earlier
+// ones runs the recurrence over those itself.
+//
+// The backward pass needs the states again.  It recomputes 16 rows at a time
+// from values and gates, from the state before them that forward records in
+// f32 (4 bytes for 16 elements; reading `out` would cost as much as reading
+// values does): no rounded state enters a gradient.
 //
 // States, products and sums are f32; results are rounded to the tensor's type
 // once, when they are written.  Segment starts cut the fold by a flag, never
@@ -40,25 +50,23 @@ namespace rgb {
 
 constexpr int kScanThreads = 256;
 constexpr int kScanWarps = kScanThreads / 32;
-constexpr int kScanCols = 64;     // columns of a tile at most
-constexpr int kScanFan = 16;      // chunks per group, groups per supergroup
-constexpr int kScanWaitLimit = 1 << 22;
-
-// Rows a thread keeps in registers: 4 with the full 16-byte vectors, 8 of the
-// narrower ones.
-__host__ __device__ constexpr int scan_rows(int elem_bytes, int vec) { return vec * elem_bytes == 16 ? 4 : 8; }
+constexpr int kScanBatch = 16;    // rows of a lane in flight; rows per recorded state
+constexpr int kScanAhead = 8;     // pairs that a join has on their way
+constexpr int kScanJoinWarps = 32;
 
 struct ScanArgs {
   const void *values, *gates, *offsets;
   const float *initial;  // [B, D] or null
   int64_t n, d;
   int64_t b;
-  int shift;        // log2 of the lanes across a tile's columns
-  int vec_cols;     // D / VEC
-  int tiles;        // column tiles
-  int64_t chunks;   // chunks that hold rows
-  int64_t blocks;   // chunks launched (more than `chunks` where many segments are empty)
-  float *carries;   // [chunks, D] state before each chunk (written by forward, read by backward)
+  int shift;           // log2 of the lanes across a tile's columns
+  int lane_rows;       // rows of a lane: 16, 32 or 64
+  int row_shift;       // log2 of a slab's rows: lane_rows * (32 >> shift)
+  int tiles;           // column tiles
+  int64_t slabs;       // slabs that hold rows
+  int64_t blocks;      // slabs launched (more than `slabs` where many segments are empty)
+  int64_t per_block;   // segments whose emptiness a slab looks at
+  float *carries;      // [N / 16, D] state before every 16th row (written by forward, read by backward)
   // forward
   void *out;
   float *final_state;  // [B, D] or null
@@ -67,52 +75,100 @@ struct ScanArgs {
   const float *grad_final;  // [B, D] or null
   void *grad_values, *grad_gates;
   float *grad_initial;  // [B, D] or null
-  // workspace (null with a single chunk)
-  unsigned *ticket;
-  unsigned long long *status;
-  unsigned *flags;        // chunk, group and supergroup flags
-  float2 *pairs;          // (A, H) of chunks, then of groups
-  float *supers;          // state at each supergroup's end
+  // workspace (null up to 256 rows)
+  float2 *pairs;    // (A, H) of each slab: [slabs][D]; A is NaN-boxed where the pair starts at a segment
+  float *states;    // state before each slab: [slabs][D]
 };
 
 __device__ __forceinline__ float scan_apply(float a, float h, float state) {
   return state == 0.0f ? h : fmaf(a, state, h);
 }
 
-__device__ __forceinline__ void st_release_gpu(unsigned *p, unsigned v) {
-  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
-}
+// In place of A: the pair starts at a segment, and no state before it counts.
+// (A NaN that arithmetic does not make; other NaNs become the usual one.)
+constexpr unsigned kScanReset = 0x7fc05e70u;
 
-// Waits until *flag is set (bounded).
-__device__ __forceinline__ void scan_wait(const unsigned *flag, unsigned long long *status) {
-  for (int i = 0; i < kScanWaitLimit; ++i) {
-    if (ld_acquire_gpu(flag)) return;
-    if (i > 16) __nanosleep(32);
+template <int VEC>
+struct ScanPair {
+  float a[VEC], h[VEC];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      a[v] = 1.0f;
+      h[v] = 0.0f;
+    }
   }
-  atomicMax(status, 1ull);
-}
-
-// Segment starts of a chunk's rows, in shared memory.  start[i]: the segment
-// whose rows begin at row row0 + i (-1: none; of empty segments and the one
-// with rows that share an offset, the last, which has the rows).  ended[i]:
-// one past the segment whose rows end before row row0 + i (INT_MAX: none).
-struct ScanMarks {
-  int *start;
-  int *ended;
-  int last;  // segment of the chunk's last row
+  // This pair after `first`.
+  __device__ __forceinline__ void after(const ScanPair &first) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      h[v] = scan_apply(a[v], h[v], first.h[v]);
+      a[v] *= first.a[v];
+    }
+  }
+  __device__ __forceinline__ void store(float2 *at, bool reset) const {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v)
+      at[v] = make_float2(__uint_as_float(reset ? kScanReset : a[v] != a[v] ? 0x7fffffffu : __float_as_uint(a[v])), h[v]);
+  }
 };
 
-constexpr int kNoEnd = 0x7fffffff;
+// Composition over a warp's row groups (lanes of one group hold one group's
+// columns), in lane order or, REV, from the last group down.  On return `own`
+// describes the groups before the lane's own, `total` all of them.
+template <int VEC, bool REV>
+__device__ __forceinline__ void scan_groups(ScanPair<VEC> &own, int &own_reset, ScanPair<VEC> &total, int &total_reset,
+                                            int shift) {
+  total = own;
+  total_reset = own_reset;
+  if (shift == 5) {  // one group
+    own.clear();
+    own_reset = 0;
+    return;
+  }
+  const int lane = threadIdx.x & 31;
+  const int lanes = 1 << shift;
+  auto from = [&](float x, int off) { return REV ? __shfl_down_sync(~0u, x, off) : __shfl_up_sync(~0u, x, off); };
+  for (int off = lanes; off < 32; off <<= 1) {
+    const bool live = REV ? lane + off < 32 : lane >= off;
+    const int r = REV ? __shfl_down_sync(~0u, total_reset, off) : __shfl_up_sync(~0u, total_reset, off);
+    ScanPair<VEC> first;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      first.a[v] = from(total.a[v], off);
+      first.h[v] = from(total.h[v], off);
+    }
+    if (live && !total_reset) {
+      total.after(first);
+      total_reset = r;
+    }
+  }
+  const bool edge = REV ? lane >= 32 - lanes : lane < lanes;
+  own_reset = REV ? __shfl_down_sync(~0u, total_reset, lanes) : __shfl_up_sync(~0u, total_reset, lanes);
+  if (edge) own_reset = 0;
+  const int last = (REV ? 0 : 32 - lanes) + (lane & (lanes - 1));
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) {
+    const float a = from(total.a[v], lanes), h = from(total.h[v], lanes);
+    own.a[v] = edge ? 1.0f : a;
+    own.h[v] = edge ? 0.0f : h;
+    total.a[v] = __shfl_sync(~0u, total.a[v], last);
+    total.h[v] = __shfl_sync(~0u, total.h[v], last);
+  }
+  total_reset = __shfl_sync(~0u, total_reset, last);
+}
 
-// Segment of row `row` (the last one that starts at or before it), by all
-// threads of the CTA: a 256-way search, one round for up to 256 segments.
+// Segment of row `row` (the last one that starts at or before it), by a warp:
+// a 32-way search.
 template <typename OffT>
 __device__ __forceinline__ int64_t scan_find(const OffT *__restrict__ offsets, int64_t b, int64_t row) {
+  const int lane = threadIdx.x & 31;
   int64_t lo = 0, hi = b;
   while (hi - lo > 1) {
-    const int64_t step = (hi - lo + kScanThreads - 1) / kScanThreads;
-    const int64_t at = lo + threadIdx.x * step;
-    const int count = __syncthreads_count(threadIdx.x == 0 || (at < hi && static_cast<int64_t>(offsets[at]) <= row));
+    const int64_t step = (hi - lo + 31) >> 5;
+    const int64_t at = lo + lane * step;
+    const unsigned below = __ballot_sync(~0u, lane == 0 || (at < hi && static_cast<int64_t>(offsets[at]) <= row));
+    const int count = __popc(below);
     const int64_t next = lo + count * step;
     lo += (count - 1) * step;
     if (next < hi) hi = next;
@@ -120,483 +176,427 @@ __device__ __forceinline__ int64_t scan_find(const OffT *__restrict__ offsets, i
   return lo;
 }
 
-// Fills the marks of rows [row0, row0 + rows]; `first` is the segment of row0.
-// Offsets outside the chunk write nothing, whatever they hold.
-template <typename OffT>
-__device__ __forceinline__ void scan_mark(const OffT *__restrict__ offsets, int64_t b, int64_t first, int64_t row0,
-                                          int rows, int64_t end_row, int *start, int *ended, int *last) {
-  for (int64_t s = first + threadIdx.x; s <= b; s += kScanThreads) {
-    const int64_t at = static_cast<int64_t>(offsets[s]) - row0;
-    if (at > rows) break;
-    if (s == first) {
-      if (at == 0) atomicMax(&start[0], static_cast<int>(s));
-      continue;
-    }
-    if (at < 0) continue;
-    atomicMin(&ended[at], static_cast<int>(s));
-    if (s == b) continue;  // the end of the last segment starts none
-    atomicMax(&start[at], static_cast<int>(s));
-    if (at < end_row - row0) atomicMax(last, static_cast<int>(s));
-  }
-}
-
-// Inclusive-to-exclusive composition over a warp's row groups (lanes of one
-// group hold one group's columns).  REV composes from the last group down.
-// On return a, h, reset describe the groups before this one (after it, REV);
-// the warp's total goes to `total` / `total_reset`.
-template <int VEC, bool REV>
-__device__ __forceinline__ void scan_warp(float (&a)[VEC], float (&h)[VEC], int &reset, int shift, float2 *total,
-                                          int *total_reset) {
-  const int lane = threadIdx.x & 31;
-  const int lanes = 1 << shift;
-  for (int off = lanes; off < 32; off <<= 1) {
-    const bool live = REV ? lane + off < 32 : lane >= off;
-    const int r = REV ? __shfl_down_sync(~0u, reset, off) : __shfl_up_sync(~0u, reset, off);
-    const bool take = live && !reset;
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) {
-      const float pa = REV ? __shfl_down_sync(~0u, a[v], off) : __shfl_up_sync(~0u, a[v], off);
-      const float ph = REV ? __shfl_down_sync(~0u, h[v], off) : __shfl_up_sync(~0u, h[v], off);
-      if (take) {
-        h[v] = scan_apply(a[v], h[v], ph);
-        a[v] *= pa;
-      }
-    }
-    if (take) reset = r;
-  }
-  const bool is_total = REV ? lane < lanes : lane >= 32 - lanes;
-  if (is_total) {
-    const int col = (lane & (lanes - 1)) * VEC;
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) total[col + v] = make_float2(a[v], h[v]);
-    *total_reset = reset;
-  }
-  const bool edge = REV ? lane >= 32 - lanes : lane < lanes;
-  reset = REV ? __shfl_down_sync(~0u, reset, lanes & 31) : __shfl_up_sync(~0u, reset, lanes & 31);
-  if (edge) reset = 0;
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    const float pa = REV ? __shfl_down_sync(~0u, a[v], lanes & 31) : __shfl_up_sync(~0u, a[v], lanes & 31);
-    const float ph = REV ? __shfl_down_sync(~0u, h[v], lanes & 31) : __shfl_up_sync(~0u, h[v], lanes & 31);
-    a[v] = edge ? 1.0f : pa;
-    h[v] = edge ? 0.0f : ph;
-  }
-}
-
-// State before chunk `pos` of this thread's column (threads of the tile's
-// columns only; whole warps).  (a, h, reset) is the chunk's own pair and
-// `first` the chunk in which the segment of the chunk's first row starts
-// (`pos`: the chunk starts with a segment).  Positions count in the order of
-// the recurrence.  Each warp publishes and polls for its own 32 columns.
-__device__ __forceinline__ float scan_lookback(const ScanArgs &p, int tile, int64_t pos, int64_t first, int width,
-                                               float a, float h, bool reset) {
-  const int lane = threadIdx.x & 31;
-  const int warp = threadIdx.x >> 5;
-  const int col = threadIdx.x;
-  const int64_t groups = (p.chunks + kScanFan - 1) / kScanFan;
-  const int64_t slots = static_cast<int64_t>(p.tiles) * 2;
-  unsigned *chunk_flags = p.flags + tile * 2 + warp;
-  unsigned *group_flags = chunk_flags + p.chunks * slots;
-  unsigned *super_flags = group_flags + groups * slots;
-  const int64_t pitch = static_cast<int64_t>(p.tiles) * kScanCols;
-  float2 *chunk_pairs = p.pairs + tile * kScanCols + col;
-  float2 *group_pairs = chunk_pairs + p.chunks * pitch;
-  float *supers = p.supers + tile * kScanCols + col;
-  const bool live = col < width;
-
-  auto publish = [&](unsigned *flag) {
-    __threadfence();
-    __syncwarp();
-    if (lane == 0) st_release_gpu(flag, 1u);
-  };
-
-  if (live) chunk_pairs[pos * pitch] = make_float2(a, h);
-  publish(chunk_flags + pos * slots);
-
-  const int64_t group = pos / kScanFan;
-  float fa = 1.0f, fh = 0.0f;     // the group's chunks before this one
-  bool fixed = first == pos;      // (fa, fh) starts at a segment: no state before it counts
-  if (!fixed) {
-    const int64_t c0 = max(first, group * kScanFan);
-    const int count = static_cast<int>(pos - c0);
-    if (lane < count) scan_wait(chunk_flags + (c0 + lane) * slots, p.status);
-    __syncwarp();
-    float2 part[kScanFan - 1];
-#pragma unroll
-    for (int i = 0; i < kScanFan - 1; ++i)
-      part[i] = i < count && live ? __ldcg(chunk_pairs + (c0 + i) * pitch) : make_float2(1.0f, 0.0f);
-    fixed = c0 == first;
-#pragma unroll
-    for (int i = 0; i < kScanFan - 1; ++i) {
-      if (i < count) {
-        fh = i == 0 ? part[0].y : scan_apply(part[i].x, part[i].y, fh);
-        fa *= part[i].x;
-      }
-    }
-  }
-  if (pos % kScanFan == kScanFan - 1) {
-    // A pair that starts at a segment is read only as the first of a fold or
-    // under a state that a later pair replaces: its A does not matter.
-    if (live) group_pairs[group * pitch] = reset ? make_float2(a, h) : make_float2(fa * a, scan_apply(a, h, fh));
-    publish(group_flags + group * slots);
-  }
-  float state = fh;
-  if (!fixed) {
-    const int64_t super = group / kScanFan, first_group = first / kScanFan;
-    const bool before = first_group < super * kScanFan;  // the segment started before this supergroup
-    const int64_t g0 = max(first_group, super * kScanFan);
-    const int count = static_cast<int>(group - g0);
-    if (lane < count) scan_wait(group_flags + (g0 + lane) * slots, p.status);
-    if (before && lane == 31) scan_wait(super_flags + (super - 1) * slots, p.status);
-    __syncwarp();
-    float2 part[kScanFan - 1];
-#pragma unroll
-    for (int i = 0; i < kScanFan - 1; ++i)
-      part[i] = i < count && live ? __ldcg(group_pairs + (g0 + i) * pitch) : make_float2(1.0f, 0.0f);
-    float s = before && live ? __ldcg(supers + (super - 1) * pitch) : 0.0f;
-#pragma unroll
-    for (int i = 0; i < kScanFan - 1; ++i)
-      if (i < count) s = i == 0 && !before ? part[0].y : scan_apply(part[i].x, part[i].y, s);
-    state = scan_apply(fa, fh, s);
-  }
-  if (pos % (kScanFan * kScanFan) == kScanFan * kScanFan - 1) {
-    if (live) supers[pos / (kScanFan * kScanFan) * pitch] = reset ? h : scan_apply(a, h, state);
-    publish(super_flags + pos / (kScanFan * kScanFan) * slots);
-  }
-  return state;
-}
-
-struct ScanShared {
-  float2 total[kScanWarps][kScanCols];
-  float carry[kScanWarps][kScanCols];  // state before each warp's rows
-  float before[kScanCols];             // backward: the recorded state before the chunk
-  int total_reset[kScanWarps];
-  int last;
-  unsigned ticket;
+// Where segments with rows start and end among a slab's rows: a bit per first
+// row in start_mask and per last row in end_mask, and the segment in start_seg
+// and end_seg (a warp's own shared memory).  Offsets that are out of order set
+// nothing outside the arrays.
+struct ScanMarks {
+  unsigned *start_mask, *end_mask;  // max(rows, 64) / 32 words each
+  int *start_seg, *end_seg;         // rows each
 };
 
-// From the warps' totals: the chunk's pair, the state before it (lookback
-// unless `first` is this chunk) and the state before each warp's rows.  All
-// threads; ends with a barrier.
-template <bool REV>
-__device__ __forceinline__ void scan_chunk(const ScanArgs &p, ScanShared &sh, int tile, int64_t pos, int64_t first,
-                                           int width) {
-  __syncthreads();
-  const int col = threadIdx.x;
-  if (threadIdx.x < ((width + 31) & ~31)) {
-    const bool live = col < width;
-    float state = 0.0f;
-    if (p.ticket) {
-      float a = 1.0f, h = 0.0f;
-      bool reset = false;
-#pragma unroll
-      for (int i = 0; i < kScanWarps; ++i) {
-        const int w = REV ? kScanWarps - 1 - i : i;
-        const float2 t = live ? sh.total[w][col] : make_float2(1.0f, 0.0f);
-        if (sh.total_reset[w]) {
-          h = t.y;
-          reset = true;
-        } else {
-          h = scan_apply(t.x, t.y, h);
-          a *= t.x;
-        }
+template <typename OffT>
+__device__ __forceinline__ void scan_mark(const OffT *__restrict__ offsets, int64_t b, int64_t first, int64_t row0,
+                                          int rows, const ScanMarks &m) {
+  const int lane = threadIdx.x & 31;
+  const int words = (rows < 64 ? 64 : rows) / 32;
+  for (int i = lane; i < 2 * words; i += 32) m.start_mask[i] = 0;
+  __syncwarp();
+  for (int64_t s = first + lane;; s += 32) {
+    const bool there = s < b;
+    const int64_t begin = there ? static_cast<int64_t>(offsets[s]) - row0 : rows;
+    const int64_t end = there ? static_cast<int64_t>(offsets[s + 1]) - 1 - row0 : rows;
+    if (begin < rows && begin <= end) {
+      if (begin >= 0) {
+        m.start_seg[begin] = static_cast<int>(s);
+        atomicOr(&m.start_mask[begin >> 5], 1u << (begin & 31));
       }
-      state = scan_lookback(p, tile, pos, first, width, a, h, reset);
-    }
-    if (live) {
-#pragma unroll
-      for (int i = 0; i < kScanWarps; ++i) {
-        const int w = REV ? kScanWarps - 1 - i : i;
-        sh.carry[w][col] = state;
-        const float2 t = sh.total[w][col];
-        state = sh.total_reset[w] ? t.y : scan_apply(t.x, t.y, state);
+      if (end >= 0 && end < rows) {
+        m.end_seg[end] = static_cast<int>(s);
+        atomicOr(&m.end_mask[end >> 5], 1u << (end & 31));
       }
     }
+    if (__any_sync(~0u, begin >= rows)) break;
   }
-  __syncthreads();
+  __syncwarp();
 }
 
-// Shared memory after ScanShared: start[rows + 1], ended[rows + 1].
+// Words of shared memory of a warp's marks.
+__host__ __device__ constexpr int scan_marks_words(int rows) { return 2 * ((rows < 64 ? 64 : rows) / 32) + 2 * rows; }
+
+// 16 rows of a lane, `d` elements apart; of `count` rows (at least one), the
+// last stands in for those that are missing.
+template <typename T, int VEC>
+__device__ __forceinline__ void scan_rows(const T *__restrict__ at, int64_t d, int count,
+                                          typename VecIO<T, VEC>::Raw (&raw)[kScanBatch]) {
+#pragma unroll
+  for (int i = 0; i < kScanBatch; ++i) {
+    raw[i] = VecIO<T, VEC>::load_raw(at);
+    at += i + 1 < count ? d : 0;
+  }
+}
+
+// What fold and walk share: a warp's place, and its slab's marks.
 template <typename T, typename OffT, int VEC, bool BACKWARD>
-__global__ void __launch_bounds__(kScanThreads, 2) scan_kernel(const ScanArgs p) {
-  constexpr int ROWS = scan_rows(Elem<T>::kBytes, VEC);
+struct ScanWarp {
   using IO = VecIO<T, VEC>;
   using Raw = typename IO::Raw;
-  using State = VecIO<float, VEC < 4 ? VEC : 4>;  // f32 states move in pieces of up to 16 bytes
-  constexpr int kPiece = VEC < 4 ? VEC : 4;
-  __shared__ ScanShared sh;
-  extern __shared__ int scan_smem[];
-  const OffT *__restrict__ offsets = static_cast<const OffT *>(p.offsets);
-  const T *__restrict__ values = static_cast<const T *>(p.values);
-  const T *__restrict__ gates = static_cast<const T *>(p.gates);
+  using State = VecIO<float, VEC>;
+  using Pair = ScanPair<VEC>;
+  const ScanArgs &p;
+  const OffT *__restrict__ offsets;
+  int lanes, rows, words, base;  // base: this lane's first row of a slab
+  int64_t pos, row0, col, seg0;  // slab in the order of the recurrence, its first row, this lane's column
+  bool col_ok;
+  ScanMarks m;
 
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int lanes = 1 << p.shift;
-  const int rows = (kScanThreads >> p.shift) * ROWS;
-  int *start = scan_smem, *ended = scan_smem + rows + 1;
-
-  unsigned task = blockIdx.x;
-  if (p.ticket) {
-    if (threadIdx.x == 0) sh.ticket = atomicAdd(p.ticket, 1u);
-    __syncthreads();
-    task = sh.ticket;
+  __device__ __forceinline__ ScanWarp(const ScanArgs &args, unsigned *smem) : p(args) {
+    offsets = static_cast<const OffT *>(p.offsets);
+    const int lane = threadIdx.x & 31;
+    lanes = 1 << p.shift;
+    rows = 1 << p.row_shift;
+    words = (rows < 64 ? 64 : rows) / 32;
+    base = (lane >> p.shift) * p.lane_rows;
+    m.start_mask = smem + (threadIdx.x >> 5) * scan_marks_words(rows);
+    m.end_mask = m.start_mask + words;
+    m.start_seg = reinterpret_cast<int *>(m.end_mask + words);
+    m.end_seg = m.start_seg + rows;
   }
-  const int tile = static_cast<int>(task % p.tiles);
-  const int64_t block = task / p.tiles;
-  // Chunk of this CTA, in the order of the recurrence; the extra blocks come last.
-  const int64_t pos = block;
-  const int64_t chunk = BACKWARD ? p.chunks - 1 - block : block;
-  const int vc = tile * lanes + (threadIdx.x & (lanes - 1));
-  const bool col_ok = vc < p.vec_cols;
-  const int64_t col = static_cast<int64_t>(vc) * VEC;
-  const int local_col = (threadIdx.x & (lanes - 1)) * VEC;
-  const int width = min(lanes, p.vec_cols - tile * lanes) * VEC;
-
-  auto load_state = [&](const float *at, float (&x)[VEC]) {
-#pragma unroll
-    for (int i = 0; i < VEC / kPiece; ++i) {
-      float y[kPiece];
-      State::load(at + i * kPiece, y);
-#pragma unroll
-      for (int v = 0; v < kPiece; ++v) x[i * kPiece + v] = y[v];
-    }
-  };
-  auto store_state = [&](float *at, const float (&x)[VEC]) {
-#pragma unroll
-    for (int i = 0; i < VEC / kPiece; ++i) {
-      float y[kPiece];
-#pragma unroll
-      for (int v = 0; v < kPiece; ++v) y[v] = x[i * kPiece + v];
-      State::store(at + i * kPiece, y);
-    }
-  };
-
-  if (block < p.chunks) {
-    const int64_t row0 = chunk * rows;
-    const int64_t end_row = min(row0 + rows, p.n);
-    const int group = threadIdx.x >> p.shift;
-    const int64_t my_row = row0 + static_cast<int64_t>(group) * ROWS;
-    const int base = group * ROWS;
-
-    Raw ra[ROWS], rx[ROWS], rg[BACKWARD ? ROWS : 1];
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-      const bool ok = col_ok && my_row + i < p.n;
-      const int64_t at = (my_row + i) * p.d + col;
-      ra[i] = ok ? IO::load_raw(gates + at) : Raw{};
-      rx[i] = ok ? IO::load_raw(values + at) : Raw{};
-      if constexpr (BACKWARD) rg[i] = ok ? IO::load_raw(static_cast<const T *>(p.grad_out) + at) : Raw{};
-    }
-
-    for (int i = threadIdx.x; i <= rows; i += kScanThreads) {
-      start[i] = -1;
-      ended[i] = kNoEnd;
-    }
-    if (threadIdx.x == 0) sh.last = -1;
-    const int64_t seg0 = scan_find(offsets, p.b, row0);
-    __syncthreads();
-    scan_mark(offsets, p.b, seg0, row0, rows, end_row, start, ended, &sh.last);
-    if (BACKWARD && threadIdx.x < width) {
-      const int64_t begin = static_cast<int64_t>(offsets[seg0]);
-      sh.before[threadIdx.x] = begin < row0 ? p.carries[chunk * p.d + static_cast<int64_t>(tile) * lanes * VEC +
-                                                        threadIdx.x]
-                                            : 0.0f;
-    }
-    __syncthreads();
-
-    float previous[BACKWARD ? ROWS : 1][VEC];  // h before each row
-    // ---------------------------------------------------- forward fold --
-    // A row with a start replaces what came before by its initial state.
-    {
-      float a[VEC], h[VEC];
-      int reset = 0;
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        a[v] = 1.0f;
-        h[v] = 0.0f;
-      }
-#pragma unroll
-      for (int i = 0; i < ROWS; ++i) {
-        if (my_row + i < p.n) {
-          float ga[VEC], x[VEC];
-          IO::unpack(ra[i], ga);
-          IO::unpack(rx[i], x);
-          const int s = start[base + i];
-          if (s >= 0) {
-            reset = 1;
-            if (p.initial && col_ok) {
-              load_state(p.initial + s * p.d + col, h);
-            } else {
-#pragma unroll
-              for (int v = 0; v < VEC; ++v) h[v] = 0.0f;
-            }
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) h[v] = p.initial ? fmaf(ga[v], h[v], x[v]) : x[v];
-          } else {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-              h[v] = fmaf(ga[v], h[v], x[v]);
-              a[v] *= ga[v];
-            }
-          }
-        }
-      }
-      scan_warp<VEC, false>(a, h, reset, p.shift, sh.total[warp], &sh.total_reset[warp]);
-      if constexpr (!BACKWARD) {
-        const int64_t begin = static_cast<int64_t>(offsets[seg0]);
-        const int64_t first = begin >= row0 ? pos : (begin > 0 ? begin / rows : 0);
-        scan_chunk<false>(p, sh, tile, pos, first, width);
-        if (p.carries && threadIdx.x < width)
-          p.carries[chunk * p.d + static_cast<int64_t>(tile) * lanes * VEC + threadIdx.x] = sh.carry[0][threadIdx.x];
-        float state[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v)
-          state[v] = reset ? h[v] : scan_apply(a[v], h[v], col_ok ? sh.carry[warp][local_col + v] : 0.0f);
-#pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-          if (col_ok && my_row + i < p.n) {
-            float ga[VEC], x[VEC];
-            IO::unpack(ra[i], ga);
-            IO::unpack(rx[i], x);
-            const int s = start[base + i];
-            if (s >= 0 && !p.initial) {
-#pragma unroll
-              for (int v = 0; v < VEC; ++v) state[v] = x[v];
-            } else {
-              if (s >= 0) load_state(p.initial + s * p.d + col, state);
-#pragma unroll
-              for (int v = 0; v < VEC; ++v) state[v] = fmaf(ga[v], state[v], x[v]);
-            }
-            IO::store(static_cast<T *>(p.out) + (my_row + i) * p.d + col, state);
-            const int e = ended[base + i + 1];
-            if (p.final_state && e != kNoEnd) store_state(p.final_state + (static_cast<int64_t>(e) - 1) * p.d + col, state);
-          }
-        }
-      } else {
-        __syncthreads();
-        if (threadIdx.x < width) {
-          float state = sh.before[threadIdx.x];
-#pragma unroll
-          for (int w = 0; w < kScanWarps; ++w) {
-            sh.carry[w][threadIdx.x] = state;
-            const float2 t = sh.total[w][threadIdx.x];
-            state = sh.total_reset[w] ? t.y : scan_apply(t.x, t.y, state);
-          }
-        }
-        __syncthreads();
-        float state[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v)
-          state[v] = reset ? h[v] : scan_apply(a[v], h[v], col_ok ? sh.carry[warp][local_col + v] : 0.0f);
-#pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-          float ga[VEC], x[VEC];
-          IO::unpack(ra[i], ga);
-          IO::unpack(rx[i], x);
-          const bool ok = col_ok && my_row + i < p.n;
-          const int s = ok ? start[base + i] : -1;
-          if (s >= 0) {
-            if (p.initial) {
-              load_state(p.initial + s * p.d + col, state);
-            } else {
-#pragma unroll
-              for (int v = 0; v < VEC; ++v) state[v] = 0.0f;
-            }
-          }
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            previous[i][v] = state[v];
-            state[v] = s >= 0 && !p.initial ? x[v] : fmaf(ga[v], state[v], x[v]);
-          }
-        }
-        __syncthreads();
-      }
-    }
-
-    // --------------------------------------------------- backward fold --
-    if constexpr (BACKWARD) {
-      float a[VEC], u[VEC];
-      int reset = 0;
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        a[v] = 1.0f;
-        u[v] = 0.0f;
-      }
-      auto at_end = [&](int i, float (&x)[VEC]) {  // u past row i where a segment ends there
-        const int e = ended[base + i + 1];
-        if (e == kNoEnd) return false;
-        if (p.grad_final && col_ok) {
-          load_state(p.grad_final + (static_cast<int64_t>(e) - 1) * p.d + col, x);
-        } else {
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) x[v] = 0.0f;
-        }
-        return true;
-      };
-#pragma unroll
-      for (int i = ROWS - 1; i >= 0; --i) {
-        if (my_row + i < p.n) {
-          float ga[VEC], g[VEC];
-          IO::unpack(ra[i], ga);
-          IO::unpack(rg[i], g);
-          if (at_end(i, u)) {
-            reset = 1;
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) u[v] = ga[v] * (g[v] + u[v]);
-          } else {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-              u[v] = ga[v] * (g[v] + u[v]);
-              a[v] *= ga[v];
-            }
-          }
-        }
-      }
-      scan_warp<VEC, true>(a, u, reset, p.shift, sh.total[warp], &sh.total_reset[warp]);
-      const int64_t last = max(seg0, static_cast<int64_t>(sh.last));
-      const int64_t stop = min(static_cast<int64_t>(offsets[last + 1]), p.n);
-      const int64_t first = stop <= end_row ? pos : p.chunks - 1 - (stop - 1) / rows;
-      scan_chunk<true>(p, sh, tile, pos, first, width);
-#pragma unroll
-      for (int v = 0; v < VEC; ++v)
-        u[v] = reset ? u[v] : scan_apply(a[v], u[v], col_ok ? sh.carry[warp][local_col + v] : 0.0f);
-#pragma unroll
-      for (int i = ROWS - 1; i >= 0; --i) {
-        if (col_ok && my_row + i < p.n) {
-          float ga[VEC], g[VEC];
-          IO::unpack(ra[i], ga);
-          IO::unpack(rg[i], g);
-          at_end(i, u);
-          const int s = start[base + i];
-          const int64_t at = (my_row + i) * p.d + col;
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) g[v] += u[v];
-          if (p.grad_values) IO::store(static_cast<T *>(p.grad_values) + at, g);
-#pragma unroll
-          for (int v = 0; v < VEC; ++v) {
-            u[v] = ga[v] * g[v];
-            g[v] = s >= 0 && !p.initial ? 0.0f : g[v] * previous[i][v];
-          }
-          if (p.grad_gates) IO::store(static_cast<T *>(p.grad_gates) + at, g);
-          if (p.grad_initial && s >= 0) store_state(p.grad_initial + s * p.d + col, u);
-        }
-      }
-    }
+  __device__ __forceinline__ void go(int64_t slab, int tile) {
+    pos = slab;
+    row0 = (BACKWARD ? p.slabs - 1 - pos : pos) << p.row_shift;
+    col = (static_cast<int64_t>(tile) * lanes + (threadIdx.x & (lanes - 1))) * VEC;
+    col_ok = col < p.d;
   }
-
-  // Segments without rows: the state passes through (as does its gradient).
-  float *state_out = BACKWARD ? p.grad_initial : p.final_state;
-  const float *state_in = BACKWARD ? p.grad_final : p.initial;
-  if (state_out && col_ok) {
-    const int64_t per = (p.b + p.blocks - 1) / p.blocks;
-    const int64_t stop = min(p.b, (block + 1) * per);
-    for (int64_t s = block * per + (threadIdx.x >> p.shift); s < stop; s += kScanThreads >> p.shift) {
-      if (static_cast<int64_t>(offsets[s]) < static_cast<int64_t>(offsets[s + 1])) continue;
-      float x[VEC];
+  __device__ __forceinline__ void mark() {
+    __syncwarp();
+    seg0 = scan_find(offsets, p.b, row0);
+    scan_mark(offsets, p.b, seg0, row0, rows, m);
+  }
+  __device__ __forceinline__ uint64_t lane_bits(const unsigned *mask) const {  // of this lane's rows
+    if (p.lane_rows == 64) return mask[base >> 5] | (static_cast<uint64_t>(mask[(base >> 5) + 1]) << 32);
+    const unsigned word = mask[base >> 5];
+    return p.lane_rows == 32 ? word : (word >> (base & 31)) & 0xffffu;
+  }
+  __device__ __forceinline__ bool starts_at_first() const { return m.start_mask[0] & 1; }
+  __device__ __forceinline__ bool ends_at_last() const {
+    const int last = static_cast<int>(min(static_cast<int64_t>(rows), p.n - row0)) - 1;
+    return (m.end_mask[last >> 5] >> (last & 31)) & 1;
+  }
+  __device__ __forceinline__ int row_count(int64_t row) const {  // rows of the batch at `row`
+    return static_cast<int>(min(max(p.n - row, int64_t{0}), int64_t{kScanBatch}));
+  }
+  __device__ __forceinline__ void state_of(const float *states, int64_t seg, float (&x)[VEC]) const {
+    if (states) {
+      State::load(states + seg * p.d + col, x);
+    } else {
 #pragma unroll
       for (int v = 0; v < VEC; ++v) x[v] = 0.0f;
-      if (state_in) load_state(state_in + s * p.d + col, x);
-      store_state(state_out + s * p.d + col, x);
+    }
+  }
+
+  // Folds this lane's rows from the last segment start on (first end,
+  // BACKWARD).  Returns whether there is one.
+  __device__ __forceinline__ bool fold(Pair &f) const {
+    constexpr int BATCH = kScanBatch;
+    f.clear();
+    const uint64_t marks = lane_bits(BACKWARD ? m.end_mask : m.start_mask);
+    if (!col_ok) return marks != 0;
+    const T *__restrict__ gates = static_cast<const T *>(p.gates);
+    const T *__restrict__ second = static_cast<const T *>(BACKWARD ? p.grad_out : p.values);
+    const int batches = p.lane_rows / BATCH;
+    const int enter = !marks ? (BACKWARD ? batches - 1 : 0)
+                             : (BACKWARD ? __ffsll(marks) - 1 : 63 - __clzll(marks)) / BATCH;
+#pragma unroll 1
+    for (int batch = enter; BACKWARD ? batch >= 0 : batch < batches; batch += BACKWARD ? -1 : 1) {
+      const int64_t row = row0 + base + batch * BATCH;
+      const int count = row_count(row);
+      if (count <= 0) continue;
+      Raw ra[BATCH], rx[BATCH];
+      scan_rows<T, VEC>(gates + row * p.d + col, p.d, count, ra);
+      scan_rows<T, VEC>(second + row * p.d + col, p.d, count, rx);
+      const unsigned mark = static_cast<unsigned>(marks >> (batch * BATCH)) & 0xffffu;
+      const int *seg = (BACKWARD ? m.end_seg : m.start_seg) + base + batch * BATCH;
+      const bool plain = mark == 0 && count == BATCH;
+      auto step = [&](int i, bool alone) {
+        float a[VEC], x[VEC];
+        IO::unpack(ra[i], a);
+        IO::unpack(rx[i], x);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          if constexpr (BACKWARD)
+            f.h[v] = a[v] * (x[v] + f.h[v]);
+          else
+            f.h[v] = alone ? x[v] : fmaf(a[v], f.h[v], x[v]);
+          f.a[v] *= a[v];
+        }
+      };
+      if (plain) {
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) step(BACKWARD ? BATCH - 1 - j : j, false);
+      } else {
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          const int i = BACKWARD ? BATCH - 1 - j : j;
+          if (i < count) {
+            const bool enters = (mark >> i) & 1;
+            if (enters) state_of(BACKWARD ? p.grad_final : p.initial, seg[i], f.h);
+            step(i, enters && !p.initial);
+          }
+        }
+      }
+    }
+    return marks != 0;
+  }
+
+  // Without a workspace: the state before this lane's rows, by running the
+  // recurrence over the rows of their segment before (after, BACKWARD) them.
+  __device__ __forceinline__ void catch_up(float (&h)[VEC]) const {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) h[v] = 0.0f;
+    const int64_t mine = row0 + base;
+    if (mine >= p.n || !col_ok) return;
+    const T *__restrict__ gates = static_cast<const T *>(p.gates);
+    const T *__restrict__ second = static_cast<const T *>(BACKWARD ? p.grad_out : p.values);
+    int64_t seg = seg0;  // the segment of this lane's first (last, BACKWARD) row
+    const int64_t here = BACKWARD ? min(mine + p.lane_rows, p.n) - 1 : mine;
+    const int at = static_cast<int>(here - row0);
+    for (int i = at >> 5; i >= 0; --i) {
+      const unsigned bits = m.start_mask[i] & (i == at >> 5 ? (2u << (at & 31)) - 1 : ~0u);
+      if (bits) {
+        seg = m.start_seg[i * 32 + 31 - __clz(bits)];
+        break;
+      }
+    }
+    const int64_t begin = max(static_cast<int64_t>(offsets[seg]), int64_t{0});
+    const int64_t end = min(static_cast<int64_t>(offsets[seg + 1]), p.n);
+    if (BACKWARD ? end - 1 <= here : begin >= mine) return;
+    state_of(BACKWARD ? p.grad_final : p.initial, seg, h);
+    const int64_t count = BACKWARD ? end - 1 - here : mine - begin;
+#pragma unroll 4
+    for (int64_t i = 0; i < count; ++i) {
+      const int64_t at = (BACKWARD ? end - 1 - i : begin + i) * p.d + col;
+      float a[VEC], x[VEC];
+      IO::load(gates + at, a);
+      IO::load(second + at, x);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        if constexpr (BACKWARD)
+          h[v] = a[v] * (x[v] + h[v]);
+        else
+          h[v] = i == 0 && !p.initial ? x[v] : fmaf(a[v], h[v], x[v]);
+      }
+    }
+  }
+};
+
+template <typename T, typename OffT, int VEC, bool BACKWARD>
+__global__ void __launch_bounds__(kScanThreads, 3) scan_fold_kernel(const ScanArgs p) {
+  extern __shared__ unsigned scan_smem[];
+  ScanWarp<T, OffT, VEC, BACKWARD> w(p, scan_smem);
+  const unsigned tasks = static_cast<unsigned>(p.slabs * p.tiles);
+  for (unsigned t = blockIdx.x * kScanWarps + (threadIdx.x >> 5); t < tasks; t += gridDim.x * kScanWarps) {
+    const unsigned slab = t / p.tiles;
+    w.go(slab, static_cast<int>(t - slab * p.tiles));
+    w.mark();
+    // A slab that ends a segment is a start for those after it.
+    const bool closed = BACKWARD ? w.starts_at_first() : w.ends_at_last();
+    ScanPair<VEC> f, total;
+    int reset = 1, total_reset = 1;
+    f.clear();
+    total.clear();
+    if (!closed) {
+      reset = w.fold(f);
+      scan_groups<VEC, BACKWARD>(f, reset, total, total_reset, p.shift);
+    }
+    if ((threadIdx.x & 31) < w.lanes && w.col_ok) total.store(p.pairs + slab * p.d + w.col, total_reset);
+  }
+}
+
+// 32 columns a block; each warp composes the pairs of a part of the slabs,
+// then all go through the parts before theirs, then each through its own.
+__global__ void __launch_bounds__(kScanJoinWarps * 32) scan_join_kernel(const ScanArgs p) {
+  __shared__ float part_a[kScanJoinWarps][32], part_h[kScanJoinWarps][32];
+  __shared__ bool part_reset[kScanJoinWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  const bool live = col < p.d;
+  const int64_t per = (p.slabs + kScanJoinWarps - 1) / kScanJoinWarps;
+  const int64_t begin = min(warp * per, p.slabs), end = min(begin + per, p.slabs);
+  float a = 1.0f, h = 0.0f;
+  bool reset = false;
+  auto each = [&](auto act) {
+#pragma unroll 1
+    for (int64_t s = begin; s < end; s += kScanAhead) {
+      float2 pair[kScanAhead];
+#pragma unroll
+      for (int i = 0; i < kScanAhead; ++i)
+        if (live && s + i < end) pair[i] = p.pairs[(s + i) * p.d + col];
+#pragma unroll
+      for (int i = 0; i < kScanAhead; ++i)
+        if (live && s + i < end) act(s + i, pair[i]);
+    }
+  };
+  each([&](int64_t, const float2 &x) {
+    const bool starts = __float_as_uint(x.x) == kScanReset;
+    h = starts ? x.y : scan_apply(x.x, x.y, h);
+    a *= x.x;
+    reset |= starts;
+  });
+  part_a[warp][lane] = a;
+  part_h[warp][lane] = h;
+  part_reset[warp][lane] = reset;
+  __syncthreads();
+  float state = 0.0f;
+  for (int w = 0; w < warp; ++w)
+    state = part_reset[w][lane] ? part_h[w][lane] : scan_apply(part_a[w][lane], part_h[w][lane], state);
+  each([&](int64_t s, const float2 &x) {
+    p.states[s * p.d + col] = state;
+    state = __float_as_uint(x.x) == kScanReset ? x.y : scan_apply(x.x, x.y, state);
+  });
+}
+
+template <typename T, typename OffT, int VEC, bool BACKWARD>
+__global__ void __launch_bounds__(kScanThreads, BACKWARD ? 2 : 3) scan_walk_kernel(const ScanArgs p) {
+  constexpr int BATCH = kScanBatch;
+  using IO = VecIO<T, VEC>;
+  using Raw = typename IO::Raw;
+  using State = VecIO<float, VEC>;
+  extern __shared__ unsigned scan_smem[];
+  const T *__restrict__ values = static_cast<const T *>(p.values);
+  const T *__restrict__ gates = static_cast<const T *>(p.gates);
+  const T *__restrict__ grads = static_cast<const T *>(p.grad_out);
+  ScanWarp<T, OffT, VEC, BACKWARD> w(p, scan_smem);
+  const unsigned tasks = static_cast<unsigned>(p.blocks * p.tiles);
+  for (unsigned t = blockIdx.x * kScanWarps + (threadIdx.x >> 5); t < tasks; t += gridDim.x * kScanWarps) {
+    const int64_t block = p.blocks - 1 - t / p.tiles;
+    const int tile = static_cast<int>(t % p.tiles);
+    if (block < p.slabs) {
+      w.go(block, tile);
+      w.mark();
+      const uint64_t starts = w.lane_bits(w.m.start_mask), ends = w.lane_bits(w.m.end_mask);
+      float h[VEC];
+      if (!p.pairs) {
+        w.catch_up(h);
+      } else {
+        ScanPair<VEC> f, total;
+        int reset = 0, total_reset;
+        f.clear();
+        if (p.shift < 5) {  // rows of other lanes come before this lane's
+          reset = w.fold(f);
+          scan_groups<VEC, BACKWARD>(f, reset, total, total_reset, p.shift);
+        }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) h[v] = 0.0f;
+        if (w.col_ok && !(BACKWARD ? w.ends_at_last() : w.starts_at_first()))
+          State::load(p.states + w.pos * p.d + w.col, h);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) h[v] = reset ? f.h[v] : scan_apply(f.a[v], f.h[v], h[v]);
+      }
+      const int batches = p.lane_rows / BATCH;
+#pragma unroll 1
+      for (int k = 0; k < batches; ++k) {
+        const int batch = BACKWARD ? batches - 1 - k : k;
+        const int64_t row = w.row0 + w.base + batch * BATCH;
+        const int count = w.row_count(row);
+        if (count <= 0 || !w.col_ok) continue;
+        const int64_t at = row * p.d + w.col;
+        const unsigned start = static_cast<unsigned>(starts >> (batch * BATCH)) & 0xffffu;
+        const unsigned end = static_cast<unsigned>(ends >> (batch * BATCH)) & 0xffffu;
+        const int *start_seg = w.m.start_seg + w.base + batch * BATCH;
+        const int *end_seg = w.m.end_seg + w.base + batch * BATCH;
+        const bool plain = (start | end) == 0 && count == BATCH;
+        Raw ra[BATCH], rx[BATCH];
+        scan_rows<T, VEC>(gates + at, p.d, count, ra);
+        scan_rows<T, VEC>(values + at, p.d, count, rx);
+        // A row that starts a segment goes on from the initial state, or is its value.
+        auto advance = [&](int i, float (&s)[VEC], bool alone) {
+          float a[VEC], x[VEC];
+          IO::unpack(ra[i], a);
+          IO::unpack(rx[i], x);
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) s[v] = alone ? x[v] : fmaf(a[v], s[v], x[v]);
+        };
+        if constexpr (!BACKWARD) {
+          if (p.carries) State::store(p.carries + (row / BATCH) * p.d + w.col, h);
+          T *to = static_cast<T *>(p.out) + at;
+          if (plain) {
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+              advance(i, h, false);
+              IO::store(to, h);
+              to += p.d;
+            }
+          } else {
+            // Four rows at a time, their initial states asked for together.
+#pragma unroll
+            for (int q = 0; q < BATCH; q += 4) {
+              float first[4][VEC];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (q + i < count && ((start >> (q + i)) & 1)) w.state_of(p.initial, start_seg[q + i], first[i]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if (q + i < count) {
+                  const bool is_first = (start >> (q + i)) & 1;
+#pragma unroll
+                  for (int v = 0; v < VEC; ++v) h[v] = is_first ? first[i][v] : h[v];
+                  advance(q + i, h, is_first && !p.initial);
+                  IO::store(to, h);
+                  to += p.d;
+                  if (p.final_state && ((end >> (q + i)) & 1))
+                    State::store(p.final_state + static_cast<int64_t>(end_seg[q + i]) * p.d + w.col, h);
+                }
+              }
+            }
+          }
+        } else {
+          Raw rg[BATCH];
+          scan_rows<T, VEC>(grads + at, p.d, count, rg);
+          float previous[BATCH][VEC], s[VEC];  // state before each row
+          State::load(p.carries + (row / BATCH) * p.d + w.col, s);
+#pragma unroll
+          for (int i = 0; i < BATCH; ++i) {
+            const bool is_first = (start >> i) & 1;
+            if (is_first) w.state_of(p.initial, start_seg[i], s);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) previous[i][v] = s[v];
+            advance(i, s, is_first && !p.initial);
+          }
+          const int64_t last = at + (count - 1) * p.d;
+          T *to_values = p.grad_values ? static_cast<T *>(p.grad_values) + last : nullptr;
+          T *to_gates = p.grad_gates ? static_cast<T *>(p.grad_gates) + last : nullptr;
+#pragma unroll
+          for (int i = BATCH - 1; i >= 0; --i) {
+            if (i < count) {
+              float a[VEC], g[VEC];
+              IO::unpack(ra[i], a);
+              IO::unpack(rg[i], g);
+              if ((end >> i) & 1) w.state_of(p.grad_final, end_seg[i], h);
+              const bool is_first = (start >> i) & 1, unused = is_first && !p.initial;
+#pragma unroll
+              for (int v = 0; v < VEC; ++v) g[v] += h[v];
+              if (to_values) {
+                IO::store(to_values, g);
+                to_values -= p.d;
+              }
+#pragma unroll
+              for (int v = 0; v < VEC; ++v) {
+                h[v] = a[v] * g[v];
+                g[v] = unused ? 0.0f : g[v] * previous[i][v];
+              }
+              if (to_gates) {
+                IO::store(to_gates, g);
+                to_gates -= p.d;
+              }
+              if (p.grad_initial && is_first)
+                State::store(p.grad_initial + static_cast<int64_t>(start_seg[i]) * p.d + w.col, h);
+            }
+          }
+        }
+      }
+    }
+    // Segments without rows: the state passes through (as does its gradient).
+    float *to = BACKWARD ? p.grad_initial : p.final_state;
+    w.go(block, tile);
+    if (to && w.col_ok) {
+      const int64_t stop = min(p.b, (block + 1) * p.per_block);
+      for (int64_t s = block * p.per_block + ((threadIdx.x & 31) >> p.shift); s < stop; s += 32 >> p.shift) {
+        if (static_cast<int64_t>(w.offsets[s]) < static_cast<int64_t>(w.offsets[s + 1])) continue;
+        float x[VEC];
+        w.state_of(BACKWARD ? p.grad_final : p.initial, s, x);
+        State::store(to + s * p.d + w.col, x);
+      }
     }
   }
 }

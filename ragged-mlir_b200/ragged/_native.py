@@ -98,11 +98,11 @@ def library(path: Path | None = None):
         lib.rg_run_noalloc.restype = i32
         lib.rg_tree_scores.argtypes = [i64, p, p, p, p, p, p, i64, p, p, i32, p, i32, p, i32, p]
         lib.rg_tree_scores.restype = i32
-        lib.rg_scan_workspace_bytes.argtypes = [i32, i32, i64, i64, i64, u32, ctypes.POINTER(i64), ctypes.POINTER(i64)]
+        lib.rg_scan_workspace_bytes.argtypes = [i32, i32, i64, i64, i64, ctypes.POINTER(i64)]
         lib.rg_scan_workspace_bytes.restype = i32
-        lib.rg_scan.argtypes = [i32, i32, i64, i64, i64, p, p, p, p, p, p, p, p, i64, u32, p, ctypes.POINTER(Report)]
+        lib.rg_scan.argtypes = [i32, i32, i64, i64, i64, p, p, p, p, p, p, p, p, i64, p, ctypes.POINTER(Report)]
         lib.rg_scan.restype = i32
-        lib.rg_scan_backward.argtypes = [i32, i32, i64, i64, i64, p, p, p, p, p, p, p, p, p, p, p, i64, u32, p,
+        lib.rg_scan_backward.argtypes = [i32, i32, i64, i64, i64, p, p, p, p, p, p, p, p, p, p, p, i64, p,
                                          ctypes.POINTER(Report)]
         lib.rg_scan_backward.restype = i32
         pi64 = ctypes.POINTER(i64)
@@ -339,30 +339,30 @@ def check_offsets(index: str, n: int, b: int, offsets_ptr: int, min_len: int | N
 
 # --------------------------------------------------------- learned operators
 
-def scan_sizes(dtype: str, index: str, d: int, n: int, b: int, flags: int = 0) -> tuple[int, int]:
-    """(scratch bytes, rows of recorded states) of a segmented scan."""
-    nbytes, rows = ctypes.c_int64(0), ctypes.c_int64(0)
-    raise_for(library().rg_scan_workspace_bytes(DTYPES[dtype], INDEX[index], d, n, b, flags, ctypes.byref(nbytes),
-                                                ctypes.byref(rows)), "rg_scan_workspace_bytes")
-    return nbytes.value, rows.value
+def scan_workspace_bytes(dtype: str, index: str, d: int, n: int, b: int) -> int:
+    """Scratch bytes of a segmented scan (either pass)."""
+    out = ctypes.c_int64(0)
+    raise_for(library().rg_scan_workspace_bytes(DTYPES[dtype], INDEX[index], d, n, b, ctypes.byref(out)),
+              "rg_scan_workspace_bytes")
+    return out.value
 
 
 def scan(dtype: str, index: str, d: int, n: int, b: int, pointers: tuple, workspace_ptr: int, workspace_bytes: int,
-         flags: int, stream: int) -> Report:
+         stream: int) -> Report:
     """``pointers``: values, gates, offsets, initial, out, final, carries (0: none)."""
     report = Report()
-    raise_for(library().rg_scan(DTYPES[dtype], INDEX[index], d, n, b, *pointers, workspace_ptr, workspace_bytes, flags,
+    raise_for(library().rg_scan(DTYPES[dtype], INDEX[index], d, n, b, *pointers, workspace_ptr, workspace_bytes,
                                 stream, ctypes.byref(report)), "rg_scan")
     return report
 
 
 def scan_backward(dtype: str, index: str, d: int, n: int, b: int, pointers: tuple, workspace_ptr: int,
-                  workspace_bytes: int, flags: int, stream: int) -> Report:
+                  workspace_bytes: int, stream: int) -> Report:
     """``pointers``: values, gates, offsets, initial, carries, grad_out,
     grad_final, grad_values, grad_gates, grad_initial (0: none)."""
     report = Report()
     raise_for(library().rg_scan_backward(DTYPES[dtype], INDEX[index], d, n, b, *pointers, workspace_ptr,
-                                         workspace_bytes, flags, stream, ctypes.byref(report)), "rg_scan_backward")
+                                         workspace_bytes, stream, ctypes.byref(report)), "rg_scan_backward")
     return report
 
 

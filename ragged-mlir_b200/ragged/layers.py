@@ -25,18 +25,7 @@ from .runtime import CompiledProgram, _checked_devices, _torch
 from .validation import STATUS_BYTES
 
 
-def scan_chunk_rows(dtype: str, d: int, vectorize: bool = True) -> int:
-    """Rows per recorded state of a scan (the kernels' chunk: 256 threads,
-    tiles of up to 128 bytes of columns, 4 rows a thread of full 16-byte
-    vectors and 8 of narrower ones)."""
-    size = 4 if dtype == "f32" else 2
-    vec = 1
-    while vectorize and 2 * vec * size <= 16 and d % (2 * vec) == 0:
-        vec *= 2
-    lanes = 1
-    while lanes < d // vec and lanes < 32 and 2 * lanes * vec * size <= 128:
-        lanes *= 2
-    return 256 // lanes * (4 if vec * size == 16 else 8)
+CARRY_ROWS = 16  # rows per state that a scan records for its backward pass
 
 
 class _LayerProgram:
@@ -177,18 +166,13 @@ class CompiledScan(_LayerProgram):
 
     kind = ScanSpec
 
-    def __init__(self, spec, artifact, *, cache_hit: bool = False):
-        super().__init__(spec, artifact, cache_hit=cache_hit)
-        self._flags = 0 if spec.vectorize else _native.FLAG_NO_VECTORIZE
-
     def carry_rows(self, n: int) -> int:
         """Rows of the ``carries`` that a call over ``n`` rows records."""
-        rows = scan_chunk_rows(self.spec.dtype, self.spec.feature_dim, self.spec.vectorize)
-        return (n + rows - 1) // rows
+        return (n + CARRY_ROWS - 1) // CARRY_ROWS
 
     def _scratch(self, n, b) -> int:
-        return self._cached((n, b), lambda: _native.scan_sizes(
-            self.spec.dtype, self.spec.offsets_dtype, self.spec.feature_dim, n, b, self._flags))[0]
+        return self._cached((n, b), lambda: _native.scan_workspace_bytes(
+            self.spec.dtype, self.spec.offsets_dtype, self.spec.feature_dim, n, b))
 
     def run(self, values, gates, offsets, out, stream=None, mode: str = "validated", *, initial=None, final=None,
             carries=None) -> ExecutionReport:
@@ -217,7 +201,7 @@ class CompiledScan(_LayerProgram):
                     _address(final), _address(carries))
 
         def call(scratch, nbytes, on):
-            return _native.scan(spec.dtype, spec.offsets_dtype, d, n, b, pointers, scratch, nbytes, self._flags, on)
+            return _native.scan(spec.dtype, spec.offsets_dtype, d, n, b, pointers, scratch, nbytes, on)
 
         return self._launch(torch, offsets, n, b, stream, mode, [t[1] for t in tensors] + [offsets],
                             [(self._scratch(n, b), call)])
@@ -246,8 +230,7 @@ class CompiledScan(_LayerProgram):
                     _address(grad_initial))
 
         def call(scratch, nbytes, on):
-            return _native.scan_backward(spec.dtype, spec.offsets_dtype, d, n, b, pointers, scratch, nbytes,
-                                         self._flags, on)
+            return _native.scan_backward(spec.dtype, spec.offsets_dtype, d, n, b, pointers, scratch, nbytes, on)
 
         return self._launch(torch, offsets, n, b, stream, "validated", [t[1] for t in tensors] + [offsets],
                             [(self._scratch(n, b), call)])

@@ -197,22 +197,18 @@ class _LayerSpec:
 class ScanSpec(_LayerSpec):
     """A gated linear recurrence over segments, out[t] = gates[t] * out[t - 1]
     + values[t], over ``feature_dim`` columns.  ``hints`` bound the segment
-    lengths that checked mode accepts; ``vectorize=False`` is for views that
-    are not 16-byte aligned."""
+    lengths that checked mode accepts."""
 
     dtype: str = "f32"
     feature_dim: int = 128
     offsets_dtype: str = "i64"
     hints: Hints = field(default_factory=Hints)
-    vectorize: bool = True
     chip: str = DEFAULT_CHIP
     op: str = field(default="scan", init=False)
 
     def __post_init__(self) -> None:
         self._check()
         self._check_dim("feature_dim")
-        if type(self.vectorize) is not bool:
-            raise ValidationError("vectorize must be bool")
 
     @property
     def signature(self) -> str:

@@ -26,7 +26,7 @@ import threading
 from typing import Any
 
 from .errors import ValidationError
-from .layers import CompiledScan, scan_chunk_rows
+from .layers import CARRY_ROWS, CompiledScan
 from .runtime import CompiledProgram, _torch
 
 MODES = ("validated", "checked")
@@ -60,13 +60,6 @@ class ProgramTable:
         with self._lock:
             self._programs[token] = program
         return token
-
-    def vectorizes(self, token: str) -> bool:
-        """Whether the scan program of ``token`` moves full vectors (a token
-        that is not registered, while tracing shapes: yes)."""
-        with self._lock:
-            program = self._programs.get(token)
-        return program is None or getattr(program.spec, "vectorize", True)
 
     def lookup(self, token: str, op: str):
         with self._lock:
@@ -188,10 +181,10 @@ def _dense(*tensors):
     return tuple(t.contiguous() if t is not None else None for t in tensors)
 
 
-def _scan_shapes(values, offsets, rows: int, record: bool) -> tuple:
+def _scan_shapes(values, offsets, record: bool) -> tuple:
     """Shapes of out, final and carries."""
     n, d = values.shape
-    return (n, d), (offsets.shape[0] - 1, d), ((n + rows - 1) // rows if record else 0, d)
+    return (n, d), (offsets.shape[0] - 1, d), ((n + CARRY_ROWS - 1) // CARRY_ROWS if record else 0, d)
 
 
 def _scan_call(values, gates, offsets, initial, token: str, mode: str, record: bool):
@@ -199,10 +192,9 @@ def _scan_call(values, gates, offsets, initial, token: str, mode: str, record: b
     torch = _torch()
     program = _table.lookup(token, "scan")
     values, gates, initial = _dense(values, gates, initial)
+    shapes = _scan_shapes(values, offsets, record)
     out = torch.empty_like(values)
-    state = dict(dtype=torch.float32, device=values.device)
-    final = torch.empty((offsets.shape[0] - 1, values.shape[1]), **state)
-    carries = torch.empty((program.carry_rows(values.shape[0]) if record else 0, values.shape[1]), **state)
+    final, carries = (torch.empty(shape, dtype=torch.float32, device=values.device) for shape in shapes[1:])
     program._run(values, gates, offsets, out, initial, final, carries if record else None, None, mode, False)
     return out, final, carries
 
@@ -240,9 +232,7 @@ def _register_scan(torch, library, contract) -> None:
     def scan_fake(values, gates, offsets, initial, program, mode="validated", record=True):
         contract.mode(mode)
         contract.scan(values, gates, offsets, initial)
-        dtype = "f32" if values.dtype == torch.float32 else "bf16"
-        rows = scan_chunk_rows(dtype, int(values.shape[1]), _table.vectorizes(program))
-        out, final, carries = _scan_shapes(values, offsets, rows, record)
+        out, final, carries = _scan_shapes(values, offsets, record)
         state = dict(dtype=torch.float32, device=values.device)
         return (torch.empty(out, dtype=values.dtype, device=values.device), torch.empty(final, **state),
                 torch.empty(carries, **state))

@@ -17,9 +17,9 @@ SENTINEL = -64.0
 
 
 @functools.lru_cache(maxsize=256)
-def scan_program(dtype, d, index="i64", vectorize=True):
+def scan_program(dtype, d, index="i64"):
     from ragged import ArtifactCache, Compiler, ScanSpec
-    return Compiler().compile(ScanSpec(dtype, d, index, vectorize=vectorize),
+    return Compiler().compile(ScanSpec(dtype, d, index),
                               ArtifactCache(_cache_dir(), max_specializations=4096))
 
 
@@ -62,12 +62,12 @@ def host(tensor):
     return None if tensor is None else tensor.float().cpu().numpy().astype(np.float64)
 
 
-def run(torch, case, dtype, index="i64", vectorize=True, backward=True, stream=None):
+def run(torch, case, dtype, index="i64", backward=True, stream=None):
     """Forward and backward through the public calls; guarded outputs."""
     t = device(torch, case, dtype, index)
     n, d = t["values"].shape
     b = t["offsets"].numel() - 1
-    program = scan_program(dtype, d, index, vectorize)
+    program = scan_program(dtype, d, index)
     kind = t["values"].dtype
     shapes = dict(out=((n, d), kind), final=((b, d), torch.float32), carries=((program.carry_rows(n), d), torch.float32),
                   grad_values=((n, d), kind), grad_gates=((n, d), kind), grad_initial=((b, d), torch.float32))
@@ -121,29 +121,37 @@ def test_widths(cuda, dtype, d):
     check(case, run(cuda, case, dtype, "i32"), dtype)
 
 
+@pytest.mark.parametrize("d", [16, 96])
+@pytest.mark.parametrize("shifts", [(1, 1, 1), (1, 0, 0), (0, 0, 1), (2, 4, 0)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-def test_unaligned_views_without_vectors(cuda, dtype):
+def test_unaligned_views(cuda, dtype, shifts, d):
+    """Views that start anywhere in their storage, states among them; the
+    recorded states serve a backward pass of other alignment."""
     torch = cuda
-    case = make_case([200, 3, 0, 90], 16, dtype, False)
+    case = make_case([200, 3, 0, 390], d, dtype, True)
     t = device(torch, case, dtype, "i64")
-    shifted = {}
-    for name in ("values", "gates"):
-        buffer = torch.empty(t[name].numel() + 1, dtype=t[name].dtype, device="cuda")
-        shifted[name] = buffer[1:].view_as(t[name])
-        shifted[name].copy_(t[name])
-    out = torch.empty_like(t["values"])
-    from ragged import ValidationError
-    with pytest.raises(ValidationError, match="aligned"):
-        scan_program(dtype, 16).run(shifted["values"], shifted["gates"], t["offsets"], out)
-    scan_program(dtype, 16, vectorize=False).run(shifted["values"], shifted["gates"], t["offsets"], out)
-    wide = [case[k].astype(np.float64) for k in ("values", "gates")]
-    ref.check_forward(ref.forward(*wide, case["offsets"]), host(out), None, dtype)
+
+    def shifted(x, by):
+        view = torch.empty(x.numel() + by, dtype=x.dtype, device="cuda")[by:].view_as(x)
+        return view.copy_(x)
+
+    values, gates, initial = (shifted(t[k], by) for k, by in zip(("values", "gates", "initial"), shifts))
+    program = scan_program(dtype, d)
+    empty = lambda x: torch.empty_like(x)  # noqa: E731
+    o = dict(out=shifted(empty(t["values"]), shifts[2]), final=empty(initial), grad_values=empty(t["values"]),
+             grad_gates=empty(t["values"]), grad_initial=empty(initial))
+    carries = torch.empty((program.carry_rows(593), d), device="cuda")
+    program.run(values, gates, t["offsets"], o["out"], initial=initial, final=o["final"], carries=carries)
+    program.run_backward(t["values"], t["gates"], t["offsets"], carries, t["grad_out"], initial=t["initial"],
+                         grad_final=t["grad_final"], grad_values=o["grad_values"], grad_gates=o["grad_gates"],
+                         grad_initial=o["grad_initial"])
+    check(case, {k: host(v) for k, v in o.items()}, dtype)
 
 
 @pytest.mark.parametrize("dtype,d,rows", [("f32", 32, 80_000), ("bf16", 66, 40_000)])
 def test_one_long_segment_passes_every_level_of_the_fold(cuda, dtype, d, rows):
-    """More than 256 chunks of 128 (64) rows, in one segment and with a start
-    in the middle; gates near one carry states over many chunks."""
+    """More than 256 chunks of 128 rows, in one segment and with a start in the
+    middle; gates near one carry states over many chunks."""
     for lengths in ([rows], [rows // 3, rows - rows // 3]):
         case = make_case(lengths, d, dtype, True, seed=5)
         case["gates"] = prepared(1 - (1 - case["gates"]) * 1e-3, dtype)

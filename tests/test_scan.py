@@ -27,7 +27,7 @@ def test_spec_round_trip_and_refusals():
     assert len({spec.ir_hash, ScanSpec("bf16", 256, "i32").ir_hash, ProgramSpec("sum", "bf16", 256, "i32").ir_hash,
                 MatmulSpec("bf16", 256, 256, "i32").ir_hash}) == 4
     for bad in (dict(dtype="f16"), dict(feature_dim=0), dict(feature_dim=65537), dict(feature_dim=2.0),
-                dict(offsets_dtype="i16"), dict(vectorize=1), dict(hints=None), dict(chip="sm_90")):
+                dict(offsets_dtype="i16"), dict(hints=None), dict(chip="sm_90")):
         with pytest.raises(ValidationError):
             ScanSpec(**bad)
     with pytest.raises(ValidationError):
@@ -42,48 +42,36 @@ def test_compile_caches_the_program(native_library, tmp_path):
     assert first.schedules == ("scan",)
 
 
-@pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("vectorize", [True, False])
-def test_recorded_rows_agree_with_the_library(native_library, dtype, vectorize):
-    from ragged import _native
-    from ragged.layers import scan_chunk_rows
-    for d in [*range(1, 150), 256, 1000, 1024, 65536]:
-        rows = scan_chunk_rows(dtype, d, vectorize)
-        for n in (0, 1, rows, rows + 1, 100_001):
-            flags = 0 if vectorize else _native.FLAG_NO_VECTORIZE
-            assert _native.scan_sizes(dtype, "i64", d, n, 3, flags)[1] == -(-n // rows)
-
-
 def test_abi_refuses_bad_arguments(native_library):
     from ragged import _native
     lib = native_library
-    one, rows = ctypes.c_int64(), ctypes.c_int64()
+    one = ctypes.c_int64()
 
     def sizes(dtype=0, index=1, d=8, n=4, b=1):
-        return lib.rg_scan_workspace_bytes(dtype, index, d, n, b, 0, ctypes.byref(one), ctypes.byref(rows))
+        return lib.rg_scan_workspace_bytes(dtype, index, d, n, b, ctypes.byref(one))
 
     assert sizes() == 0
     for bad in (dict(dtype=2), dict(index=5), dict(d=0), dict(d=65537), dict(n=-1), dict(b=-1), dict(b=0),
                 dict(n=2**31, index=0), dict(b=2**31), dict(n=2**62)):
         assert sizes(**bad) == _native.RG_ERR_INVALID_ARGUMENT, bad
-    assert lib.rg_scan_workspace_bytes(0, 1, 8, 4, 1, 0, None, ctypes.byref(rows)) == _native.RG_ERR_INVALID_ARGUMENT
+    assert lib.rg_scan_workspace_bytes(0, 1, 8, 4, 1, None) == _native.RG_ERR_INVALID_ARGUMENT
     buffer = (ctypes.c_char * 4096)()
     base = (ctypes.addressof(buffer) + 255) // 256 * 256
     v, g, o, out = base, base + 128, base + 256, base + 512
 
     def scan(values=v, gates=g, offsets=o, initial=None, out=out, final=None, carries=None):
-        return lib.rg_scan(0, 1, 8, 4, 1, values, gates, offsets, initial, out, final, carries, None, 0, 0, None, None)
+        return lib.rg_scan(0, 1, 8, 4, 1, values, gates, offsets, initial, out, final, carries, None, 0, None, None)
 
-    for bad in (dict(values=None), dict(gates=None), dict(offsets=None), dict(out=None), dict(values=v + 4),
+    for bad in (dict(values=None), dict(gates=None), dict(offsets=None), dict(out=None), dict(values=v + 2),
                 dict(out=v), dict(out=g + 16), dict(final=v), dict(final=out + 4), dict(carries=out),
                 dict(out=o - 64), dict(initial=base + 1024 + 2)):
         assert scan(**bad) == _native.RG_ERR_INVALID_ARGUMENT, bad
-    assert lib.rg_scan(0, 1, 8, 0, 0, *[None] * 8, 0, 0, None, None) == 0  # no segments: nothing to do
+    assert lib.rg_scan(0, 1, 8, 0, 0, *[None] * 8, 0, None, None) == 0  # no segments: nothing to do
     grads = dict(values=v, gates=g, offsets=o, initial=None, carries=base + 768, grad_out=base + 896, grad_final=None,
                  grad_values=base + 1024, grad_gates=base + 1152, grad_initial=None)
 
     def backward(**change):
-        return lib.rg_scan_backward(0, 1, 8, 4, 1, *dict(grads, **change).values(), None, 0, 0, None, None)
+        return lib.rg_scan_backward(0, 1, 8, 4, 1, *dict(grads, **change).values(), None, 0, None, None)
 
     for bad in (dict(carries=None), dict(grad_out=None), dict(grad_values=base + 896), dict(grad_gates=base + 1024),
                 dict(grad_initial=base + 1280), dict(grad_values=v)):
@@ -126,8 +114,7 @@ def test_fake_shapes_and_refusals(monkeypatch):
     assert out.shape == (700, 24) and out.dtype == torch.bfloat16
     assert final.shape == (4, 24) and final.dtype == torch.float32
     ops = torch.ops.ragged_mlir
-    rows = torch_adapter.scan_chunk_rows("bf16", 24)
-    assert ops.segment_scan(values, values, offsets, None, "scan-24")[2].shape == (-(-700 // rows), 24)
+    assert ops.segment_scan(values, values, offsets, None, "scan-24")[2].shape == (44, 24)
     assert ops.segment_scan(values, values, offsets, None, "scan-24", "validated", False)[2].shape == (0, 24)
     initial = torch.empty((4, 24), **meta)
     for bad in (dict(gates=values.float()), dict(gates=values[:5]), dict(initial=initial.bfloat16()),
