@@ -328,6 +328,17 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
 }
 
+// -------------------------------------------------- dependent launches --
+//
+// A kernel launched with programmatic stream serialization may start while
+// the one before it still runs; what it reads of that kernel's results comes
+// after grid_dependency_wait, which waits for its end.  The earlier kernel
+// allows the start with grid_dependents_launch (its blocks that run keep
+// their place; without the call the start is at its end).
+
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ------------------------------------------------ bulk copies (TMA, 1-D) --
 //
 // cp.async.bulk moves a contiguous, 16-byte aligned block of global memory

@@ -25,8 +25,7 @@ struct ScanShape {
 constexpr int64_t kAloneRows = 256;  // rows up to which walk is the only launch
 
 // 32 lanes, or as many as cover a row, of one vector each.  A lane takes 64
-// rows of a slab where that leaves the GPU's warps two tasks each, and 16 where
-// there are fewer.
+// rows of a slab, fewer where that would leave resident warps without a task.
 ScanShape make_shape(int dtype, int64_t d, int64_t n, int64_t b, bool aligned_pairs) {
   ScanShape s;
   s.pair = dtype == RG_DTYPE_BF16 && d % 2 == 0 ? 2 : 1;
@@ -37,7 +36,7 @@ ScanShape make_shape(int dtype, int64_t d, int64_t n, int64_t b, bool aligned_pa
   const int groups = 32 >> s.shift;
   constexpr int64_t warps = 148 * 24;
   s.lane_rows = 64;
-  while (s.lane_rows > 16 && (ceil_div(n, s.lane_rows * groups) * s.tiles < 2 * warps || s.lane_rows * groups > 512))
+  while (s.lane_rows > 16 && (ceil_div(n, s.lane_rows * groups) * s.tiles < warps || s.lane_rows * groups > 512))
     s.lane_rows /= 2;
   s.row_shift = 0;
   while ((1 << s.row_shift) < s.lane_rows * groups) ++s.row_shift;
@@ -113,27 +112,37 @@ template <typename T, typename OffT, int VEC, bool BACKWARD>
 int launch(const ScanArgs &p, const ScanShape &s, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
   const int smem = kScanWarps * scan_marks_words(1 << s.row_shift) * 4;
   constexpr int usual = kScanWarps * scan_marks_words(64) * 4, limit = kScanWarps * scan_marks_words(512) * 4;
-  auto run = [&](void (*kernel)(ScanArgs), int id, int64_t tasks) {
+  // The second and third launch may start before the one before them ends.
+  auto start = [&](void (*kernel)(ScanArgs), int id, int64_t ctas, int threads, int bytes, bool after) {
+    cudaLaunchAttribute serial;
+    serial.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    serial.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
+    config.blockDim = dim3(threads, 1, 1);
+    config.dynamicSmemBytes = bytes;
+    config.stream = stream;
+    config.attrs = &serial;
+    config.numAttrs = after ? 1 : 0;
+    record_launch(report, id, config.gridDim, threads, bytes);
+    return check_cuda(cudaLaunchKernelEx(&config, kernel, p), "scan kernel launch");
+  };
+  auto run = [&](void (*kernel)(ScanArgs), int id, int64_t tasks, bool after) {
     int per_sm = 0;
     int status = prepare_kernel(reinterpret_cast<const void *>(kernel), dev.device, kScanThreads, usual, limit, &per_sm);
     if (status) return status;
-    const int64_t ctas = std::min(static_cast<int64_t>(per_sm) * dev.sm_count, ceil_div(tasks, kScanWarps));
-    const dim3 grid(static_cast<unsigned>(ctas), 1, 1);
-    kernel<<<grid, kScanThreads, smem, stream>>>(p);
-    record_launch(report, id, grid, kScanThreads, smem);
-    return check_cuda(cudaGetLastError(), "scan kernel launch");
+    return start(kernel, id, std::min(static_cast<int64_t>(per_sm) * dev.sm_count, ceil_div(tasks, kScanWarps)),
+                 kScanThreads, smem, after);
   };
   if (p.pairs) {
     int status = run(scan_fold_kernel<T, OffT, VEC, BACKWARD>, BACKWARD ? K_SCAN_FOLD_BACKWARD : K_SCAN_FOLD,
-                     s.slabs * s.tiles);
+                     s.slabs * s.tiles, false);
     if (status) return status;
-    const dim3 grid(static_cast<unsigned>(ceil_div(p.d, 32)), 1, 1);
-    scan_join_kernel<<<grid, kScanJoinWarps * 32, 0, stream>>>(p);
-    record_launch(report, K_SCAN_JOIN, grid, kScanJoinWarps * 32, 0);
-    status = check_cuda(cudaGetLastError(), "scan_join_kernel launch");
+    status = start(scan_join_kernel, K_SCAN_JOIN, ceil_div(p.d, kJoinCols), kJoinCols * kJoinParts, 0, true);
     if (status) return status;
   }
-  return run(scan_walk_kernel<T, OffT, VEC, BACKWARD>, BACKWARD ? K_SCAN_BACKWARD : K_SCAN, s.blocks * s.tiles);
+  return run(scan_walk_kernel<T, OffT, VEC, BACKWARD>, BACKWARD ? K_SCAN_BACKWARD : K_SCAN, s.blocks * s.tiles,
+             p.pairs != nullptr);
 }
 
 template <typename OffT, bool BACKWARD>

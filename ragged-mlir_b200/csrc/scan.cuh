@@ -51,8 +51,9 @@ namespace rgb {
 constexpr int kScanThreads = 256;
 constexpr int kScanWarps = kScanThreads / 32;
 constexpr int kScanBatch = 16;    // rows of a lane in flight; rows per recorded state
-constexpr int kScanAhead = 8;     // pairs that a join has on their way
-constexpr int kScanJoinWarps = 32;
+constexpr int kJoinCols = 8;      // columns of a join's block
+constexpr int kJoinParts = 128;   // parts that it cuts the slabs into, a thread each
+constexpr int kJoinBatch = 8;     // pairs of a thread in flight
 
 struct ScanArgs {
   const void *values, *gates, *offsets;
@@ -383,6 +384,7 @@ struct ScanWarp {
 template <typename T, typename OffT, int VEC, bool BACKWARD>
 __global__ void __launch_bounds__(kScanThreads, 3) scan_fold_kernel(const ScanArgs p) {
   extern __shared__ unsigned scan_smem[];
+  grid_dependents_launch();
   ScanWarp<T, OffT, VEC, BACKWARD> w(p, scan_smem);
   const unsigned tasks = static_cast<unsigned>(p.slabs * p.tiles);
   for (unsigned t = blockIdx.x * kScanWarps + (threadIdx.x >> 5); t < tasks; t += gridDim.x * kScanWarps) {
@@ -403,47 +405,79 @@ __global__ void __launch_bounds__(kScanThreads, 3) scan_fold_kernel(const ScanAr
   }
 }
 
-// 32 columns a block; each warp composes the pairs of a part of the slabs,
-// then all go through the parts before theirs, then each through its own.
-__global__ void __launch_bounds__(kScanJoinWarps * 32) scan_join_kernel(const ScanArgs p) {
-  __shared__ float part_a[kScanJoinWarps][32], part_h[kScanJoinWarps][32];
-  __shared__ bool part_reset[kScanJoinWarps][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+// (a, h) of rows, and whether a segment starts in them (a does not count then).
+struct ScanSpan {
+  float a, h;
+  bool reset;
+  // This span after `first`.
+  __device__ __forceinline__ void after(const ScanSpan &first) {
+    if (reset) return;
+    h = scan_apply(a, h, first.h);
+    a *= first.a;
+    reset = first.reset;
+  }
+};
+
+__device__ __forceinline__ ScanSpan scan_span(const float2 &pair) {
+  return ScanSpan{pair.x, pair.y, __float_as_uint(pair.x) == kScanReset};
+}
+
+// 8 columns by 128 parts of the slabs a block: each thread composes its part,
+// a doubling scan over the parts gives the state before each, and each thread
+// goes through its part again (from registers up to 8 slabs a part).
+__global__ void __launch_bounds__(kJoinCols * kJoinParts) scan_join_kernel(const ScanArgs p) {
+  __shared__ ScanSpan spans[2][kJoinParts][kJoinCols];
+  const int c = threadIdx.x % kJoinCols, part = threadIdx.x / kJoinCols;
+  const int64_t col = static_cast<int64_t>(blockIdx.x) * kJoinCols + c;
   const bool live = col < p.d;
-  const int64_t per = (p.slabs + kScanJoinWarps - 1) / kScanJoinWarps;
-  const int64_t begin = min(warp * per, p.slabs), end = min(begin + per, p.slabs);
-  float a = 1.0f, h = 0.0f;
-  bool reset = false;
-  auto each = [&](auto act) {
-#pragma unroll 1
-    for (int64_t s = begin; s < end; s += kScanAhead) {
-      float2 pair[kScanAhead];
+  const int64_t per = (p.slabs + kJoinParts - 1) / kJoinParts;
+  const int64_t begin = min(part * per, p.slabs), end = live ? min(begin + per, p.slabs) : begin;
+  const float2 *pairs = p.pairs + col;
+  float *states = p.states + col;
+  float2 pair[kJoinBatch];
+  auto load = [&](int64_t s) {
 #pragma unroll
-      for (int i = 0; i < kScanAhead; ++i)
-        if (live && s + i < end) pair[i] = p.pairs[(s + i) * p.d + col];
-#pragma unroll
-      for (int i = 0; i < kScanAhead; ++i)
-        if (live && s + i < end) act(s + i, pair[i]);
-    }
+    for (int i = 0; i < kJoinBatch; ++i)
+      if (s + i < end) pair[i] = pairs[(s + i) * p.d];
   };
-  each([&](int64_t, const float2 &x) {
-    const bool starts = __float_as_uint(x.x) == kScanReset;
-    h = starts ? x.y : scan_apply(x.x, x.y, h);
-    a *= x.x;
-    reset |= starts;
-  });
-  part_a[warp][lane] = a;
-  part_h[warp][lane] = h;
-  part_reset[warp][lane] = reset;
+  grid_dependents_launch();
+  grid_dependency_wait();
+  ScanSpan all{1.0f, 0.0f, false};
+#pragma unroll 1
+  for (int64_t s = begin; s < end; s += kJoinBatch) {
+    load(s);
+#pragma unroll
+    for (int i = 0; i < kJoinBatch; ++i) {
+      if (s + i < end) {
+        ScanSpan next = scan_span(pair[i]);
+        next.after(all);
+        all = next;
+      }
+    }
+  }
+  int from = 0;
+  spans[0][part][c] = all;
   __syncthreads();
-  float state = 0.0f;
-  for (int w = 0; w < warp; ++w)
-    state = part_reset[w][lane] ? part_h[w][lane] : scan_apply(part_a[w][lane], part_h[w][lane], state);
-  each([&](int64_t s, const float2 &x) {
-    p.states[s * p.d + col] = state;
-    state = __float_as_uint(x.x) == kScanReset ? x.y : scan_apply(x.x, x.y, state);
-  });
+#pragma unroll 1
+  for (int off = 1; off < kJoinParts; off <<= 1) {
+    if (part >= off) all.after(spans[from][part - off][c]);
+    spans[from ^ 1][part][c] = all;
+    from ^= 1;
+    __syncthreads();
+  }
+  float state = part ? spans[from][part - 1][c].h : 0.0f;
+#pragma unroll 1
+  for (int64_t s = begin; s < end; s += kJoinBatch) {
+    if (per > kJoinBatch) load(s);
+#pragma unroll
+    for (int i = 0; i < kJoinBatch; ++i) {
+      if (s + i < end) {
+        states[(s + i) * p.d] = state;
+        const ScanSpan x = scan_span(pair[i]);
+        state = x.reset ? x.h : scan_apply(x.a, x.h, state);
+      }
+    }
+  }
 }
 
 template <typename T, typename OffT, int VEC, bool BACKWARD>
@@ -469,6 +503,7 @@ __global__ void __launch_bounds__(kScanThreads, BACKWARD ? 2 : 3) scan_walk_kern
       if (!p.pairs) {
         w.catch_up(h);
       } else {
+        grid_dependency_wait();
         ScanPair<VEC> f, total;
         int reset = 0, total_reset;
         f.clear();
