@@ -296,6 +296,30 @@ int rg_scan_backward(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b
                      float *grad_initial, void *workspace, int64_t workspace_bytes, void *stream,
                      rg_report *report);
 
+/* ----------------------------------------------- segmented matrix product
+ * This build's extension (the reference has no such operation): the rows of
+ * segment s times a matrix of its own, and the two products of the backward
+ * pass.  K columns in, M columns out, 1 <= K, M <= 65536, all row-major and
+ * contiguous, of one dtype; offsets as everywhere.
+ *   kind                          left              right            out
+ *   RG_MATMUL_FORWARD             values [N, K]     weights [B,K,M]  [N, M]
+ *   RG_MATMUL_GRAD_VALUES         grad_out [N, M]   weights [B,K,M]  [N, K]
+ *   RG_MATMUL_GRAD_WEIGHTS        values [N, K]     grad_out [N, M]  [B, K, M]
+ * Sums are f32, rounded once.  A segment without rows has zeros for the
+ * gradient of its weights; its weights are not read.  out overlaps nothing.
+ * bf16 runs on the tensor cores, f32 in f32 arithmetic.
+ *
+ * rg_matmul_workspace_bytes: scratch of a call (256-byte aligned; 0: none),
+ * for tensors at these addresses: bf16 rows that do not start at 16-byte
+ * boundaries are copied to some that do.  Where rg_report.status_offset is not
+ * -1, a word for each CTA of the last launch is there (nonzero: a wait gave up). */
+enum rg_matmul_kind { RG_MATMUL_FORWARD = 0, RG_MATMUL_GRAD_VALUES = 1, RG_MATMUL_GRAD_WEIGHTS = 2 };
+int rg_matmul_workspace_bytes(int kind, int dtype, int index_dtype, int64_t k, int64_t m, int64_t n, int64_t b,
+                              const void *left, const void *right, int64_t *bytes);
+int rg_matmul(int kind, int dtype, int index_dtype, int64_t k, int64_t m, int64_t n, int64_t b, const void *left,
+              const void *right, const void *offsets, void *out, void *workspace, int64_t workspace_bytes,
+              void *stream, rg_report *report);
+
 /* ------------------------------------------------------- schedule choice
  * This build's extension (the reference chooses in Python,
  * python/ragged/selection.py:106-126): the scores of the boosted decision

@@ -63,6 +63,9 @@ enum KernelId : int {
   K_SCAN_FOLD = 16,
   K_SCAN_FOLD_BACKWARD = 17,
   K_SCAN_JOIN = 18,
+  K_MATMUL_SIMT = 19,
+  K_MATMUL_TENSOR = 20,
+  K_MATMUL_PACK = 21,
 };
 
 // Recording helper for rg_report.
@@ -82,11 +85,27 @@ int check_device(DeviceProps *props);     // current device must be sm_100
 // current device, once, and gives the CTAs of `threads` with `smem` bytes that
 // an SM holds (cached per kernel and device).
 int prepare_kernel(const void *kernel, int device, int threads, int smem, int smem_limit, int *per_sm);
-// Tensor map of `rows` rows of `cols` elements (16-byte aligned rows), loaded
-// in boxes; with `swizzle` a box is 128 bytes wide and its 16-byte pieces are
-// permuted within groups of 8 rows as tcgen05's 128-byte swizzle expects.
-int make_tensor_map_2d(CUtensorMap *map, int dtype, const void *base, int64_t rows, int64_t cols, int box_rows,
-                       int box_cols, bool swizzle);
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+inline int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
+
+// Checks of the learned operators' tensors: NULL where there are bytes,
+// misaligned, or written and overlapping another.
+struct TensorRange {
+  const char *name;
+  const void *ptr;
+  int64_t bytes;
+  int align;
+  bool written;
+};
+int check_ranges(const TensorRange *ranges, int count);
+void clear_report(rg_report *report);
+
+// Tensor map of a bf16 tensor of `rank` (2 or 3) dimensions, the innermost
+// first; `strides` (elements, of the outer dimensions) are multiples of 8 and
+// `base` is 16-byte aligned.  Its boxes are 128 bytes wide, and their 16-byte
+// pieces permuted within groups of 8 rows (the 128-byte swizzle of tcgen05).
+int make_tensor_map(CUtensorMap *map, const void *base, int rank, const int64_t *dims, const int64_t *strides,
+                    const int *box);
 
 // Per-schedule entry points (launch on stream, record into report).
 int launch_naive(const Problem &p, const Geometry &g, cudaStream_t stream, rg_report *report);

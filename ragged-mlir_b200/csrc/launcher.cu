@@ -100,6 +100,38 @@ int device_props(DeviceProps *props) {
   return RG_OK;
 }
 
+int check_ranges(const TensorRange *r, int count) {
+  char buffer[200];
+  for (int i = 0; i < count; ++i) {
+    if (!r[i].bytes) continue;
+    if (!r[i].ptr) {
+      std::snprintf(buffer, sizeof buffer, "%s pointer is NULL", r[i].name);
+      return fail(RG_ERR_INVALID_ARGUMENT, buffer);
+    }
+    if (!aligned(r[i].ptr, r[i].align)) {
+      std::snprintf(buffer, sizeof buffer, "%s must be %d-byte aligned", r[i].name, r[i].align);
+      return fail(RG_ERR_INVALID_ARGUMENT, buffer);
+    }
+  }
+  for (int i = 0; i < count; ++i)
+    for (int j = 0; j < count; ++j) {
+      if (i == j || !r[i].written || !r[i].bytes || !r[j].bytes) continue;
+      const uintptr_t a = reinterpret_cast<uintptr_t>(r[i].ptr), b = reinterpret_cast<uintptr_t>(r[j].ptr);
+      if (a < b + r[j].bytes && b < a + r[i].bytes) {
+        std::snprintf(buffer, sizeof buffer, "%s overlaps %s", r[i].name, r[j].name);
+        return fail(RG_ERR_INVALID_ARGUMENT, buffer);
+      }
+    }
+  return RG_OK;
+}
+
+void clear_report(rg_report *report) {
+  if (!report) return;
+  std::memset(report, 0, sizeof *report);
+  report->status_offset = -1;
+  report->streams = 1;
+}
+
 int prepare_kernel(const void *kernel, int device, int threads, int smem, int smem_limit, int *per_sm) {
   std::lock_guard<std::mutex> lock(g_prepared_mutex);
   for (int i = 0; i < g_prepared_count; ++i) {
@@ -121,8 +153,8 @@ int prepare_kernel(const void *kernel, int device, int threads, int smem, int sm
   return RG_OK;
 }
 
-int make_tensor_map_2d(CUtensorMap *map, int dtype, const void *base, int64_t rows, int64_t cols, int box_rows,
-                       int box_cols, bool swizzle) {
+int make_tensor_map(CUtensorMap *map, const void *base, int rank, const int64_t *dims, const int64_t *strides,
+                    const int *box) {
   using Encode = decltype(&cuTensorMapEncodeTiled);
   static std::atomic<void *> cached{nullptr};
   void *entry = cached.load();
@@ -136,14 +168,17 @@ int make_tensor_map_2d(CUtensorMap *map, int dtype, const void *base, int64_t ro
       return fail(RG_ERR_DEVICE, "the CUDA driver has no cuTensorMapEncodeTiled");
     cached.store(entry);
   }
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols * elem_bytes(dtype))};
-  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
-  const cuuint32_t steps[2] = {1, 1};
+  cuuint64_t sizes[3], pitches[2];
+  cuuint32_t boxes[3];
+  const cuuint32_t steps[3] = {1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    sizes[i] = static_cast<cuuint64_t>(dims[i]);
+    boxes[i] = static_cast<cuuint32_t>(box[i]);
+    if (i + 1 < rank) pitches[i] = static_cast<cuuint64_t>(strides[i] * 2);
+  }
   const CUresult result = reinterpret_cast<Encode>(entry)(
-      map, dtype == RG_DTYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-      const_cast<void *>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-      swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank), const_cast<void *>(base), sizes, pitches,
+      boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (result != CUDA_SUCCESS) {
     char buffer[96];
@@ -277,6 +312,9 @@ const char *rg_kernel_name(int kernel_id) {
     case K_SCAN_FOLD: return "scan_fold";
     case K_SCAN_FOLD_BACKWARD: return "scan_fold_backward";
     case K_SCAN_JOIN: return "scan_join";
+    case K_MATMUL_SIMT: return "matmul_simt";
+    case K_MATMUL_TENSOR: return "matmul_tensor";
+    case K_MATMUL_PACK: return "matmul_pack";
   }
   return "";
 }

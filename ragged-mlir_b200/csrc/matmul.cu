@@ -1,0 +1,255 @@
+// Launch code of the segmented matrix products (kernels: matmul_tensor.cuh for
+// bf16, matmul_simt.cuh for f32).
+#include <algorithm>
+#include <cstring>
+
+#include "internal.h"
+#include "matmul_simt.cuh"
+#include "matmul_tensor.cuh"
+
+namespace rgb {
+
+namespace {
+
+constexpr int64_t kMaxWidth = 65536;
+
+struct MatmulShape {
+  int64_t rows, cols, depth;         // rows (depth) of a segment's product in the weights kind (else): N
+  int64_t left_rows, left_cols;      // operands as matrices
+  int64_t right_rows, right_cols;
+  int64_t left_pitch, right_pitch;   // after packing
+  bool pack_left, pack_right;
+  int64_t left_at, right_at, bytes;  // workspace
+};
+
+int64_t status_bytes() { return 1024 * 8; }
+
+bool takes_tma(const void *p, int64_t cols) { return cols % 8 == 0 && aligned(p, 16); }
+
+MatmulShape make_shape(int kind, int dtype, int64_t k, int64_t m, int64_t n, int64_t b, const void *left,
+                       const void *right) {
+  MatmulShape s{};
+  s.rows = kind == MATMUL_GRAD_WEIGHTS ? k : n;
+  s.cols = kind == MATMUL_GRAD_VALUES ? k : m;
+  s.depth = kind == MATMUL_FORWARD ? k : kind == MATMUL_GRAD_VALUES ? m : n;
+  s.left_rows = n;
+  s.left_cols = kind == MATMUL_GRAD_VALUES ? m : k;
+  s.right_rows = kind == MATMUL_GRAD_WEIGHTS ? n : b * k;
+  s.right_cols = m;
+  s.left_pitch = s.left_cols;
+  s.right_pitch = s.right_cols;
+  if (dtype == RG_DTYPE_F32) return s;
+  s.bytes = status_bytes();
+  if (!takes_tma(left, s.left_cols)) {
+    s.pack_left = true;
+    s.left_pitch = (s.left_cols + 7) / 8 * 8;
+    s.left_at = s.bytes;
+    s.bytes = align256(s.bytes + s.left_rows * s.left_pitch * 2);
+  }
+  if (!takes_tma(right, s.right_cols)) {
+    s.pack_right = true;
+    s.right_pitch = (s.right_cols + 7) / 8 * 8;
+    s.right_at = s.bytes;
+    s.bytes = align256(s.bytes + s.right_rows * s.right_pitch * 2);
+  }
+  return s;
+}
+
+int check_shape(int kind, int dtype, int index_dtype, int64_t k, int64_t m, int64_t n, int64_t b) {
+  if (kind < MATMUL_FORWARD || kind > MATMUL_GRAD_WEIGHTS)
+    return fail(RG_ERR_INVALID_ARGUMENT, "kind must be forward, gradient of values or gradient of weights");
+  if (dtype != RG_DTYPE_F32 && dtype != RG_DTYPE_BF16) return fail(RG_ERR_INVALID_ARGUMENT, "dtype must be f32 or bf16");
+  if (index_dtype != RG_INDEX_I32 && index_dtype != RG_INDEX_I64)
+    return fail(RG_ERR_INVALID_ARGUMENT, "offsets dtype must be i32 or i64");
+  if (k < 1 || k > kMaxWidth || m < 1 || m > kMaxWidth)
+    return fail(RG_ERR_INVALID_ARGUMENT, "K and M must lie in [1, 65536]");
+  if (n < 0 || b < 0) return fail(RG_ERR_INVALID_ARGUMENT, "N and B must be nonnegative");
+  if (b == 0 && n != 0) return fail(RG_ERR_INVALID_ARGUMENT, "B=0 requires N=0");
+  if (n > 2147483647LL || b > 2147483647LL)
+    return fail(RG_ERR_INVALID_ARGUMENT, "a matrix product takes up to 2^31 - 1 rows and segments");
+  if (b > INT64_MAX / 16 / (k * m)) return fail(RG_ERR_INVALID_ARGUMENT, "tensor byte size overflows signed 64-bit");
+  return RG_OK;
+}
+
+// Row tiles of `tile` rows, at most: a segment has one that is not full.
+int64_t most_row_tiles(int kind, const MatmulArgs &p, int tile) {
+  return kind == MATMUL_GRAD_WEIGHTS ? p.b * ceil_div(p.k, tile) : p.n / tile + std::min(p.n, p.b);
+}
+
+template <typename OffT, int KIND, int TILE>
+int launch_simt_tile(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
+  const auto kernel = matmul_simt_kernel<OffT, KIND, TILE>;
+  int per_sm = 0;
+  const int status = prepare_kernel(reinterpret_cast<const void *>(kernel), dev.device, kSimtThreads, 0, 0, &per_sm);
+  if (status) return status;
+  p.col_tiles = static_cast<int>(ceil_div(p.cols, TILE));
+  p.row_tiles = static_cast<int>(ceil_div(p.k, TILE));
+  const int64_t tiles = most_row_tiles(KIND, p, TILE) * p.col_tiles;
+  const dim3 grid(static_cast<unsigned>(std::min(tiles, static_cast<int64_t>(per_sm) * dev.sm_count)), 1, 1);
+  kernel<<<grid, kSimtThreads, 0, stream>>>(p);
+  record_launch(report, K_MATMUL_SIMT, grid, kSimtThreads, 0);
+  return check_cuda(cudaGetLastError(), "matmul_simt_kernel launch");
+}
+
+// 128 x 128 tiles where they give every SM one, 64 x 64 where they do not.
+template <typename OffT, int KIND>
+int launch_simt(const MatmulArgs &p, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
+  const int64_t tiles =
+      (KIND == MATMUL_GRAD_WEIGHTS ? p.b * ceil_div(p.k, 128) : ceil_div(p.n, 128)) * ceil_div(p.cols, 128);
+  if (tiles >= dev.sm_count) return launch_simt_tile<OffT, KIND, 128>(p, dev, stream, report);
+  return launch_simt_tile<OffT, KIND, 64>(p, dev, stream, report);
+}
+
+template <typename OffT, int KIND, int COLS>
+int launch_tensor_cols(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
+  const auto kernel = matmul_tensor_kernel<OffT, KIND, COLS>;
+  const int smem = tensor_smem_bytes(COLS);
+  int per_sm = 0;
+  int status = prepare_kernel(reinterpret_cast<const void *>(kernel), dev.device, kTensorThreads, smem, smem, &per_sm);
+  if (status) return status;
+  TensorMaps maps;
+  std::memset(&maps, 0, sizeof maps);
+  constexpr bool weights = KIND == MATMUL_GRAD_WEIGHTS;
+  const int64_t left_cols = KIND == MATMUL_GRAD_VALUES ? p.m : p.k;
+  const int64_t left_dims[2] = {left_cols, p.n};
+  const int left_box[2] = {64, weights ? kTensorDepth : 32};
+  status = make_tensor_map(&maps.left, p.left, 2, left_dims, &p.left_pitch, left_box);
+  if (status) return status;
+  if (weights) {
+    const int64_t dims[2] = {p.m, p.n};
+    const int box[2] = {64, kTensorDepth};
+    status = make_tensor_map(&maps.right, p.right, 2, dims, &p.right_pitch, box);
+  } else {
+    const int64_t dims[3] = {p.m, p.k, p.b}, strides[2] = {p.right_pitch, p.right_pitch * p.k};
+    const int box[3] = {64, KIND == MATMUL_FORWARD ? kTensorDepth : COLS, 1};
+    status = make_tensor_map(&maps.right, p.right, 3, dims, strides, box);
+  }
+  if (status) return status;
+  p.col_tiles = static_cast<int>(ceil_div(p.cols, COLS));
+  p.row_tiles = static_cast<int>(ceil_div(p.k, kTensorRows));
+  const int64_t tiles = most_row_tiles(KIND, p, kTensorRows) * p.col_tiles;
+  const dim3 grid(static_cast<unsigned>(std::min(tiles, static_cast<int64_t>(std::min(dev.sm_count, 1024)))), 1, 1);
+  kernel<<<grid, kTensorThreads, smem, stream>>>(p, maps);
+  record_launch(report, K_MATMUL_TENSOR, grid, kTensorThreads, smem);
+  return check_cuda(cudaGetLastError(), "matmul_tensor_kernel launch");
+}
+
+// The widest tiles that give every SM one (a segment's last row tile counted half).
+template <typename OffT, int KIND>
+int launch_tensor(const MatmulArgs &p, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
+  const int64_t row_tiles = KIND == MATMUL_GRAD_WEIGHTS ? p.b * ceil_div(p.k, kTensorRows)
+                                                         : p.n / kTensorRows + std::max<int64_t>(std::min(p.n, p.b) / 2, 1);
+  if (p.cols > 128 && row_tiles * ceil_div(p.cols, 256) >= dev.sm_count)
+    return launch_tensor_cols<OffT, KIND, 256>(p, dev, stream, report);
+  if (p.cols > 64 && row_tiles * ceil_div(p.cols, 128) >= dev.sm_count)
+    return launch_tensor_cols<OffT, KIND, 128>(p, dev, stream, report);
+  return launch_tensor_cols<OffT, KIND, 64>(p, dev, stream, report);
+}
+
+template <typename OffT>
+int launch_kind(int kind, int dtype, const MatmulArgs &p, const DeviceProps &dev, cudaStream_t stream,
+                rg_report *report) {
+  if (dtype == RG_DTYPE_F32) {
+    if (kind == MATMUL_FORWARD) return launch_simt<OffT, MATMUL_FORWARD>(p, dev, stream, report);
+    if (kind == MATMUL_GRAD_VALUES) return launch_simt<OffT, MATMUL_GRAD_VALUES>(p, dev, stream, report);
+    return launch_simt<OffT, MATMUL_GRAD_WEIGHTS>(p, dev, stream, report);
+  }
+  if (kind == MATMUL_FORWARD) return launch_tensor<OffT, MATMUL_FORWARD>(p, dev, stream, report);
+  if (kind == MATMUL_GRAD_VALUES) return launch_tensor<OffT, MATMUL_GRAD_VALUES>(p, dev, stream, report);
+  return launch_tensor<OffT, MATMUL_GRAD_WEIGHTS>(p, dev, stream, report);
+}
+
+int pack(const void *from, void *to, int64_t rows, int64_t cols, int64_t pitch, const DeviceProps &dev,
+         cudaStream_t stream, rg_report *report) {
+  if (rows == 0) return RG_OK;
+  const dim3 grid(static_cast<unsigned>(std::min(ceil_div(rows, 8), static_cast<int64_t>(dev.sm_count) * 8)), 1, 1);
+  matmul_pack_kernel<<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16 *>(from),
+                                               static_cast<__nv_bfloat16 *>(to), rows, cols, pitch);
+  record_launch(report, K_MATMUL_PACK, grid, 256, 0);
+  return check_cuda(cudaGetLastError(), "matmul_pack_kernel launch");
+}
+
+}  // namespace
+
+}  // namespace rgb
+
+using namespace rgb;
+
+extern "C" {
+
+int rg_matmul_workspace_bytes(int kind, int dtype, int index_dtype, int64_t k, int64_t m, int64_t n, int64_t b,
+                              const void *left, const void *right, int64_t *bytes) {
+  if (!bytes) return fail(RG_ERR_INVALID_ARGUMENT, "bytes is NULL");
+  const int status = check_shape(kind, dtype, index_dtype, k, m, n, b);
+  if (status) return status;
+  *bytes = make_shape(kind, dtype, k, m, n, b, left, right).bytes;
+  return RG_OK;
+}
+
+int rg_matmul(int kind, int dtype, int index_dtype, int64_t k, int64_t m, int64_t n, int64_t b, const void *left,
+              const void *right, const void *offsets, void *out, void *workspace, int64_t workspace_bytes,
+              void *stream, rg_report *report) {
+  clear_report(report);
+  int status = check_shape(kind, dtype, index_dtype, k, m, n, b);
+  if (status) return status;
+  const MatmulShape s = make_shape(kind, dtype, k, m, n, b, left, right);
+  const int esize = elem_bytes(dtype), isize = index_dtype == RG_INDEX_I32 ? 4 : 8;
+  const int64_t out_bytes = (kind == MATMUL_GRAD_WEIGHTS ? b * k * m : n * s.cols) * esize;
+  if (b == 0 || out_bytes == 0) return RG_OK;
+  const TensorRange ranges[] = {
+      {"the left operand", left, s.left_rows * s.left_cols * esize, esize, false},
+      {"the right operand", right, s.right_rows * s.right_cols * esize, esize, false},
+      {"offsets", offsets, (b + 1) * isize, isize, false},
+      {"out", out, out_bytes, esize, true}};
+  status = check_ranges(ranges, 4);
+  if (status) return status;
+  DeviceProps dev;
+  status = check_device(&dev);
+  if (status) return status;
+  cudaStream_t on = static_cast<cudaStream_t>(stream);
+  if (kind == MATMUL_GRAD_WEIGHTS && n == 0) {  // no rows at all: no operand to map
+    if (report) report->memsets = 1;
+    return check_cuda(cudaMemsetAsync(out, 0, out_bytes, on), "cudaMemsetAsync");
+  }
+  if (report) {
+    report->workspace_bytes = s.bytes;
+    report->d_vector = 1;
+    report->d_tile = 1;
+    report->status_offset = s.bytes ? 0 : -1;
+  }
+  if (s.bytes) {
+    if (!workspace || workspace_bytes < s.bytes) return fail(RG_ERR_WORKSPACE, "workspace missing or too small");
+    if (!aligned(workspace, 256)) return fail(RG_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  }
+  MatmulArgs p{};
+  p.left = left;
+  p.right = right;
+  p.offsets = offsets;
+  p.out = out;
+  p.n = n;
+  p.b = b;
+  p.k = k;
+  p.m = m;
+  p.rows = s.rows;
+  p.cols = s.cols;
+  p.depth = s.depth;
+  p.left_pitch = s.left_pitch;
+  p.right_pitch = s.right_pitch;
+  p.out_pitch = s.cols;
+  p.status = static_cast<unsigned long long *>(workspace);
+  char *scratch = static_cast<char *>(workspace);
+  if (s.pack_left) {
+    p.left = scratch + s.left_at;
+    status = pack(left, scratch + s.left_at, s.left_rows, s.left_cols, s.left_pitch, dev, on, report);
+    if (status) return status;
+  }
+  if (s.pack_right) {
+    p.right = scratch + s.right_at;
+    status = pack(right, scratch + s.right_at, s.right_rows, s.right_cols, s.right_pitch, dev, on, report);
+    if (status) return status;
+  }
+  if (index_dtype == RG_INDEX_I32) return launch_kind<int32_t>(kind, dtype, p, dev, on, report);
+  return launch_kind<int64_t>(kind, dtype, p, dev, on, report);
+}
+
+}  // extern "C"

@@ -1,0 +1,99 @@
+// Segmented matrix products: out[t] = left[t] @ right[s] for the rows t of
+// segment s, and the two products of its backward pass.
+//
+//   kind     out                  left (rows x contraction)   right
+//   forward  [N, M]               values [N, K]               weights[s] [K, M]
+//   values   [N, K] (gradient)    grad_out [N, M]             weights[s] transposed
+//   weights  [s] [K, M] (grad.)   values_s transposed         grad_out_s
+//
+// This file has what both kernels share: the list of output tiles, which the
+// device derives from the offsets.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace rgb {
+
+enum MatmulKind : int { MATMUL_FORWARD = 0, MATMUL_GRAD_VALUES = 1, MATMUL_GRAD_WEIGHTS = 2 };
+
+struct MatmulArgs {
+  const void *left, *right, *offsets;
+  void *out;
+  int64_t n, b;
+  int64_t k, m;              // widths of values and of out (forward)
+  int64_t rows, cols, depth; // of a product; for the kinds whose rows (depth) are a segment's: unused
+  int64_t left_pitch, right_pitch, out_pitch;  // elements between rows
+  int col_tiles;
+  int row_tiles;             // weights kind: row tiles of a segment
+  unsigned long long *status;
+};
+
+// One output tile: rows [row, row_end) of the output (of segment `seg` for the
+// weights kind), and the segment's rows [begin, end).
+struct MatmulTile {
+  int64_t seg, row, row_end, begin, end;
+  int col_tile;
+};
+
+// Walks a CTA's tiles, in ascending order.  Forward and values: the tiles of a
+// segment are its rows in steps of TILE, so the segment of a tile is found by
+// counting them, 32 segments at a time and on from the last one found.  All
+// lanes of a warp take part and get the same answer.
+template <typename OffT, int KIND, int TILE>
+struct MatmulWalk {
+  const OffT *__restrict__ offsets;
+  int64_t b, first, before;  // tiles before segment `first`
+  __device__ __forceinline__ MatmulWalk(const void *o, int64_t segments)
+      : offsets(static_cast<const OffT *>(o)), b(segments), first(0), before(0) {}
+
+  // False past the last tile.  `n` clamps offsets that are out of order.
+  __device__ __forceinline__ bool find(const MatmulArgs &p, int64_t index, MatmulTile &t) {
+    t.col_tile = static_cast<int>(index % p.col_tiles);
+    const int64_t tile = index / p.col_tiles;
+    if constexpr (KIND == MATMUL_GRAD_WEIGHTS) {
+      t.seg = tile / p.row_tiles;
+      if (t.seg >= b) return false;
+      t.row = (tile - t.seg * p.row_tiles) * TILE;
+      t.row_end = min(t.row + TILE, p.rows);
+      t.begin = min(max(static_cast<int64_t>(offsets[t.seg]), int64_t{0}), p.n);
+      t.end = max(min(static_cast<int64_t>(offsets[t.seg + 1]), p.n), t.begin);
+      return true;
+    } else {
+      const int lane = threadIdx.x & 31;
+      for (;;) {
+        if (first >= b) return false;
+        const int64_t s = first + lane;
+        int64_t lo = 0, hi = 0;
+        if (s < b) {
+          lo = min(max(static_cast<int64_t>(offsets[s]), int64_t{0}), p.n);
+          hi = max(min(static_cast<int64_t>(offsets[s + 1]), p.n), lo);
+        }
+        int64_t sum = (hi - lo + TILE - 1) / TILE;  // tiles up to this lane's segment
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const int64_t up = __shfl_up_sync(~0u, sum, off);
+          if (lane >= off) sum += up;
+        }
+        const unsigned past = __ballot_sync(~0u, before + sum > tile);
+        if (past) {
+          const int src = __ffs(past) - 1;
+          const int64_t up = __shfl_up_sync(~0u, sum, 1);
+          const int64_t start = __shfl_sync(~0u, lane ? up : int64_t{0}, src) + before;
+          t.begin = __shfl_sync(~0u, lo, src);
+          t.end = __shfl_sync(~0u, hi, src);
+          t.seg = first + src;
+          t.row = t.begin + (tile - start) * TILE;
+          t.row_end = min(t.row + TILE, t.end);
+          return true;
+        }
+        before += __shfl_sync(~0u, sum, 31);
+        first += 32;
+      }
+    }
+  }
+};
+
+}  // namespace rgb

@@ -12,8 +12,6 @@ namespace {
 
 constexpr int64_t kMaxScanDim = 65536;
 
-int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
-int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
 struct ScanShape {
   int pair;            // elements of 4 bytes of a row (1 where D is odd)
@@ -66,43 +64,8 @@ int check_shape(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b) {
   return RG_OK;
 }
 
-struct Range {
-  const char *name;
-  const void *ptr;
-  int64_t bytes;
-  int align;
-  bool written;
-};
-
-// Null pointers of tensors with bytes, misaligned ones, and written tensors
-// that overlap any other.
-int check_ranges(const Range *r, int count) {
-  char buffer[200];
-  for (int i = 0; i < count; ++i) {
-    if (!r[i].bytes) continue;
-    if (!r[i].ptr) {
-      std::snprintf(buffer, sizeof buffer, "%s pointer is NULL", r[i].name);
-      return fail(RG_ERR_INVALID_ARGUMENT, buffer);
-    }
-    if (!aligned(r[i].ptr, r[i].align)) {
-      std::snprintf(buffer, sizeof buffer, "%s must be %d-byte aligned", r[i].name, r[i].align);
-      return fail(RG_ERR_INVALID_ARGUMENT, buffer);
-    }
-  }
-  for (int i = 0; i < count; ++i)
-    for (int j = 0; j < count; ++j) {
-      if (i == j || !r[i].written || !r[i].bytes || !r[j].bytes) continue;
-      const uintptr_t a = reinterpret_cast<uintptr_t>(r[i].ptr), b = reinterpret_cast<uintptr_t>(r[j].ptr);
-      if (a < b + r[j].bytes && b < a + r[i].bytes) {
-        std::snprintf(buffer, sizeof buffer, "%s overlaps %s", r[i].name, r[j].name);
-        return fail(RG_ERR_INVALID_ARGUMENT, buffer);
-      }
-    }
-  return RG_OK;
-}
-
 // Whether the tensors' alignment (of one element, in `r`) allows pairs.
-bool pairs_aligned(const Range *r, int count) {
+bool pairs_aligned(const TensorRange *r, int count) {
   for (int i = 0; i < count; ++i)
     if (std::strcmp(r[i].name, "offsets") && r[i].bytes && !aligned(r[i].ptr, r[i].align * 2)) return false;
   return true;
@@ -184,13 +147,6 @@ int run_scan(int dtype, int index_dtype, bool aligned_pairs, ScanArgs &p, void *
   return launch_vec<int64_t, BACKWARD>(dtype, p, s, dev, stream, report);
 }
 
-void clear_report(rg_report *report) {
-  if (!report) return;
-  std::memset(report, 0, sizeof *report);
-  report->status_offset = -1;
-  report->streams = 1;
-}
-
 }  // namespace
 
 }  // namespace rgb
@@ -221,7 +177,7 @@ int rg_scan(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, const v
   const int esize = elem_bytes(dtype);
   const int isize = index_dtype == RG_INDEX_I32 ? 4 : 8;
   const int64_t full = n * d * esize, states = b * d * 4;
-  const Range ranges[] = {{"values", values, full, esize, false},
+  const TensorRange ranges[] = {{"values", values, full, esize, false},
                           {"gates", gates, full, esize, false},
                           {"offsets", offsets, (b + 1) * isize, isize, false},
                           {"initial", initial, initial ? states : 0, 4, false},
@@ -258,7 +214,7 @@ int rg_scan_backward(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b
   const int esize = elem_bytes(dtype);
   const int isize = index_dtype == RG_INDEX_I32 ? 4 : 8;
   const int64_t full = n * d * esize, states = b * d * 4;
-  const Range ranges[] = {{"values", values, full, esize, false},
+  const TensorRange ranges[] = {{"values", values, full, esize, false},
                           {"gates", gates, full, esize, false},
                           {"offsets", offsets, (b + 1) * isize, isize, false},
                           {"initial", initial, initial ? states : 0, 4, false},

@@ -36,7 +36,7 @@ EXPORTED = ("rg_version", "rg_error_string", "rg_last_error", "rg_get_device_inf
             "rg_shard_rows", "rg_shard_split", "rg_shard_edge_bytes", "rg_shard_workspace_bytes",
             "rg_shard_segments", "rg_shard_softmax_workspace_bytes", "rg_run_shard_softmax",
             "rg_shard_softmax_finish", "rg_run_shard", "rg_shard_combine", "rg_run_noalloc", "rg_tree_scores",
-            "rg_scan_workspace_bytes", "rg_scan", "rg_scan_backward")
+            "rg_scan_workspace_bytes", "rg_scan", "rg_scan_backward", "rg_matmul_workspace_bytes", "rg_matmul")
 
 
 class Report(ctypes.Structure):
@@ -105,6 +105,10 @@ def library(path: Path | None = None):
         lib.rg_scan_backward.argtypes = [i32, i32, i64, i64, i64, p, p, p, p, p, p, p, p, p, p, p, i64, p,
                                          ctypes.POINTER(Report)]
         lib.rg_scan_backward.restype = i32
+        lib.rg_matmul_workspace_bytes.argtypes = [i32, i32, i32, i64, i64, i64, i64, p, p, ctypes.POINTER(i64)]
+        lib.rg_matmul_workspace_bytes.restype = i32
+        lib.rg_matmul.argtypes = [i32, i32, i32, i64, i64, i64, i64, p, p, p, p, p, i64, p, ctypes.POINTER(Report)]
+        lib.rg_matmul.restype = i32
         pi64 = ctypes.POINTER(i64)
         lib.rg_shard_rows.argtypes = [i64, i32, i32, pi64, pi64]
         lib.rg_shard_rows.restype = i32
@@ -363,6 +367,24 @@ def scan_backward(dtype: str, index: str, d: int, n: int, b: int, pointers: tupl
     report = Report()
     raise_for(library().rg_scan_backward(DTYPES[dtype], INDEX[index], d, n, b, *pointers, workspace_ptr,
                                          workspace_bytes, stream, ctypes.byref(report)), "rg_scan_backward")
+    return report
+
+
+def matmul_workspace_bytes(kind: str, dtype: str, index: str, k: int, m: int, n: int, b: int, left_ptr: int,
+                           right_ptr: int) -> int:
+    """Scratch bytes of a segmented product of operands at these addresses."""
+    out = ctypes.c_int64(0)
+    raise_for(library().rg_matmul_workspace_bytes(PRODUCTS[kind], DTYPES[dtype], INDEX[index], k, m, n, b, left_ptr,
+                                                  right_ptr, ctypes.byref(out)), "rg_matmul_workspace_bytes")
+    return out.value
+
+
+def matmul(kind: str, dtype: str, index: str, k: int, m: int, n: int, b: int, left_ptr: int, right_ptr: int,
+           offsets_ptr: int, out_ptr: int, workspace_ptr: int, workspace_bytes: int, stream: int) -> Report:
+    report = Report()
+    raise_for(library().rg_matmul(PRODUCTS[kind], DTYPES[dtype], INDEX[index], k, m, n, b, left_ptr, right_ptr,
+                                  offsets_ptr, out_ptr, workspace_ptr, workspace_bytes, stream, ctypes.byref(report)),
+              "rg_matmul")
     return report
 
 

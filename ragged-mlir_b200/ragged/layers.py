@@ -45,7 +45,6 @@ class _LayerProgram:
 
     schedules = property(lambda self: (self.spec.op,))
     _check_offsets = CompiledProgram._check_offsets
-    _check_device_status = staticmethod(CompiledProgram._check_device_status)
 
     def close(self) -> None:
         """Nothing to unload: kernels live in the shared library."""
@@ -139,9 +138,19 @@ class _LayerProgram:
                     report = call(scratch.data_ptr() if nbytes else 0, nbytes, active.cuda_stream)
                     reports.append(report)
                     total = max(total, nbytes)
-                    if checked and nbytes and report.status_offset >= 0:
-                        self._check_device_status(scratch, int(report.status_offset), active, torch)
+                    if checked and report.status_offset >= 0:
+                        self._check_status_words(scratch, report, active, torch)
         return self._report(started, reports, total, validation)
+
+    @staticmethod
+    def _check_status_words(scratch, report, active, torch):
+        """Checked mode, after the launch: the words in which the last
+        launch's CTAs say that a bounded wait gave up."""
+        count = int(report.grid[report.num_launches - 1][0])
+        with torch.cuda.stream(active):
+            words = scratch.narrow(0, int(report.status_offset), 8 * count).view(torch.int64).cpu()
+        if words.any():
+            raise RuntimeError("a bounded wait inside the kernel gave up; the call's results are undefined")
 
     def _report(self, started, reports, nbytes, validation) -> ExecutionReport:
         check, check_ms = validation if validation is not None else (None, None)
@@ -240,3 +249,53 @@ class CompiledMatmul(_LayerProgram):
     """out[t] = values[t] @ weights[s] for the rows t of segment s."""
 
     kind = MatmulSpec
+
+    def _product(self, torch, kind, left, right, offsets, out, n, b):
+        """(scratch bytes, call) of one product."""
+        spec = self.spec
+        shape = (kind, spec.dtype, spec.offsets_dtype, spec.feature_dim, spec.out_dim, n, b)
+        operands = (left.data_ptr(), right.data_ptr())
+        pointers = (offsets.data_ptr(), out.data_ptr())
+        # (the scratch of a product goes by the addresses of its operands as far as their alignment)
+        nbytes = self._cached((kind, n, b, operands[0] % 16, operands[1] % 16),
+                              lambda: _native.matmul_workspace_bytes(*shape, *operands))
+        return nbytes, lambda scratch, size, on: _native.matmul(*shape, *operands, *pointers, scratch, size, on)
+
+    def run(self, values, weights, offsets, out, stream=None, mode: str = "validated") -> ExecutionReport:
+        """Writes ``out`` [N, out_dim] from ``values`` [N, feature_dim] and
+        ``weights`` [B, feature_dim, out_dim]; all of the program's dtype and
+        contiguous.  ``out`` overlaps nothing."""
+        return self._run(values, weights, offsets, out, stream, mode, True)
+
+    def _run(self, values, weights, offsets, out, stream, mode, gradless):
+        torch = _torch()
+        k, m = self.spec.feature_dim, self.spec.out_dim
+        b, n = self._segments(torch, offsets), self._rows(values, torch)
+        dtype = torch.float32 if self.spec.dtype == "f32" else torch.bfloat16
+        tensors = (("values", values, (n, k), dtype), ("weights", weights, (b, k, m), dtype), ("out", out, (n, m), dtype))
+        self._tensors(torch, tensors, offsets, mode, gradless)
+        return self._launch(torch, offsets, n, b, stream, mode, (values, weights, offsets, out),
+                            (self._product(torch, "forward", values, weights, offsets, out, n, b),))
+
+    def run_backward(self, values, weights, offsets, grad_out, stream=None, *, grad_values=None,
+                     grad_weights=None) -> ExecutionReport:
+        """Gradients of ``run`` from that of ``out``: those of ``grad_values``
+        and ``grad_weights`` that are given (zero for the weights of a segment
+        without rows)."""
+        torch = _torch()
+        k, m = self.spec.feature_dim, self.spec.out_dim
+        b, n = self._segments(torch, offsets), self._rows(values, torch)
+        dtype = torch.float32 if self.spec.dtype == "f32" else torch.bfloat16
+        tensors = [("values", values, (n, k), dtype), ("weights", weights, (b, k, m), dtype),
+                   ("grad_out", grad_out, (n, m), dtype)]
+        if grad_values is not None:
+            tensors.append(("grad_values", grad_values, (n, k), dtype))
+        if grad_weights is not None:
+            tensors.append(("grad_weights", grad_weights, (b, k, m), dtype))
+        self._tensors(torch, tensors, offsets, "validated", False)
+        work = []
+        if grad_values is not None:
+            work.append(self._product(torch, "grad_values", grad_out, weights, offsets, grad_values, n, b))
+        if grad_weights is not None:
+            work.append(self._product(torch, "grad_weights", values, grad_out, offsets, grad_weights, n, b))
+        return self._launch(torch, offsets, n, b, stream, "validated", [t[1] for t in tensors] + [offsets], work)

@@ -26,7 +26,7 @@ import threading
 from typing import Any
 
 from .errors import ValidationError
-from .layers import CARRY_ROWS, CompiledScan
+from .layers import CARRY_ROWS, CompiledMatmul, CompiledScan
 from .runtime import CompiledProgram, _torch
 
 MODES = ("validated", "checked")
@@ -43,6 +43,10 @@ SCHEMAS = {
     "segment_scan_backward": 'segment_scan_backward(Tensor values, Tensor gates, Tensor offsets, Tensor? initial, '
                              'Tensor carries, Tensor grad_out, Tensor? grad_final, str program) '
                              '-> (Tensor, Tensor, Tensor)',
+    "segment_matmul": 'segment_matmul(Tensor values, Tensor weights, Tensor offsets, str program, '
+                      'str mode="validated") -> Tensor',
+    "segment_matmul_backward": 'segment_matmul_backward(Tensor values, Tensor weights, Tensor offsets, '
+                               'Tensor grad_out, str program, bool[2] wanted) -> (Tensor, Tensor)',
 }
 
 
@@ -136,6 +140,12 @@ class OpContract:
         if initial is not None and (tuple(initial.shape) != (offsets.shape[0] - 1, values.shape[1])
                                     or initial.dtype != self.torch.float32 or initial.device != values.device):
             raise ValidationError("initial must be f32 [B, D] on the values device")
+
+    def matmul(self, values, weights, offsets) -> None:
+        self.inputs_of("matmul", values, offsets)
+        if (weights.ndim != 3 or weights.shape[0] != offsets.shape[0] - 1 or weights.shape[1] != values.shape[1]
+                or weights.dtype != values.dtype or weights.device != values.device):
+            raise ValidationError("weights must be [B, D, out] with the dtype and device of values")
 
     def inputs_of(self, op: str, values, offsets) -> None:
         """What the learned operators ask of values and offsets."""
@@ -267,6 +277,53 @@ def _register_scan(torch, library, contract) -> None:
     torch.library.register_autograd("ragged_mlir::segment_scan", backward, setup_context=setup, lib=library)
 
 
+def _register_matmul(torch, library, contract) -> None:
+    def matmul_kernel(values, weights, offsets, program, mode="validated"):
+        compiled = _table.lookup(program, "matmul")
+        values, weights = _dense(values, weights)
+        out = values.new_empty((values.shape[0], compiled.spec.out_dim))
+        compiled._run(values, weights, offsets, out, None, mode, False)
+        return out
+
+    def matmul_backward_kernel(values, weights, offsets, grad_out, program, wanted):
+        compiled = _table.lookup(program, "matmul")
+        values, weights, grad_out = _dense(values, weights, grad_out)
+        grads = tuple(torch.empty_like(t) if want else t.new_empty((0,)) for t, want in zip((values, weights), wanted))
+        compiled.run_backward(values, weights, offsets, grad_out, grad_values=grads[0] if wanted[0] else None,
+                              grad_weights=grads[1] if wanted[1] else None)
+        return grads
+
+    for key in ("CPU", "CUDA"):
+        library.impl("segment_matmul", matmul_kernel, key)
+        library.impl("segment_matmul_backward", matmul_backward_kernel, key)
+
+    @torch.library.register_fake("ragged_mlir::segment_matmul", lib=library)
+    def matmul_fake(values, weights, offsets, program, mode="validated"):
+        contract.mode(mode)
+        contract.matmul(values, weights, offsets)
+        return values.new_empty((values.shape[0], weights.shape[2]))
+
+    @torch.library.register_fake("ragged_mlir::segment_matmul_backward", lib=library)
+    def matmul_backward_fake(values, weights, offsets, grad_out, program, wanted):
+        return tuple(t.new_empty(t.shape if want else (0,)) for t, want in zip((values, weights), wanted))
+
+    def setup(ctx, inputs, output):
+        values, weights, offsets, ctx.program, _ = inputs
+        ctx.save_for_backward(values, weights, offsets)
+        ctx.set_materialize_grads(False)
+
+    def backward(ctx, grad_out):
+        _first_derivative(torch)
+        wanted = list(ctx.needs_input_grad[:2])
+        if grad_out is None or not any(wanted):
+            return (None,) * 5
+        values, weights, offsets = ctx.saved_tensors
+        grads = torch.ops.ragged_mlir.segment_matmul_backward(values, weights, offsets, grad_out, ctx.program, wanted)
+        return grads[0] if wanted[0] else None, grads[1] if wanted[1] else None, None, None, None
+
+    torch.library.register_autograd("ragged_mlir::segment_matmul", backward, setup_context=setup, lib=library)
+
+
 def register_torch_ops() -> dict[str, Any]:
     """Define the ``ragged_mlir`` operators (once); returns name -> operator of
     segment_reduce and segment_softmax, as the reference's function does
@@ -307,6 +364,7 @@ def register_torch_ops() -> dict[str, Any]:
             return values.new_empty(output_shape("softmax", values, offsets))
 
         _register_scan(torch, library, contract)
+        _register_matmul(torch, library, contract)
         _library = library
         namespace = torch.ops.ragged_mlir
         _operators.update(segment_reduce=namespace.segment_reduce, segment_softmax=namespace.segment_softmax)
@@ -339,6 +397,14 @@ def segment_scan(values, gates, offsets, *, program: CompiledScan, initial=None,
     out, final, _ = torch.ops.ragged_mlir.segment_scan(values, gates, offsets, initial, register_program(program),
                                                        mode, record)
     return out, final
+
+
+def segment_matmul(values, weights, offsets, *, program: CompiledMatmul, mode: str = "validated"):
+    """[N, out] of values[t] @ weights[s] for the rows t of segment s,
+    differentiable (once) in values and weights.  (On captured backward
+    passes: see ``segment_scan``.)"""
+    register_torch_ops()
+    return _torch().ops.ragged_mlir.segment_matmul(values, weights, offsets, register_program(program), mode)
 
 
 def bind(program: CompiledProgram, *, mode: str = "validated"):
@@ -394,6 +460,14 @@ def njt_scan(nt, gates, *, program: CompiledScan, initial=None, mode: str = "val
         raise ValidationError("gates must share the offsets of the values")
     out, final = segment_scan(values, gate_values, offsets, program=program, initial=initial, mode=mode)
     return _torch().nested.nested_tensor_from_jagged(out, offsets=offsets), final
+
+
+def njt_matmul(nt, weights, *, program: CompiledMatmul, mode: str = "validated"):
+    """``segment_matmul`` over the ragged dimension of an NJT, returned as an
+    NJT on the same offsets."""
+    values, offsets = jagged_components(nt)
+    out = segment_matmul(values, weights, offsets, program=program, mode=mode)
+    return _torch().nested.nested_tensor_from_jagged(out, offsets=offsets)
 
 
 def njt_softmax(nt, *, program: CompiledProgram, mode: str = "validated", mask=None):
