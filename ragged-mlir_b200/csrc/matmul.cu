@@ -76,9 +76,9 @@ int64_t most_row_tiles(int kind, const MatmulArgs &p, int tile) {
   return kind == MATMUL_GRAD_WEIGHTS ? p.b * ceil_div(p.k, tile) : p.n / tile + std::min(p.n, p.b);
 }
 
-template <typename OffT, int KIND, int TILE>
+template <typename OffT, int KIND, int TILE, int SIZE>
 int launch_simt_tile(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
-  const auto kernel = matmul_simt_kernel<OffT, KIND, TILE>;
+  const auto kernel = matmul_simt_kernel<OffT, KIND, TILE, SIZE>;
   int per_sm = 0;
   const int status = prepare_kernel(reinterpret_cast<const void *>(kernel), dev.device, kSimtThreads, 0, 0, &per_sm);
   if (status) return status;
@@ -91,13 +91,19 @@ int launch_simt_tile(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream, 
   return check_cuda(cudaGetLastError(), "matmul_simt_kernel launch");
 }
 
-// 128 x 128 tiles where they give every SM one, 64 x 64 where they do not.
+// 128 x 128 tiles where they give every SM one, 64 x 64 where they do not;
+// 16-byte pieces where all rows start at 16-byte boundaries.
 template <typename OffT, int KIND>
 int launch_simt(const MatmulArgs &p, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
   const int64_t tiles =
       (KIND == MATMUL_GRAD_WEIGHTS ? p.b * ceil_div(p.k, 128) : ceil_div(p.n, 128)) * ceil_div(p.cols, 128);
-  if (tiles >= dev.sm_count) return launch_simt_tile<OffT, KIND, 128>(p, dev, stream, report);
-  return launch_simt_tile<OffT, KIND, 64>(p, dev, stream, report);
+  const bool large = tiles >= dev.sm_count;
+  if (p.k % 4 == 0 && p.m % 4 == 0 && aligned(p.left, 16) && aligned(p.right, 16) && aligned(p.out, 16)) {
+    if (large) return launch_simt_tile<OffT, KIND, 128, 4>(p, dev, stream, report);
+    return launch_simt_tile<OffT, KIND, 64, 4>(p, dev, stream, report);
+  }
+  if (large) return launch_simt_tile<OffT, KIND, 128, 1>(p, dev, stream, report);
+  return launch_simt_tile<OffT, KIND, 64, 1>(p, dev, stream, report);
 }
 
 template <typename OffT, int KIND, int COLS>

@@ -4,8 +4,9 @@
 // (tf32) or fewer bits of mantissa.  A CTA of 256 threads computes a TILE x
 // TILE block of the output, 8 x 8 (4 x 4) values a thread held in registers, from
 // slices of 16 of the contraction in shared memory, the next slice on its way
-// in registers.  Bound: 128 FMAs a clock and SM; a thread loads 16 values from
-// shared memory for 64 FMAs, so the pipes and not the loads set the pace.
+// in registers; two CTAs an SM fill each other's waits.  Bound: 128 FMAs a
+// clock and SM; a thread loads 16 values from shared memory for 64 FMAs, so the
+// pipes and not the loads set the pace.
 #pragma once
 
 #include "matmul.cuh"
@@ -15,71 +16,93 @@ namespace rgb {
 constexpr int kSimtThreads = 256;
 constexpr int kSimtDepth = 16;
 
-// LEFT_T / RIGHT_T: how the operand lies in memory.  Left: rows x depth, or
-// (transposed) depth x rows; right: depth x cols, or (transposed) cols x depth.
-template <typename OffT, int KIND, int TILE>
-__global__ void __launch_bounds__(kSimtThreads) matmul_simt_kernel(const MatmulArgs p) {
-  constexpr bool LEFT_T = KIND == MATMUL_GRAD_WEIGHTS, RIGHT_T = KIND == MATMUL_GRAD_VALUES;
+// A thread's share of a slice of one operand: pieces of SIZE elements.  ALONG:
+// the tile's rows (columns) are contiguous in memory; else the contraction is.
+template <int TILE, int SIZE, bool ALONG>
+struct SimtOperand {
+  static constexpr int kPieces = TILE * kSimtDepth / (kSimtThreads * SIZE);
+  static constexpr int kAcross = (ALONG ? TILE : kSimtDepth) / SIZE;  // pieces of a line
+  static constexpr int kLines = kSimtThreads / kAcross;               // lines between a thread's pieces
+  using Piece = typename std::conditional<SIZE == 4, float4, float>::type;
+  const float *at;
+  int64_t pitch;
+  int line, place;   // of the first piece
+  int64_t limit;     // lines (elements of a line) of the tile that exist
+  Piece piece[kPieces];
+
+  __device__ __forceinline__ void begin(const float *base, int64_t row_pitch, int64_t first, int64_t end) {
+    line = threadIdx.x / kAcross;
+    place = threadIdx.x % kAcross * SIZE;
+    pitch = row_pitch;
+    limit = end - first;
+    at = ALONG ? base + line * pitch + first + place : base + (first + line) * pitch + place;
+  }
+  // The slice with `left` of the contraction to go; moves on to the next.
+  __device__ __forceinline__ void load(int64_t left) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int l = line + i * kLines;
+      const bool ok = ALONG ? l < left && place < limit : l < limit && place < left;
+      piece[i] = ok ? __ldg(reinterpret_cast<const Piece *>(at + i * kLines * pitch)) : Piece{};
+    }
+    at += ALONG ? kSimtDepth * pitch : int64_t{kSimtDepth};
+  }
+  template <int PITCH>
+  __device__ __forceinline__ void stage(float (*to)[PITCH]) const {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int l = line + i * kLines;
+      if constexpr (ALONG) {
+        *reinterpret_cast<Piece *>(&to[l][place]) = piece[i];
+      } else {
+        const float *x = reinterpret_cast<const float *>(&piece[i]);
+#pragma unroll
+        for (int e = 0; e < SIZE; ++e) to[place + e][l] = x[e];
+      }
+    }
+  }
+};
+
+template <typename OffT, int KIND, int TILE, int SIZE>
+__global__ void __launch_bounds__(kSimtThreads, TILE == 128 ? 2 : 3) matmul_simt_kernel(const MatmulArgs p) {
   constexpr int DEPTH = kSimtDepth;
-  constexpr int PER = TILE / 16;                      // outputs of a thread in each direction
-  constexpr int LOADS = TILE * DEPTH / kSimtThreads;  // elements of an operand's slice a thread loads
+  constexpr int PER = TILE / 16;  // outputs of a thread in each direction
   constexpr int PITCH = TILE + 4;
   __shared__ __align__(16) float left_s[2][DEPTH][PITCH], right_s[2][DEPTH][PITCH];
-  const float *__restrict__ left = static_cast<const float *>(p.left);
-  const float *__restrict__ right = static_cast<const float *>(p.right);
   float *__restrict__ out = static_cast<float *>(p.out);
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   MatmulWalk<OffT, KIND, TILE> walk(p.offsets, p.b);
   MatmulTile t;
+  SimtOperand<TILE, SIZE, KIND == MATMUL_GRAD_WEIGHTS> left;
+  SimtOperand<TILE, SIZE, KIND != MATMUL_GRAD_VALUES> right;
   for (int64_t index = blockIdx.x; walk.find(p, index, t); index += gridDim.x) {
     const int64_t col0 = static_cast<int64_t>(t.col_tile) * TILE;
     const int64_t depth = KIND == MATMUL_GRAD_WEIGHTS ? t.end - t.begin : p.depth;
-    const float *lbase = left + (LEFT_T ? t.begin * p.left_pitch : int64_t{0});
-    const float *rbase = right + (KIND == MATMUL_GRAD_WEIGHTS ? t.begin * p.right_pitch : t.seg * p.k * p.m);
-    const int64_t row_limit = t.row_end, col_limit = p.cols;
-    float lreg[LOADS], rreg[LOADS];
-    auto load = [&](int64_t d0) {
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int e = i * kSimtThreads + threadIdx.x;
-        {
-          const int d = LEFT_T ? e / TILE : e % DEPTH, r = LEFT_T ? e % TILE : e / DEPTH;
-          const int64_t row = t.row + r, at = LEFT_T ? (d0 + d) * p.left_pitch + row : row * p.left_pitch + d0 + d;
-          lreg[i] = row < row_limit && d0 + d < depth ? __ldg(lbase + at) : 0.0f;
-        }
-        {
-          const int d = RIGHT_T ? e % DEPTH : e / TILE, c = RIGHT_T ? e / DEPTH : e % TILE;
-          const int64_t col = col0 + c, at = RIGHT_T ? col * p.right_pitch + d0 + d : (d0 + d) * p.right_pitch + col;
-          rreg[i] = col < col_limit && d0 + d < depth ? __ldg(rbase + at) : 0.0f;
-        }
-      }
-    };
-    auto stage = [&](int buffer) {
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int e = i * kSimtThreads + threadIdx.x;
-        if (LEFT_T)
-          left_s[buffer][e / TILE][e % TILE] = lreg[i];
-        else
-          left_s[buffer][e % DEPTH][e / DEPTH] = lreg[i];
-        if (RIGHT_T)
-          right_s[buffer][e % DEPTH][e / DEPTH] = rreg[i];
-        else
-          right_s[buffer][e / TILE][e % TILE] = rreg[i];
-      }
-    };
+    left.begin(static_cast<const float *>(p.left) + (KIND == MATMUL_GRAD_WEIGHTS ? t.begin * p.left_pitch : int64_t{0}),
+               p.left_pitch, t.row, t.row_end);
+    right.begin(static_cast<const float *>(p.right) +
+                    (KIND == MATMUL_GRAD_WEIGHTS ? t.begin * p.right_pitch : t.seg * p.k * p.m),
+                p.right_pitch, col0, p.cols);
     // Columns in pairs, for the packed FMA.
     unsigned long long acc[PER][PER / 2];
 #pragma unroll
     for (int i = 0; i < PER; ++i)
 #pragma unroll
       for (int j = 0; j < PER / 2; ++j) acc[i][j] = 0;
-    if (depth > 0) load(0);
+    if (depth > 0) {
+      left.load(depth);
+      right.load(depth);
+    }
     int buffer = 0;
-    for (int64_t d0 = 0; d0 < depth; d0 += DEPTH, buffer ^= 1) {
-      stage(buffer);
+#pragma unroll 1
+    for (int64_t to_go = depth; to_go > 0; to_go -= DEPTH, buffer ^= 1) {
+      left.stage(left_s[buffer]);
+      right.stage(right_s[buffer]);
       __syncthreads();  // the slice is there; the other buffer's readers are done
-      if (d0 + DEPTH < depth) load(d0 + DEPTH);
+      if (to_go > DEPTH) {
+        left.load(to_go - DEPTH);
+        right.load(to_go - DEPTH);
+      }
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) {
         float l[PER];
@@ -107,14 +130,21 @@ __global__ void __launch_bounds__(kSimtThreads) matmul_simt_kernel(const MatmulA
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int64_t row = t.row + (i / 4) * 64 + ty * 4 + i % 4;
-      if (row >= row_limit) continue;
+      if (row >= t.row_end) continue;
 #pragma unroll
-      for (int j = 0; j < PER / 2; ++j) {
-        const int64_t col = col0 + (j / 2) * 64 + tx * 4 + (j % 2) * 2;
-        float lo, hi;
-        unpack2(acc[i][j], lo, hi);
-        if (col < col_limit) to[row * p.out_pitch + col] = lo;
-        if (col + 1 < col_limit) to[row * p.out_pitch + col + 1] = hi;
+      for (int g = 0; g < PER / 4; ++g) {
+        const int64_t col = col0 + g * 64 + tx * 4;
+        float *at = to + row * p.out_pitch + col;
+        float x[4];
+        unpack2(acc[i][g * 2], x[0], x[1]);
+        unpack2(acc[i][g * 2 + 1], x[2], x[3]);
+        if constexpr (SIZE == 4) {
+          if (col < p.cols) *reinterpret_cast<float4 *>(at) = make_float4(x[0], x[1], x[2], x[3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (col + e < p.cols) at[e] = x[e];
+        }
       }
     }
     __syncthreads();  // the last slice has been read

@@ -61,6 +61,8 @@ _lib = None
 def library(path: Path | None = None):
     """The loaded library (raises RuntimeUnavailable when it is missing)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -352,22 +354,22 @@ def scan_workspace_bytes(dtype: str, index: str, d: int, n: int, b: int) -> int:
 
 
 def scan(dtype: str, index: str, d: int, n: int, b: int, pointers: tuple, workspace_ptr: int, workspace_bytes: int,
-         stream: int) -> Report:
+         stream: int, report: Report | None) -> None:
     """``pointers``: values, gates, offsets, initial, out, final, carries (0: none)."""
-    report = Report()
-    raise_for(library().rg_scan(DTYPES[dtype], INDEX[index], d, n, b, *pointers, workspace_ptr, workspace_bytes,
-                                stream, ctypes.byref(report)), "rg_scan")
-    return report
+    status = library().rg_scan(DTYPES[dtype], INDEX[index], d, n, b, *pointers, workspace_ptr, workspace_bytes, stream,
+                               report)
+    if status:
+        raise_for(status, "rg_scan")
 
 
 def scan_backward(dtype: str, index: str, d: int, n: int, b: int, pointers: tuple, workspace_ptr: int,
-                  workspace_bytes: int, stream: int) -> Report:
+                  workspace_bytes: int, stream: int, report: Report | None) -> None:
     """``pointers``: values, gates, offsets, initial, carries, grad_out,
     grad_final, grad_values, grad_gates, grad_initial (0: none)."""
-    report = Report()
-    raise_for(library().rg_scan_backward(DTYPES[dtype], INDEX[index], d, n, b, *pointers, workspace_ptr,
-                                         workspace_bytes, stream, ctypes.byref(report)), "rg_scan_backward")
-    return report
+    status = library().rg_scan_backward(DTYPES[dtype], INDEX[index], d, n, b, *pointers, workspace_ptr,
+                                        workspace_bytes, stream, report)
+    if status:
+        raise_for(status, "rg_scan_backward")
 
 
 def matmul_workspace_bytes(kind: str, dtype: str, index: str, k: int, m: int, n: int, b: int, left_ptr: int,
@@ -380,12 +382,12 @@ def matmul_workspace_bytes(kind: str, dtype: str, index: str, k: int, m: int, n:
 
 
 def matmul(kind: str, dtype: str, index: str, k: int, m: int, n: int, b: int, left_ptr: int, right_ptr: int,
-           offsets_ptr: int, out_ptr: int, workspace_ptr: int, workspace_bytes: int, stream: int) -> Report:
-    report = Report()
-    raise_for(library().rg_matmul(PRODUCTS[kind], DTYPES[dtype], INDEX[index], k, m, n, b, left_ptr, right_ptr,
-                                  offsets_ptr, out_ptr, workspace_ptr, workspace_bytes, stream, ctypes.byref(report)),
-              "rg_matmul")
-    return report
+           offsets_ptr: int, out_ptr: int, workspace_ptr: int, workspace_bytes: int, stream: int,
+           report: Report | None) -> None:
+    status = library().rg_matmul(PRODUCTS[kind], DTYPES[dtype], INDEX[index], k, m, n, b, left_ptr, right_ptr,
+                                 offsets_ptr, out_ptr, workspace_ptr, workspace_bytes, stream, report)
+    if status:
+        raise_for(status, "rg_matmul")
 
 
 def tree_scores(arrays: dict, x, classes: int, max_depth: int):

@@ -41,7 +41,8 @@ class _LayerProgram:
         self.spec, self.artifact, self.cache_hit = spec, artifact, cache_hit
         self._digest = artifact.key.digest
         self._dtypes = None
-        self._sizes: dict[tuple, object] = {}
+        self._sizes: dict[tuple, int] = {}
+        self._launches: dict[tuple, _Launch] = {}
 
     schedules = property(lambda self: (self.spec.op,))
     _check_offsets = CompiledProgram._check_offsets
@@ -77,10 +78,10 @@ class _LayerProgram:
         for name, tensor, shape, dtype in tensors:
             if not isinstance(tensor, torch.Tensor):
                 raise ValidationError(f"{name} must be a torch.Tensor")
-            if not tensor.is_cuda:
-                raise RuntimeUnavailable(f"{name} must be on a CUDA device that runs {self.spec.chip} code; "
-                                         "no CPU execution fallback exists")
             if tensor.device != device:
+                if not tensor.is_cuda:
+                    raise RuntimeUnavailable(f"{name} must be on a CUDA device that runs {self.spec.chip} code; "
+                                             "no CPU execution fallback exists")
                 raise ValidationError(f"{name} must use the CUDA device of offsets")
             if tensor.dtype != dtype:
                 raise ValidationError(f"{name} must have dtype {dtype}: tensor dtype differs from compiled "
@@ -104,8 +105,9 @@ class _LayerProgram:
         return values.shape[0]
 
     def _launch(self, torch, offsets, n, b, stream, mode, used, work) -> ExecutionReport:
-        """For each (bytes, call) of ``work``: ``call(scratch address, bytes,
-        stream)`` on the execution stream."""
+        """For each (key, scratch bytes, call) of ``work``: ``call(scratch
+        address, bytes, stream, report)`` on the execution stream.  What a call
+        launches goes by its key, and is asked for once for each."""
         started = time.perf_counter()
         checked = mode == "checked"
         if b == 0 and n != 0 and not checked:  # checked mode reports it from the device
@@ -113,61 +115,91 @@ class _LayerProgram:
         if self.spec.offsets_dtype == "i32" and n > 2**31 - 1:
             raise ValidationError("N exceeds the i32 offsets range")
         device = offsets.device
-        reports, validation, total = [], None, 0
-        with torch.cuda.device(device):
-            if device.index not in _checked_devices:
-                capability = tuple(torch.cuda.get_device_capability(device))
-                if not runs_on(self.spec.chip, capability):
-                    raise RuntimeUnavailable(f"compiled target {self.spec.chip} does not run on the current device "
-                                             f"(sm_{capability[0]}{capability[1]})")
-                _checked_devices.add(device.index)
-            active = stream if stream is not None else torch.cuda.current_stream(device)
-            if not isinstance(active, torch.cuda.Stream) or active.device != device:
-                raise ValidationError("stream must be a torch.cuda.Stream on the values device")
-            if checked:
-                validation = self._check_offsets(offsets, offsets, n, b, active, torch)
-            if b:
-                if stream is not None:
-                    for tensor in used:
-                        tensor.record_stream(active)
-                for nbytes, call in work:
-                    scratch = None
-                    if nbytes:
-                        with torch.cuda.stream(active) if stream is not None else nullcontext():
-                            scratch = torch.empty((nbytes,), dtype=torch.uint8, device=device)
-                    report = call(scratch.data_ptr() if nbytes else 0, nbytes, active.cuda_stream)
-                    reports.append(report)
+        if torch.cuda.current_device() != device.index:
+            with torch.cuda.device(device):
+                return self._launch(torch, offsets, n, b, stream, mode, used, work)
+        if device.index not in _checked_devices:
+            capability = tuple(torch.cuda.get_device_capability(device))
+            if not runs_on(self.spec.chip, capability):
+                raise RuntimeUnavailable(f"compiled target {self.spec.chip} does not run on the current device "
+                                         f"(sm_{capability[0]}{capability[1]})")
+            _checked_devices.add(device.index)
+        active = stream if stream is not None else torch.cuda.current_stream()
+        if not isinstance(active, torch.cuda.Stream) or active.device != device:
+            raise ValidationError("stream must be a torch.cuda.Stream on the values device")
+        validation = self._check_offsets(offsets, offsets, n, b, active, torch) if checked else None
+        launches, total = (), 0
+        if b:
+            on = active.cuda_stream
+            if stream is not None:
+                for tensor in used:
+                    tensor.record_stream(active)
+            for key, nbytes, call in work:
+                address = 0
+                if nbytes:
+                    # Scratch comes from the caching allocator on the execution
+                    # stream, so reuse is ordered after this call's kernels.
+                    with torch.cuda.stream(active) if stream is not None else nullcontext():
+                        scratch = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+                    address = scratch.data_ptr()
                     total = max(total, nbytes)
-                    if checked and report.status_offset >= 0:
-                        self._check_status_words(scratch, report, active, torch)
-        return self._report(started, reports, total, validation)
+                launch = self._launches.get(key)
+                if launch is None:
+                    report = _native.Report()
+                    call(address, nbytes, on, report)
+                    if len(self._launches) >= 256:
+                        self._launches.clear()
+                    launch = self._launches[key] = _Launch(report)
+                else:
+                    call(address, nbytes, on, None)
+                launches += (launch,)
+                if checked and launch.status_offset >= 0:
+                    self._check_status_words(scratch, launch, active, torch)
+        return self._report(started, launches, total, validation)
 
     @staticmethod
-    def _check_status_words(scratch, report, active, torch):
+    def _check_status_words(scratch, launch, active, torch):
         """Checked mode, after the launch: the words in which the last
         launch's CTAs say that a bounded wait gave up."""
-        count = int(report.grid[report.num_launches - 1][0])
         with torch.cuda.stream(active):
-            words = scratch.narrow(0, int(report.status_offset), 8 * count).view(torch.int64).cpu()
+            words = scratch.narrow(0, launch.status_offset, 8 * launch.grids[-1][0]).view(torch.int64).cpu()
         if words.any():
             raise RuntimeError("a bounded wait inside the kernel gave up; the call's results are undefined")
 
-    def _report(self, started, reports, nbytes, validation) -> ExecutionReport:
+    def _report(self, started, launches, nbytes, validation) -> ExecutionReport:
         check, check_ms = validation if validation is not None else (None, None)
-        parts = ([check] if check is not None else []) + reports
-        names = tuple(_native.kernel_name(r.kernel_ids[i]) for r in parts for i in range(r.num_launches))
-        grids = tuple(tuple(r.grid[i]) for r in parts for i in range(r.num_launches))
+        parts = (_Launch(check),) + launches if check is not None else launches
         checked_bytes = STATUS_BYTES if check is not None else 0
-        return ExecutionReport(("rows",) if reports else (), (), grids, nbytes + checked_bytes, self._digest, None,
-                               "checked" if check is not None else "validated", names,
+        last = launches[-1] if launches else None
+        return ExecutionReport(("rows",) if launches else (), (), sum((x.grids for x in parts), ()),
+                               nbytes + checked_bytes, self._digest, None,
+                               "checked" if check is not None else "validated", sum((x.names for x in parts), ()),
                                (time.perf_counter() - started) * 1000, cache_hit=self.cache_hit,
                                validation_workspace_bytes=checked_bytes, validation_host_ms=check_ms,
-                               d_tile=int(reports[-1].d_tile) if reports else None,
-                               d_vector=int(reports[-1].d_vector) if reports else 1, selected=self.spec.op)
+                               d_tile=last.d_tile if last else None, d_vector=last.d_vector if last else 1,
+                               selected=self.spec.op)
+
+
+class _Launch:
+    """What a call launched, from the library's report."""
+
+    __slots__ = ("names", "grids", "d_tile", "d_vector", "status_offset")
+
+    def __init__(self, report):
+        count = report.num_launches
+        self.names = tuple(_native.kernel_name(report.kernel_ids[i]) for i in range(count))
+        self.grids = tuple(tuple(report.grid[i]) for i in range(count))
+        self.d_tile, self.d_vector = int(report.d_tile), int(report.d_vector)
+        self.status_offset = int(report.status_offset)
 
 
 def _address(tensor) -> int:
     return 0 if tensor is None else tensor.data_ptr()
+
+
+def _alignment(pointers) -> tuple:
+    """What of the addresses decides how a call runs."""
+    return tuple(p % 16 for p in pointers)
 
 
 class CompiledScan(_LayerProgram):
@@ -209,11 +241,11 @@ class CompiledScan(_LayerProgram):
         pointers = (values.data_ptr(), gates.data_ptr(), offsets.data_ptr(), _address(initial), out.data_ptr(),
                     _address(final), _address(carries))
 
-        def call(scratch, nbytes, on):
-            return _native.scan(spec.dtype, spec.offsets_dtype, d, n, b, pointers, scratch, nbytes, on)
+        def call(scratch, nbytes, on, report):
+            _native.scan(spec.dtype, spec.offsets_dtype, d, n, b, pointers, scratch, nbytes, on, report)
 
         return self._launch(torch, offsets, n, b, stream, mode, [t[1] for t in tensors] + [offsets],
-                            [(self._scratch(n, b), call)])
+                            (((False, n, b) + _alignment(pointers), self._scratch(n, b), call),))
 
     def run_backward(self, values, gates, offsets, carries, grad_out, stream=None, *, initial=None, grad_final=None,
                      grad_values=None, grad_gates=None, grad_initial=None) -> ExecutionReport:
@@ -238,11 +270,11 @@ class CompiledScan(_LayerProgram):
                     grad_out.data_ptr(), _address(grad_final), _address(grad_values), _address(grad_gates),
                     _address(grad_initial))
 
-        def call(scratch, nbytes, on):
-            return _native.scan_backward(spec.dtype, spec.offsets_dtype, d, n, b, pointers, scratch, nbytes, on)
+        def call(scratch, nbytes, on, report):
+            _native.scan_backward(spec.dtype, spec.offsets_dtype, d, n, b, pointers, scratch, nbytes, on, report)
 
         return self._launch(torch, offsets, n, b, stream, "validated", [t[1] for t in tensors] + [offsets],
-                            [(self._scratch(n, b), call)])
+                            (((True, n, b) + _alignment(pointers), self._scratch(n, b), call),))
 
 
 class CompiledMatmul(_LayerProgram):
@@ -250,16 +282,15 @@ class CompiledMatmul(_LayerProgram):
 
     kind = MatmulSpec
 
-    def _product(self, torch, kind, left, right, offsets, out, n, b):
-        """(scratch bytes, call) of one product."""
+    def _product(self, kind, left, right, offsets, out, n, b):
+        """(key, scratch bytes, call) of one product."""
         spec = self.spec
         shape = (kind, spec.dtype, spec.offsets_dtype, spec.feature_dim, spec.out_dim, n, b)
-        operands = (left.data_ptr(), right.data_ptr())
-        pointers = (offsets.data_ptr(), out.data_ptr())
-        # (the scratch of a product goes by the addresses of its operands as far as their alignment)
-        nbytes = self._cached((kind, n, b, operands[0] % 16, operands[1] % 16),
-                              lambda: _native.matmul_workspace_bytes(*shape, *operands))
-        return nbytes, lambda scratch, size, on: _native.matmul(*shape, *operands, *pointers, scratch, size, on)
+        left, right = left.data_ptr(), right.data_ptr()
+        pointers = (left, right, offsets.data_ptr(), out.data_ptr())
+        key = (kind, n, b) + _alignment(pointers)
+        nbytes = self._cached(key, lambda: _native.matmul_workspace_bytes(*shape, left, right))
+        return key, nbytes, lambda scratch, size, on, report: _native.matmul(*shape, *pointers, scratch, size, on, report)
 
     def run(self, values, weights, offsets, out, stream=None, mode: str = "validated") -> ExecutionReport:
         """Writes ``out`` [N, out_dim] from ``values`` [N, feature_dim] and
@@ -275,7 +306,7 @@ class CompiledMatmul(_LayerProgram):
         tensors = (("values", values, (n, k), dtype), ("weights", weights, (b, k, m), dtype), ("out", out, (n, m), dtype))
         self._tensors(torch, tensors, offsets, mode, gradless)
         return self._launch(torch, offsets, n, b, stream, mode, (values, weights, offsets, out),
-                            (self._product(torch, "forward", values, weights, offsets, out, n, b),))
+                            (self._product("forward", values, weights, offsets, out, n, b),))
 
     def run_backward(self, values, weights, offsets, grad_out, stream=None, *, grad_values=None,
                      grad_weights=None) -> ExecutionReport:
@@ -295,7 +326,7 @@ class CompiledMatmul(_LayerProgram):
         self._tensors(torch, tensors, offsets, "validated", False)
         work = []
         if grad_values is not None:
-            work.append(self._product(torch, "grad_values", grad_out, weights, offsets, grad_values, n, b))
+            work.append(self._product("grad_values", grad_out, weights, offsets, grad_values, n, b))
         if grad_weights is not None:
-            work.append(self._product(torch, "grad_weights", values, grad_out, offsets, grad_weights, n, b))
+            work.append(self._product("grad_weights", values, grad_out, offsets, grad_weights, n, b))
         return self._launch(torch, offsets, n, b, stream, "validated", [t[1] for t in tensors] + [offsets], work)

@@ -197,10 +197,9 @@ def _scan_shapes(values, offsets, record: bool) -> tuple:
     return (n, d), (offsets.shape[0] - 1, d), ((n + CARRY_ROWS - 1) // CARRY_ROWS if record else 0, d)
 
 
-def _scan_call(values, gates, offsets, initial, token: str, mode: str, record: bool):
-    """The real kernel of segment_scan."""
+def _scan_call(values, gates, offsets, initial, program, mode: str, record: bool):
+    """(out, final, carries) of segment_scan, on the GPU."""
     torch = _torch()
-    program = _table.lookup(token, "scan")
     values, gates, initial = _dense(values, gates, initial)
     shapes = _scan_shapes(values, offsets, record)
     out = torch.empty_like(values)
@@ -209,10 +208,9 @@ def _scan_call(values, gates, offsets, initial, token: str, mode: str, record: b
     return out, final, carries
 
 
-def _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final, token: str):
-    """The real kernel of segment_scan_backward."""
+def _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final, program):
+    """The gradients of values, gates and initial, on the GPU."""
     torch = _torch()
-    program = _table.lookup(token, "scan")
     values, gates, initial, grad_out, grad_final = _dense(values, gates, initial, grad_out, grad_final)
     grad_values, grad_gates = torch.empty_like(values), torch.empty_like(values)
     grad_initial = torch.empty_like(initial) if initial is not None else carries.new_empty((0,))
@@ -229,10 +227,11 @@ def _first_derivative(torch) -> None:
 
 def _register_scan(torch, library, contract) -> None:
     def scan_kernel(values, gates, offsets, initial, program, mode="validated", record=True):
-        return _scan_call(values, gates, offsets, initial, program, mode, record)
+        return _scan_call(values, gates, offsets, initial, _table.lookup(program, "scan"), mode, record)
 
     def scan_backward_kernel(values, gates, offsets, initial, carries, grad_out, grad_final, program):
-        return _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final, program)
+        return _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final,
+                                   _table.lookup(program, "scan"))
 
     for key in ("CPU", "CUDA"):
         library.impl("segment_scan", scan_kernel, key)
@@ -277,21 +276,89 @@ def _register_scan(torch, library, contract) -> None:
     torch.library.register_autograd("ragged_mlir::segment_scan", backward, setup_context=setup, lib=library)
 
 
+def _matmul_call(values, weights, offsets, program, mode: str):
+    """The output of segment_matmul, on the GPU."""
+    values, weights = _dense(values, weights)
+    out = values.new_empty((values.shape[0], program.spec.out_dim))
+    program._run(values, weights, offsets, out, None, mode, False)
+    return out
+
+
+def _matmul_backward_call(values, weights, offsets, grad_out, program, wanted):
+    """The gradients of values and weights (None: not wanted), on the GPU."""
+    torch = _torch()
+    values, weights, grad_out = _dense(values, weights, grad_out)
+    grads = [torch.empty_like(t) if want else None for t, want in zip((values, weights), wanted)]
+    program.run_backward(values, weights, offsets, grad_out, grad_values=grads[0], grad_weights=grads[1])
+    return grads
+
+
+def _plain(torch, *tensors) -> bool:
+    """Whether a call can go to the GPU as it is: CUDA tensors, and nothing
+    that traces, fakes or wraps calls.  It then skips the operator's dispatch,
+    which costs several times what its launches do; everything else (tracing,
+    meta and wrapped tensors) takes the operator."""
+    return (all(t is None or (type(t) in (torch.Tensor, torch.nn.Parameter) and t.is_cuda) for t in tensors)
+            and not torch.compiler.is_compiling() and not torch._C._len_torch_dispatch_stack()
+            and not torch._C._functorch.peek_interpreter_stack())
+
+
+_functions: dict[str, Any] = {}
+
+
+def _autograd_functions(torch) -> dict[str, Any]:
+    """The operators' differentiable forms for plain calls."""
+    if _functions:
+        return _functions
+
+    class Scan(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, values, gates, offsets, initial, program, mode):
+            out, final, carries = _scan_call(values, gates, offsets, initial, program, mode, True)
+            ctx.save_for_backward(values, gates, offsets, carries, initial)
+            ctx.program = program
+            ctx.set_materialize_grads(False)
+            return out, final
+
+        @staticmethod
+        def backward(ctx, grad_out, grad_final):
+            _first_derivative(torch)
+            if grad_out is None and grad_final is None:
+                return (None,) * 6
+            values, gates, offsets, carries, initial = ctx.saved_tensors
+            if grad_out is None:
+                grad_out = torch.zeros_like(values)
+            grads = _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final, ctx.program)
+            return grads[0], grads[1], None, grads[2] if initial is not None else None, None, None
+
+    class Matmul(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, values, weights, offsets, program, mode):
+            ctx.save_for_backward(values, weights, offsets)
+            ctx.program = program
+            ctx.set_materialize_grads(False)
+            return _matmul_call(values, weights, offsets, program, mode)
+
+        @staticmethod
+        def backward(ctx, grad_out):
+            _first_derivative(torch)
+            wanted = ctx.needs_input_grad[:2]
+            if grad_out is None or not any(wanted):
+                return (None,) * 5
+            values, weights, offsets = ctx.saved_tensors
+            return (*_matmul_backward_call(values, weights, offsets, grad_out, ctx.program, wanted), None, None, None)
+
+    _functions.update(scan=Scan, matmul=Matmul)
+    return _functions
+
+
 def _register_matmul(torch, library, contract) -> None:
     def matmul_kernel(values, weights, offsets, program, mode="validated"):
-        compiled = _table.lookup(program, "matmul")
-        values, weights = _dense(values, weights)
-        out = values.new_empty((values.shape[0], compiled.spec.out_dim))
-        compiled._run(values, weights, offsets, out, None, mode, False)
-        return out
+        return _matmul_call(values, weights, offsets, _table.lookup(program, "matmul"), mode)
 
     def matmul_backward_kernel(values, weights, offsets, grad_out, program, wanted):
-        compiled = _table.lookup(program, "matmul")
-        values, weights, grad_out = _dense(values, weights, grad_out)
-        grads = tuple(torch.empty_like(t) if want else t.new_empty((0,)) for t, want in zip((values, weights), wanted))
-        compiled.run_backward(values, weights, offsets, grad_out, grad_values=grads[0] if wanted[0] else None,
-                              grad_weights=grads[1] if wanted[1] else None)
-        return grads
+        grads = _matmul_backward_call(values, weights, offsets, grad_out, _table.lookup(program, "matmul"), wanted)
+        return tuple(values.new_empty((0,)) if g is None else g for g in grads)
 
     for key in ("CPU", "CUDA"):
         library.impl("segment_matmul", matmul_kernel, key)
@@ -392,8 +459,12 @@ def segment_scan(values, gates, offsets, *, program: CompiledScan, initial=None,
     on the stream they were first used on, and the capture fails.  Take the
     gradients with ``torch.autograd.grad``, or drop earlier graphs first."""
     torch = _torch()
-    register_torch_ops()
     record = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (values, gates, initial))
+    if _plain(torch, values, gates, offsets, initial):
+        if record:
+            return _autograd_functions(torch)["scan"].apply(values, gates, offsets, initial, program, mode)
+        return _scan_call(values, gates, offsets, initial, program, mode, False)[:2]
+    register_torch_ops()
     out, final, _ = torch.ops.ragged_mlir.segment_scan(values, gates, offsets, initial, register_program(program),
                                                        mode, record)
     return out, final
@@ -403,8 +474,13 @@ def segment_matmul(values, weights, offsets, *, program: CompiledMatmul, mode: s
     """[N, out] of values[t] @ weights[s] for the rows t of segment s,
     differentiable (once) in values and weights.  (On captured backward
     passes: see ``segment_scan``.)"""
+    torch = _torch()
+    if _plain(torch, values, weights, offsets):
+        if torch.is_grad_enabled() and (values.requires_grad or weights.requires_grad):
+            return _autograd_functions(torch)["matmul"].apply(values, weights, offsets, program, mode)
+        return _matmul_call(values, weights, offsets, program, mode)
     register_torch_ops()
-    return _torch().ops.ragged_mlir.segment_matmul(values, weights, offsets, register_program(program), mode)
+    return torch.ops.ragged_mlir.segment_matmul(values, weights, offsets, register_program(program), mode)
 
 
 def bind(program: CompiledProgram, *, mode: str = "validated"):

@@ -280,6 +280,27 @@ def test_gradients_are_the_differences_of_the_outputs(cuda):
         assert abs(there - base - (got[grad] * step).sum()) <= noise + more + slack, name
 
 
+@pytest.mark.parametrize("compiled", [False, True])
+def test_operator_in_a_graph(cuda, compiled):
+    """The operator below the eager call, alone and in a compiled full graph."""
+    torch = cuda
+    from ragged import torch_adapter
+    case = make_case([5, 0, 130, 2], 32, 48, "bf16")
+    t = device(torch, case, "bf16")
+    token = torch_adapter.register_program(matmul_program("bf16", 32, 48))
+    torch_adapter.register_torch_ops()
+
+    def model(values, weights, offsets):
+        return torch.ops.ragged_mlir.segment_matmul(values, weights, offsets, token)
+
+    if compiled:
+        model = torch.compile(model, backend="aot_eager", fullgraph=True)
+    leaves = [t[k].requires_grad_() for k in ("values", "weights")]
+    out = model(*leaves, t["offsets"])
+    gv, gw = torch.autograd.grad(out, leaves, t["grad_out"])
+    check(case, dict(out=host(out), grad_values=host(gv), grad_weights=host(gw)), "bf16")
+
+
 def test_jagged_tensors(cuda):
     torch = cuda
     from ragged import torch_adapter

@@ -290,15 +290,28 @@ def test_captured_calls_replay_on_new_inputs(cuda):
     del graphs
 
 
+@pytest.mark.parametrize("route", ["call", "operator", "compiled"])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-def test_autograd(cuda, dtype):
+def test_autograd(cuda, dtype, route):
+    """The eager call, the operator below it, and a compiled full graph."""
     torch = cuda
     from ragged import torch_adapter
     case = make_case(LENGTHS["mixed"], 40, dtype, True)
     t = device(torch, case, dtype, "i64")
     leaves = [t[k].requires_grad_() for k in ("values", "gates", "initial")]
-    out, final = torch_adapter.segment_scan(leaves[0], leaves[1], t["offsets"], program=scan_program(dtype, 40),
-                                            initial=leaves[2])
+    program = scan_program(dtype, 40)
+    if route == "call":
+        out, final = torch_adapter.segment_scan(leaves[0], leaves[1], t["offsets"], program=program, initial=leaves[2])
+    else:
+        token = torch_adapter.register_program(program)
+        torch_adapter.register_torch_ops()
+
+        def model(values, gates, initial, offsets):
+            return torch.ops.ragged_mlir.segment_scan(values, gates, offsets, initial, token)[:2]
+
+        if route == "compiled":
+            model = torch.compile(model, backend="aot_eager", fullgraph=True)
+        out, final = model(*leaves, t["offsets"])
     grads = torch.autograd.grad((out, final), leaves, (t["grad_out"], t["grad_final"]))
     got = dict(out=out, final=final, grad_values=grads[0], grad_gates=grads[1], grad_initial=grads[2])
     check(case, {k: host(v.detach()) for k, v in got.items()}, dtype)
