@@ -118,9 +118,13 @@ int launch_tensor_cols(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream
   constexpr bool weights = KIND == MATMUL_GRAD_WEIGHTS;
   const int64_t left_cols = KIND == MATMUL_GRAD_VALUES ? p.m : p.k;
   const int64_t left_dims[2] = {left_cols, p.n};
-  const int left_box[2] = {64, weights ? kTensorDepth : 32};
+  const int left_box[2] = {64, weights ? kTensorDepth : kTensorRows}, part_box[2] = {64, 32};
   status = make_tensor_map(&maps.left, p.left, 2, left_dims, &p.left_pitch, left_box);
   if (status) return status;
+  if (!weights) {
+    status = make_tensor_map(&maps.left_part, p.left, 2, left_dims, &p.left_pitch, part_box);
+    if (status) return status;
+  }
   if (weights) {
     const int64_t dims[2] = {p.m, p.n};
     const int box[2] = {64, kTensorDepth};

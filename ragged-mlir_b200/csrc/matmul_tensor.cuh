@@ -40,7 +40,7 @@ constexpr int tensor_stages(int cols) { return cols == 256 ? 4 : cols == 128 ? 6
 constexpr int tensor_smem_bytes(int cols) { return tensor_stages(cols) * (kLeftBytes + cols * 128) + kStoreBytes + 1024; }
 
 struct TensorMaps {
-  CUtensorMap left, right;
+  CUtensorMap left, left_part, right;  // left_part: boxes of 32 rows
 };
 
 __device__ __forceinline__ void tma_load_3d(void *smem_dst, const void *map, int x, int y, int z, uint64_t *bar) {
@@ -188,8 +188,12 @@ matmul_tensor_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps
             for (int i = 0; i < COLS / 64; ++i)
               tma_load_2d(right + i * kSlab, &maps.right, col0 + i * 64, row, &full[stage]);
           } else {
-            for (int i = 0; i < boxes; ++i)
-              tma_load_2d(left + i * 32 * 128, &maps.left, d0, static_cast<int>(t.row) + i * 32, &full[stage]);
+            if (boxes == 4) {
+              tma_load_2d(left, &maps.left, d0, static_cast<int>(t.row), &full[stage]);
+            } else {
+              for (int i = 0; i < boxes; ++i)
+                tma_load_2d(left + i * 32 * 128, &maps.left_part, d0, static_cast<int>(t.row) + i * 32, &full[stage]);
+            }
             if constexpr (RIGHT_MN) {
 #pragma unroll
               for (int i = 0; i < COLS / 64; ++i)

@@ -43,6 +43,7 @@ class _LayerProgram:
         self._dtypes = None
         self._sizes: dict[tuple, int] = {}
         self._launches: dict[tuple, _Launch] = {}
+        self._reports: dict[tuple, dict] = {}
 
     schedules = property(lambda self: (self.spec.op,))
     _check_offsets = CompiledProgram._check_offsets
@@ -124,25 +125,29 @@ class _LayerProgram:
                 raise RuntimeUnavailable(f"compiled target {self.spec.chip} does not run on the current device "
                                          f"(sm_{capability[0]}{capability[1]})")
             _checked_devices.add(device.index)
-        active = stream if stream is not None else torch.cuda.current_stream()
-        if not isinstance(active, torch.cuda.Stream) or active.device != device:
+        if stream is not None and (not isinstance(stream, torch.cuda.Stream) or stream.device != device):
             raise ValidationError("stream must be a torch.cuda.Stream on the values device")
-        validation = self._check_offsets(offsets, offsets, n, b, active, torch) if checked else None
+        validation, active = None, stream
+        if checked:
+            active = stream if stream is not None else torch.cuda.current_stream()
+            validation = self._check_offsets(offsets, offsets, n, b, active, torch)
         launches, total = (), 0
         if b:
-            on = active.cuda_stream
+            # (the current stream's handle alone: a Stream object costs as much as a launch)
+            on = stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(device.index)
             if stream is not None:
                 for tensor in used:
-                    tensor.record_stream(active)
+                    tensor.record_stream(stream)
             for key, nbytes, call in work:
                 address = 0
                 if nbytes:
                     # Scratch comes from the caching allocator on the execution
                     # stream, so reuse is ordered after this call's kernels.
-                    with torch.cuda.stream(active) if stream is not None else nullcontext():
+                    with torch.cuda.stream(stream) if stream is not None else nullcontext():
                         scratch = torch.empty((nbytes,), dtype=torch.uint8, device=device)
                     address = scratch.data_ptr()
-                    total = max(total, nbytes)
+                    if nbytes > total:
+                        total = nbytes
                 launch = self._launches.get(key)
                 if launch is None:
                     report = _native.Report()
@@ -167,17 +172,29 @@ class _LayerProgram:
             raise RuntimeError("a bounded wait inside the kernel gave up; the call's results are undefined")
 
     def _report(self, started, launches, nbytes, validation) -> ExecutionReport:
-        check, check_ms = validation if validation is not None else (None, None)
-        parts = (_Launch(check),) + launches if check is not None else launches
-        checked_bytes = STATUS_BYTES if check is not None else 0
-        last = launches[-1] if launches else None
-        return ExecutionReport(("rows",) if launches else (), (), sum((x.grids for x in parts), ()),
-                               nbytes + checked_bytes, self._digest, None,
-                               "checked" if check is not None else "validated", sum((x.names for x in parts), ()),
-                               (time.perf_counter() - started) * 1000, cache_hit=self.cache_hit,
-                               validation_workspace_bytes=checked_bytes, validation_host_ms=check_ms,
-                               d_tile=last.d_tile if last else None, d_vector=last.d_vector if last else 1,
-                               selected=self.spec.op)
+        """The call's report: what depends on its launches alone is kept, as
+        filling all the fields costs a good part of a small call."""
+        template = self._reports.get(launches) if validation is None else None
+        if template is None:
+            check, check_ms = validation if validation is not None else (None, None)
+            parts = (_Launch(check),) + launches if check is not None else launches
+            checked_bytes = STATUS_BYTES if check is not None else 0
+            last = launches[-1] if launches else None
+            template = ExecutionReport(("rows",) if launches else (), (), sum((x.grids for x in parts), ()),
+                                       nbytes + checked_bytes, self._digest, None,
+                                       "checked" if check is not None else "validated",
+                                       sum((x.names for x in parts), ()), cache_hit=self.cache_hit,
+                                       validation_workspace_bytes=checked_bytes, validation_host_ms=check_ms,
+                                       d_tile=last.d_tile if last else None, d_vector=last.d_vector if last else 1,
+                                       selected=self.spec.op).__dict__
+            if check is None:
+                if len(self._reports) >= 256:
+                    self._reports.clear()
+                self._reports[launches] = template
+        report = object.__new__(ExecutionReport)
+        report.__dict__.update(template, workspace_bytes=nbytes + template["validation_workspace_bytes"],
+                               host_enqueue_ms=(time.perf_counter() - started) * 1000)
+        return report
 
 
 class _Launch:
