@@ -100,7 +100,7 @@ struct TensorRange {
 int check_ranges(const TensorRange *ranges, int count);
 void clear_report(rg_report *report);
 
-// Tensor map of a bf16 tensor of `rank` (2 or 3) dimensions, the innermost
+// Tensor map of a bf16 tensor of `rank` (2 to 4) dimensions, the innermost
 // first; `strides` (elements, of the outer dimensions) are multiples of 8 and
 // `base` is 16-byte aligned.  Its boxes are 128 bytes wide, and their 16-byte
 // pieces permuted within groups of 8 rows (the 128-byte swizzle of tcgen05).

@@ -168,9 +168,9 @@ int make_tensor_map(CUtensorMap *map, const void *base, int rank, const int64_t 
       return fail(RG_ERR_DEVICE, "the CUDA driver has no cuTensorMapEncodeTiled");
     cached.store(entry);
   }
-  cuuint64_t sizes[3], pitches[2];
-  cuuint32_t boxes[3];
-  const cuuint32_t steps[3] = {1, 1, 1};
+  cuuint64_t sizes[4], pitches[3];
+  cuuint32_t boxes[4];
+  const cuuint32_t steps[4] = {1, 1, 1, 1};
   for (int i = 0; i < rank; ++i) {
     sizes[i] = static_cast<cuuint64_t>(dims[i]);
     boxes[i] = static_cast<cuuint32_t>(box[i]);

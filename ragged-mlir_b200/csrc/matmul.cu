@@ -117,18 +117,31 @@ int launch_tensor_cols(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream
   std::memset(&maps, 0, sizeof maps);
   constexpr bool weights = KIND == MATMUL_GRAD_WEIGHTS;
   const int64_t left_cols = KIND == MATMUL_GRAD_VALUES ? p.m : p.k;
-  const int64_t left_dims[2] = {left_cols, p.n};
-  const int left_box[2] = {64, weights ? kTensorDepth : kTensorRows}, part_box[2] = {64, 32};
-  status = make_tensor_map(&maps.left, p.left, 2, left_dims, &p.left_pitch, left_box);
-  if (status) return status;
-  if (!weights) {
-    status = make_tensor_map(&maps.left_part, p.left, 2, left_dims, &p.left_pitch, part_box);
-    if (status) return status;
+  if (weights && left_cols % 64 == 0) {
+    const int64_t dims[3] = {64, p.n, left_cols / 64}, strides[2] = {p.left_pitch, 64};
+    const int box[3] = {64, kTensorDepth, kTensorRows / 64};
+    status = make_tensor_map(&maps.left, p.left, 3, dims, strides, box);
+    maps.left_slabs = 1;
+  } else {
+    const int64_t dims[2] = {left_cols, p.n};
+    const int box[2] = {64, weights ? kTensorDepth : kTensorRows}, part[2] = {64, 32};
+    status = make_tensor_map(&maps.left, p.left, 2, dims, &p.left_pitch, box);
+    if (!status && !weights) status = make_tensor_map(&maps.left_part, p.left, 2, dims, &p.left_pitch, part);
   }
-  if (weights) {
+  if (status) return status;
+  maps.right_slabs = KIND != MATMUL_GRAD_VALUES && p.m % 64 == 0;
+  if (weights && maps.right_slabs) {
+    const int64_t dims[3] = {64, p.n, p.m / 64}, strides[2] = {p.right_pitch, 64};
+    const int box[3] = {64, kTensorDepth, COLS / 64};
+    status = make_tensor_map(&maps.right, p.right, 3, dims, strides, box);
+  } else if (weights) {
     const int64_t dims[2] = {p.m, p.n};
     const int box[2] = {64, kTensorDepth};
     status = make_tensor_map(&maps.right, p.right, 2, dims, &p.right_pitch, box);
+  } else if (maps.right_slabs) {
+    const int64_t dims[4] = {64, p.k, p.m / 64, p.b}, strides[3] = {p.right_pitch, 64, p.right_pitch * p.k};
+    const int box[4] = {64, kTensorDepth, COLS / 64, 1};
+    status = make_tensor_map(&maps.right, p.right, 4, dims, strides, box);
   } else {
     const int64_t dims[3] = {p.m, p.k, p.b}, strides[2] = {p.right_pitch, p.right_pitch * p.k};
     const int box[3] = {64, KIND == MATMUL_FORWARD ? kTensorDepth : COLS, 1};

@@ -41,6 +41,9 @@ constexpr int tensor_smem_bytes(int cols) { return tensor_stages(cols) * (kLeftB
 
 struct TensorMaps {
   CUtensorMap left, left_part, right;  // left_part: boxes of 32 rows
+  // MN-major operands whose width is a multiple of 64 are mapped with their
+  // slabs of 64 as a dimension of their own, and a tile's slabs come in one box.
+  int left_slabs, right_slabs;
 };
 
 __device__ __forceinline__ void tma_load_3d(void *smem_dst, const void *map, int x, int y, int z, uint64_t *bar) {
@@ -48,6 +51,14 @@ __device__ __forceinline__ void tma_load_3d(void *smem_dst, const void *map, int
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n" ::"r"(
           smem_u32(smem_dst)),
       "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(void *smem_dst, const void *map, int x, int y, int z, int w, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
 }
 
@@ -181,12 +192,18 @@ matmul_tensor_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps
           const int d0 = static_cast<int>(k * DEPTH);
           if constexpr (LEFT_MN) {
             const int row = static_cast<int>(t.begin) + d0;
-#pragma unroll
-            for (int i = 0; i < ROWS / 64; ++i)
-              tma_load_2d(left + i * kSlab, &maps.left, static_cast<int>(t.row) + i * 64, row, &full[stage]);
-#pragma unroll
-            for (int i = 0; i < COLS / 64; ++i)
-              tma_load_2d(right + i * kSlab, &maps.right, col0 + i * 64, row, &full[stage]);
+            if (maps.left_slabs) {
+              tma_load_3d(left, &maps.left, 0, row, static_cast<int>(t.row) / 64, &full[stage]);
+            } else {
+              for (int i = 0; i < ROWS / 64; ++i)
+                tma_load_2d(left + i * kSlab, &maps.left, static_cast<int>(t.row) + i * 64, row, &full[stage]);
+            }
+            if (maps.right_slabs) {
+              tma_load_3d(right, &maps.right, 0, row, col0 / 64, &full[stage]);
+            } else {
+              for (int i = 0; i < COLS / 64; ++i)
+                tma_load_2d(right + i * kSlab, &maps.right, col0 + i * 64, row, &full[stage]);
+            }
           } else {
             if (boxes == 4) {
               tma_load_2d(left, &maps.left, d0, static_cast<int>(t.row), &full[stage]);
@@ -195,9 +212,12 @@ matmul_tensor_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps
                 tma_load_2d(left + i * 32 * 128, &maps.left_part, d0, static_cast<int>(t.row) + i * 32, &full[stage]);
             }
             if constexpr (RIGHT_MN) {
-#pragma unroll
-              for (int i = 0; i < COLS / 64; ++i)
-                tma_load_3d(right + i * kSlab, &maps.right, col0 + i * 64, d0, static_cast<int>(t.seg), &full[stage]);
+              if (maps.right_slabs) {
+                tma_load_4d(right, &maps.right, 0, d0, col0 / 64, static_cast<int>(t.seg), &full[stage]);
+              } else {
+                for (int i = 0; i < COLS / 64; ++i)
+                  tma_load_3d(right + i * kSlab, &maps.right, col0 + i * 64, d0, static_cast<int>(t.seg), &full[stage]);
+              }
             } else {
               tma_load_3d(right, &maps.right, d0, col0, static_cast<int>(t.seg), &full[stage]);
             }
