@@ -80,14 +80,16 @@ template <typename OffT, int KIND, int TILE, int SIZE>
 int launch_simt_tile(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
   const auto kernel = matmul_simt_kernel<OffT, KIND, TILE, SIZE>;
   int per_sm = 0;
-  const int status = prepare_kernel(reinterpret_cast<const void *>(kernel), dev.device, kSimtThreads, 0, 0, &per_sm);
+  constexpr int smem = simt_smem_bytes(TILE);
+  const int status =
+      prepare_kernel(reinterpret_cast<const void *>(kernel), dev.device, kSimtThreads, smem, smem, &per_sm);
   if (status) return status;
   p.col_tiles = static_cast<int>(ceil_div(p.cols, TILE));
   p.row_tiles = static_cast<int>(ceil_div(p.k, TILE));
   const int64_t tiles = most_row_tiles(KIND, p, TILE) * p.col_tiles;
   const dim3 grid(static_cast<unsigned>(std::min(tiles, static_cast<int64_t>(per_sm) * dev.sm_count)), 1, 1);
-  kernel<<<grid, kSimtThreads, 0, stream>>>(p);
-  record_launch(report, K_MATMUL_SIMT, grid, kSimtThreads, 0);
+  kernel<<<grid, kSimtThreads, smem, stream>>>(p);
+  record_launch(report, K_MATMUL_SIMT, grid, kSimtThreads, smem);
   return check_cuda(cudaGetLastError(), "matmul_simt_kernel launch");
 }
 

@@ -3,10 +3,10 @@
 // f32 tensors take this kernel: the tensor cores round f32 operands to 10-bit
 // (tf32) or fewer bits of mantissa.  A CTA of 256 threads computes a TILE x
 // TILE block of the output, 8 x 8 (4 x 4) values a thread held in registers, from
-// slices of 16 of the contraction in shared memory, the next slice on its way
-// in registers; two CTAs an SM fill each other's waits.  Bound: 128 FMAs a
-// clock and SM; a thread loads 16 values from shared memory for 64 FMAs, so the
-// pipes and not the loads set the pace.
+// slices of 16 of the contraction in a ring of shared-memory stages that
+// asynchronous copies fill three slices ahead; two CTAs an SM fill each other's
+// waits.  Bound: 128 FMAs a clock and SM; a thread loads 16 values from shared
+// memory for 64 FMAs, so the pipes and not the loads set the pace.
 #pragma once
 
 #include "matmul.cuh"
@@ -15,51 +15,54 @@ namespace rgb {
 
 constexpr int kSimtThreads = 256;
 constexpr int kSimtDepth = 16;
+constexpr int kSimtStages = 4;
 
-// A thread's share of a slice of one operand: pieces of SIZE elements.  ALONG:
-// the tile's rows (columns) are contiguous in memory; else the contraction is.
+constexpr int simt_pitch(int tile) { return tile + 4; }
+constexpr int simt_smem_bytes(int tile) { return kSimtStages * 2 * kSimtDepth * simt_pitch(tile) * 4; }
+
+// Copies BYTES (4 or 16) or, not `ok`, writes zeros.
+template <int BYTES>
+__device__ __forceinline__ void copy_or_zero(uint32_t to, const float *from, bool ok) {
+  const int count = ok ? BYTES : 0;
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(to), "l"(from), "r"(count) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(to), "l"(from), "r"(count) : "memory");
+}
+
+// A thread's share of a slice of one operand, [contraction][tile] in shared
+// memory.  ALONG: the tile's rows (columns) are contiguous in memory, and SIZE
+// of them go at once; else the contraction is, and elements go one by one.
 template <int TILE, int SIZE, bool ALONG>
 struct SimtOperand {
-  static constexpr int kPieces = TILE * kSimtDepth / (kSimtThreads * SIZE);
-  static constexpr int kAcross = (ALONG ? TILE : kSimtDepth) / SIZE;  // pieces of a line
-  static constexpr int kLines = kSimtThreads / kAcross;               // lines between a thread's pieces
-  using Piece = typename std::conditional<SIZE == 4, float4, float>::type;
-  const float *at;
+  static constexpr int kSize = ALONG ? SIZE : 1;
+  static constexpr int kPieces = TILE * kSimtDepth / (kSimtThreads * kSize);
+  static constexpr int kAcross = (ALONG ? TILE : kSimtDepth) / kSize;  // pieces of a line
+  static constexpr int kLines = kSimtThreads / kAcross;                // lines between a thread's pieces
+  const float *base, *at;
   int64_t pitch;
-  int line, place;   // of the first piece
-  int64_t limit;     // lines (elements of a line) of the tile that exist
-  Piece piece[kPieces];
+  int line, place;  // of the first piece
+  int64_t limit;    // lines (elements of a line) of the tile that exist
 
-  __device__ __forceinline__ void begin(const float *base, int64_t row_pitch, int64_t first, int64_t end) {
+  __device__ __forceinline__ void begin(const float *from, int64_t row_pitch, int64_t first, int64_t end) {
     line = threadIdx.x / kAcross;
-    place = threadIdx.x % kAcross * SIZE;
+    place = threadIdx.x % kAcross * kSize;
     pitch = row_pitch;
     limit = end - first;
+    base = from;
     at = ALONG ? base + line * pitch + first + place : base + (first + line) * pitch + place;
   }
-  // The slice with `left` of the contraction to go; moves on to the next.
-  __device__ __forceinline__ void load(int64_t left) {
+  // Starts the copies of the slice with `left` of the contraction to go (none:
+  // zeros); moves on to the next.
+  __device__ __forceinline__ void copy(uint32_t stage, int64_t left) {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       const int l = line + i * kLines;
       const bool ok = ALONG ? l < left && place < limit : l < limit && place < left;
-      piece[i] = ok ? __ldg(reinterpret_cast<const Piece *>(at + i * kLines * pitch)) : Piece{};
+      const uint32_t to = stage + (ALONG ? l * simt_pitch(TILE) + place : place * simt_pitch(TILE) + l) * 4;
+      copy_or_zero<kSize * 4>(to, ok ? at + i * kLines * pitch : base, ok);
     }
     at += ALONG ? kSimtDepth * pitch : int64_t{kSimtDepth};
-  }
-  template <int PITCH>
-  __device__ __forceinline__ void stage(float (*to)[PITCH]) const {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int l = line + i * kLines;
-      if constexpr (ALONG) {
-        *reinterpret_cast<Piece *>(&to[l][place]) = piece[i];
-      } else {
-        const float *x = reinterpret_cast<const float *>(&piece[i]);
-#pragma unroll
-        for (int e = 0; e < SIZE; ++e) to[place + e][l] = x[e];
-      }
-    }
   }
 };
 
@@ -67,8 +70,9 @@ template <typename OffT, int KIND, int TILE, int SIZE>
 __global__ void __launch_bounds__(kSimtThreads, TILE == 128 ? 2 : 3) matmul_simt_kernel(const MatmulArgs p) {
   constexpr int DEPTH = kSimtDepth;
   constexpr int PER = TILE / 16;  // outputs of a thread in each direction
-  constexpr int PITCH = TILE + 4;
-  __shared__ __align__(16) float left_s[2][DEPTH][PITCH], right_s[2][DEPTH][PITCH];
+  constexpr int PITCH = simt_pitch(TILE);
+  constexpr int kOperand = DEPTH * PITCH;  // floats of an operand's stage
+  extern __shared__ __align__(16) float simt_smem[];
   float *__restrict__ out = static_cast<float *>(p.out);
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   MatmulWalk<OffT, KIND, TILE> walk(p.offsets, p.b);
@@ -89,20 +93,26 @@ __global__ void __launch_bounds__(kSimtThreads, TILE == 128 ? 2 : 3) matmul_simt
     for (int i = 0; i < PER; ++i)
 #pragma unroll
       for (int j = 0; j < PER / 2; ++j) acc[i][j] = 0;
-    if (depth > 0) {
-      left.load(depth);
-      right.load(depth);
-    }
-    int buffer = 0;
-#pragma unroll 1
-    for (int64_t to_go = depth; to_go > 0; to_go -= DEPTH, buffer ^= 1) {
-      left.stage(left_s[buffer]);
-      right.stage(right_s[buffer]);
-      __syncthreads();  // the slice is there; the other buffer's readers are done
-      if (to_go > DEPTH) {
-        left.load(to_go - DEPTH);
-        right.load(to_go - DEPTH);
+    int64_t ahead = depth;  // of the contraction, not asked for yet
+    auto copy = [&](int stage) {
+      if (ahead > 0) {
+        const uint32_t to = smem_u32(simt_smem + stage * 2 * kOperand);
+        left.copy(to, ahead);
+        right.copy(to + kOperand * 4, ahead);
       }
+      ahead -= DEPTH;
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kSimtStages - 1; ++i) copy(i);
+    int stage = 0;
+#pragma unroll 1
+    for (int64_t to_go = depth; to_go > 0; to_go -= DEPTH) {
+      cp_async_wait<kSimtStages - 2>();
+      __syncthreads();  // all copies of the slice are there, and the last slice's readers done
+      copy((stage + kSimtStages - 1) % kSimtStages);
+      const float *left_s = simt_smem + stage * 2 * kOperand, *right_s = left_s + kOperand;
+      stage = (stage + 1) % kSimtStages;
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) {
         float l[PER];
@@ -111,9 +121,9 @@ __global__ void __launch_bounds__(kSimtThreads, TILE == 128 ? 2 : 3) matmul_simt
         // loads then meet no other thread's banks.
 #pragma unroll
         for (int g = 0; g < PER / 4; ++g) {
-          const float4 v = *reinterpret_cast<const float4 *>(&left_s[buffer][d][g * 64 + ty * 4]);
+          const float4 v = *reinterpret_cast<const float4 *>(left_s + d * PITCH + g * 64 + ty * 4);
           l[g * 4] = v.x; l[g * 4 + 1] = v.y; l[g * 4 + 2] = v.z; l[g * 4 + 3] = v.w;
-          const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(&right_s[buffer][d][g * 64 + tx * 4]);
+          const ulonglong2 w = *reinterpret_cast<const ulonglong2 *>(right_s + d * PITCH + g * 64 + tx * 4);
           r[g * 2] = w.x;
           r[g * 2 + 1] = w.y;
         }
@@ -147,6 +157,7 @@ __global__ void __launch_bounds__(kSimtThreads, TILE == 128 ? 2 : 3) matmul_simt
         }
       }
     }
+    cp_async_wait<0>();
     __syncthreads();  // the last slice has been read
   }
 }
