@@ -382,7 +382,7 @@ struct ScanWarp {
 };
 
 template <typename T, typename OffT, int VEC, bool BACKWARD>
-__global__ void __launch_bounds__(kScanThreads, 3) scan_fold_kernel(const ScanArgs p) {
+__global__ void __launch_bounds__(kScanThreads, 4) scan_fold_kernel(const ScanArgs p) {
   extern __shared__ unsigned scan_smem[];
   grid_dependents_launch();
   ScanWarp<T, OffT, VEC, BACKWARD> w(p, scan_smem);
@@ -422,6 +422,9 @@ __device__ __forceinline__ ScanSpan scan_span(const float2 &pair) {
   return ScanSpan{pair.x, pair.y, __float_as_uint(pair.x) == kScanReset};
 }
 
+// (Pairs and states are read past L1: the launch that writes them may still
+// run when the one that reads them starts.)
+//
 // 8 columns by 128 parts of the slabs a block: each thread composes its part,
 // a doubling scan over the parts gives the state before each, and each thread
 // goes through its part again (from registers up to 8 slabs a part).
@@ -438,7 +441,7 @@ __global__ void __launch_bounds__(kJoinCols * kJoinParts) scan_join_kernel(const
   auto load = [&](int64_t s) {
 #pragma unroll
     for (int i = 0; i < kJoinBatch; ++i)
-      if (s + i < end) pair[i] = pairs[(s + i) * p.d];
+      if (s + i < end) pair[i] = __ldcg(pairs + (s + i) * p.d);
   };
   grid_dependents_launch();
   grid_dependency_wait();
@@ -513,8 +516,10 @@ __global__ void __launch_bounds__(kScanThreads, BACKWARD ? 2 : 3) scan_walk_kern
         }
 #pragma unroll
         for (int v = 0; v < VEC; ++v) h[v] = 0.0f;
-        if (w.col_ok && !(BACKWARD ? w.ends_at_last() : w.starts_at_first()))
-          State::load(p.states + w.pos * p.d + w.col, h);
+        if (w.col_ok && !(BACKWARD ? w.ends_at_last() : w.starts_at_first())) {
+#pragma unroll
+          for (int v = 0; v < VEC; ++v) h[v] = __ldcg(p.states + w.pos * p.d + w.col + v);
+        }
 #pragma unroll
         for (int v = 0; v < VEC; ++v) h[v] = reset ? f.h[v] : scan_apply(f.a[v], f.h[v], h[v]);
       }

@@ -162,12 +162,15 @@ class _LayerProgram:
                     self._check_status_words(scratch, launch, active, torch)
         return self._report(started, launches, total, validation)
 
-    @staticmethod
-    def _check_status_words(scratch, launch, active, torch):
-        """Checked mode, after the launch: the words in which the last
-        launch's CTAs say that a bounded wait gave up."""
+    def _status_words(self, launch) -> int:
+        """Words at a report's status_offset (CompiledProgram's: one)."""
+        return 1
+
+    def _check_status_words(self, scratch, launch, active, torch):
+        """Checked mode, after the launch: the words in which a bounded wait
+        that gave up says so."""
         with torch.cuda.stream(active):
-            words = scratch.narrow(0, launch.status_offset, 8 * launch.grids[-1][0]).view(torch.int64).cpu()
+            words = scratch.narrow(0, launch.status_offset, 8 * self._status_words(launch)).view(torch.int64).cpu()
         if words.any():
             raise RuntimeError("a bounded wait inside the kernel gave up; the call's results are undefined")
 
@@ -298,6 +301,9 @@ class CompiledMatmul(_LayerProgram):
     """out[t] = values[t] @ weights[s] for the rows t of segment s."""
 
     kind = MatmulSpec
+
+    def _status_words(self, launch) -> int:
+        return launch.grids[-1][0]  # one for each CTA
 
     def _product(self, kind, left, right, offsets, out, n, b):
         """(key, scratch bytes, call) of one product."""
