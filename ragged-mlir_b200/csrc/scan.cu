@@ -14,27 +14,33 @@ constexpr int64_t kMaxScanDim = 65536;
 
 
 struct ScanShape {
-  int pair;            // elements of 4 bytes of a row (1 where D is odd)
-  int vec;             // of this call: 1 where a tensor is not aligned for pairs
-  int shift, lane_rows, row_shift, tiles;
+  int vec, tiles;            // 4 bytes of a row a lane (one element where D is odd or a tensor is not aligned)
+  int wide_vec, wide_tiles;  // 8 bytes where they fill 32 lanes, else as vec
+  int shift, lane_rows, row_shift;
   int64_t slabs, blocks;
 };
 
 constexpr int64_t kAloneRows = 256;  // rows up to which walk is the only launch
 
-// 32 lanes, or as many as cover a row, of one vector each.  A lane takes 64
-// rows of a slab, fewer where that would leave resident warps without a task.
-ScanShape make_shape(int dtype, int64_t d, int64_t n, int64_t b, bool aligned_pairs) {
+// 32 lanes, or as many as cover a row, of one vector each.  8 bytes a lane take
+// two thirds of the instructions of 4 (B200, bf16 65536 x 1024: see the kernels);
+// a backward walk, which keeps 16 states of each column, has the registers for
+// 4.  A lane takes 64 rows of a slab, fewer where that would leave resident
+// warps without a task.  `align`: elements that all tensors are aligned for.
+ScanShape make_shape(int dtype, int64_t d, int64_t n, int64_t b, int align) {
   ScanShape s;
-  s.pair = dtype == RG_DTYPE_BF16 && d % 2 == 0 ? 2 : 1;
-  s.vec = aligned_pairs ? s.pair : 1;
+  s.vec = dtype == RG_DTYPE_BF16 && d % 2 == 0 && align >= 2 ? 2 : 1;
   s.shift = 0;
   while ((int64_t{1} << s.shift) * s.vec < d && s.shift < 5) ++s.shift;
   s.tiles = static_cast<int>(ceil_div(d, (int64_t{1} << s.shift) * s.vec));
+  const int wide = 8 / elem_bytes(dtype);
+  s.wide_vec = d % wide == 0 && d >= 32 * wide && align >= wide ? wide : s.vec;
+  s.wide_tiles = static_cast<int>(ceil_div(d, (int64_t{1} << s.shift) * s.wide_vec));
   const int groups = 32 >> s.shift;
   constexpr int64_t warps = 148 * 24;
   s.lane_rows = 64;
-  while (s.lane_rows > 16 && (ceil_div(n, s.lane_rows * groups) * s.tiles < warps || s.lane_rows * groups > 512))
+  while (s.lane_rows > 16 &&
+         (ceil_div(n, s.lane_rows * groups) * s.wide_tiles < warps || s.lane_rows * groups > 512))
     s.lane_rows /= 2;
   s.row_shift = 0;
   while ((1 << s.row_shift) < s.lane_rows * groups) ++s.row_shift;
@@ -64,15 +70,17 @@ int check_shape(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b) {
   return RG_OK;
 }
 
-// Whether the tensors' alignment (of one element, in `r`) allows pairs.
-bool pairs_aligned(const TensorRange *r, int count) {
+// Elements (4, 2 or 1) that all tensors are aligned for (in `r`: one's alignment).
+int aligned_elements(const TensorRange *r, int count) {
+  int most = 4;
   for (int i = 0; i < count; ++i)
-    if (std::strcmp(r[i].name, "offsets") && r[i].bytes && !aligned(r[i].ptr, r[i].align * 2)) return false;
-  return true;
+    while (std::strcmp(r[i].name, "offsets") && r[i].bytes && !aligned(r[i].ptr, r[i].align * most)) most /= 2;
+  return most;
 }
 
-template <typename T, typename OffT, int VEC, bool BACKWARD>
-int launch(const ScanArgs &p, const ScanShape &s, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
+// WIDE: of fold and of a forward walk.
+template <typename T, typename OffT, int WIDE, int VEC, bool BACKWARD>
+int launch(ScanArgs p, const ScanShape &s, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
   const int smem = kScanWarps * scan_marks_words(1 << s.row_shift) * 4;
   constexpr int usual = kScanWarps * scan_marks_words(64) * 4, limit = kScanWarps * scan_marks_words(512) * 4;
   // The second and third launch may start before the one before them ends.
@@ -90,50 +98,54 @@ int launch(const ScanArgs &p, const ScanShape &s, const DeviceProps &dev, cudaSt
     record_launch(report, id, config.gridDim, threads, bytes);
     return check_cuda(cudaLaunchKernelEx(&config, kernel, p), "scan kernel launch");
   };
-  auto run = [&](void (*kernel)(ScanArgs), int id, int64_t tasks, bool after) {
+  auto run = [&](void (*kernel)(ScanArgs), int id, int64_t slabs, int tiles, bool after) {
     int per_sm = 0;
+    p.tiles = tiles;
     int status = prepare_kernel(reinterpret_cast<const void *>(kernel), dev.device, kScanThreads, usual, limit, &per_sm);
     if (status) return status;
-    return start(kernel, id, std::min(static_cast<int64_t>(per_sm) * dev.sm_count, ceil_div(tasks, kScanWarps)),
+    return start(kernel, id, std::min(static_cast<int64_t>(per_sm) * dev.sm_count, ceil_div(slabs * tiles, kScanWarps)),
                  kScanThreads, smem, after);
   };
   if (p.pairs) {
-    int status = run(scan_fold_kernel<T, OffT, VEC, BACKWARD>, BACKWARD ? K_SCAN_FOLD_BACKWARD : K_SCAN_FOLD,
-                     s.slabs * s.tiles, false);
+    int status = run(scan_fold_kernel<T, OffT, WIDE, BACKWARD>, BACKWARD ? K_SCAN_FOLD_BACKWARD : K_SCAN_FOLD, s.slabs,
+                     s.wide_tiles, false);
     if (status) return status;
     status = start(scan_join_kernel, K_SCAN_JOIN, ceil_div(p.d, kJoinCols), kJoinCols * kJoinParts, 0, true);
     if (status) return status;
   }
-  return run(scan_walk_kernel<T, OffT, VEC, BACKWARD>, BACKWARD ? K_SCAN_BACKWARD : K_SCAN, s.blocks * s.tiles,
-             p.pairs != nullptr);
+  return run(scan_walk_kernel<T, OffT, BACKWARD ? VEC : WIDE, BACKWARD>, BACKWARD ? K_SCAN_BACKWARD : K_SCAN, s.blocks,
+             BACKWARD ? s.tiles : s.wide_tiles, p.pairs != nullptr);
 }
 
 template <typename OffT, bool BACKWARD>
 int launch_vec(int dtype, const ScanArgs &p, const ScanShape &s, const DeviceProps &dev, cudaStream_t stream,
                rg_report *report) {
-  if (dtype == RG_DTYPE_F32) return launch<float, OffT, 1, BACKWARD>(p, s, dev, stream, report);
-  if (s.vec == 2) return launch<__nv_bfloat16, OffT, 2, BACKWARD>(p, s, dev, stream, report);
-  return launch<__nv_bfloat16, OffT, 1, BACKWARD>(p, s, dev, stream, report);
+  if (dtype == RG_DTYPE_F32) {
+    if (s.wide_vec == 2) return launch<float, OffT, 2, 1, BACKWARD>(p, s, dev, stream, report);
+    return launch<float, OffT, 1, 1, BACKWARD>(p, s, dev, stream, report);
+  }
+  if (s.wide_vec == 4) return launch<__nv_bfloat16, OffT, 4, 2, BACKWARD>(p, s, dev, stream, report);
+  if (s.vec == 2) return launch<__nv_bfloat16, OffT, 2, 2, BACKWARD>(p, s, dev, stream, report);
+  return launch<__nv_bfloat16, OffT, 1, 1, BACKWARD>(p, s, dev, stream, report);
 }
 
 template <bool BACKWARD>
-int run_scan(int dtype, int index_dtype, bool aligned_pairs, ScanArgs &p, void *workspace, int64_t workspace_bytes,
+int run_scan(int dtype, int index_dtype, int align, ScanArgs &p, void *workspace, int64_t workspace_bytes,
              cudaStream_t stream, rg_report *report) {
   DeviceProps dev;
   int status = check_device(&dev);
   if (status) return status;
-  const ScanShape s = make_shape(dtype, p.d, p.n, p.b, aligned_pairs);
+  const ScanShape s = make_shape(dtype, p.d, p.n, p.b, align);
   if (s.blocks > 2000000000LL / s.tiles) return fail(RG_ERR_INVALID_ARGUMENT, "the call needs more than 2e9 tasks");
   const int64_t need = layout_bytes(s, p.n, p.d);
   if (report) {
     report->workspace_bytes = need;
-    report->d_vector = s.vec;
+    report->d_vector = BACKWARD ? s.vec : s.wide_vec;
     report->d_tile = 1 << s.shift;
   }
   p.shift = s.shift;
   p.lane_rows = s.lane_rows;
   p.row_shift = s.row_shift;
-  p.tiles = s.tiles;
   p.slabs = s.slabs;
   p.blocks = s.blocks;
   p.per_block = ceil_div(p.b, s.blocks);
@@ -159,11 +171,10 @@ int rg_scan_workspace_bytes(int dtype, int index_dtype, int64_t d, int64_t n, in
   if (!bytes) return fail(RG_ERR_INVALID_ARGUMENT, "bytes is NULL");
   const int status = check_shape(dtype, index_dtype, d, n, b);
   if (status) return status;
-  // The pairs take the same bytes per column, but the tiles and the slabs that
-  // go by them differ with the alignment of the tensors.
-  const int64_t pairs = layout_bytes(make_shape(dtype, d, n, b, true), n, d);
-  const int64_t singles = layout_bytes(make_shape(dtype, d, n, b, false), n, d);
-  *bytes = pairs > singles ? pairs : singles;
+  // (the slabs go by the tensors' alignment)
+  *bytes = 0;
+  for (int align = 1; align <= 4; align *= 2)
+    *bytes = std::max(*bytes, layout_bytes(make_shape(dtype, d, n, b, align), n, d));
   return RG_OK;
 }
 
@@ -186,7 +197,7 @@ int rg_scan(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, const v
                           {"carries", carries, carries ? ceil_div(n, kScanBatch) * d * 4 : 0, 4, true}};
   status = check_ranges(ranges, 7);
   if (status) return status;
-  const bool pairs = pairs_aligned(ranges, 7);
+  const int align = aligned_elements(ranges, 7);
   ScanArgs p{};
   p.values = values;
   p.gates = gates;
@@ -198,7 +209,7 @@ int rg_scan(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, const v
   p.carries = carries;
   p.out = out;
   p.final_state = final_state;
-  return run_scan<false>(dtype, index_dtype, pairs, p, workspace, workspace_bytes, static_cast<cudaStream_t>(stream), report);
+  return run_scan<false>(dtype, index_dtype, align, p, workspace, workspace_bytes, static_cast<cudaStream_t>(stream), report);
 }
 
 int rg_scan_backward(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, const void *values,
@@ -226,7 +237,7 @@ int rg_scan_backward(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b
                           {"grad_initial", grad_initial, grad_initial ? states : 0, 4, true}};
   status = check_ranges(ranges, 10);
   if (status) return status;
-  const bool pairs = pairs_aligned(ranges, 10);
+  const int align = aligned_elements(ranges, 10);
   ScanArgs p{};
   p.values = values;
   p.gates = gates;
@@ -241,7 +252,7 @@ int rg_scan_backward(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b
   p.grad_values = grad_values;
   p.grad_gates = grad_gates;
   p.grad_initial = grad_initial;
-  return run_scan<true>(dtype, index_dtype, pairs, p, workspace, workspace_bytes, static_cast<cudaStream_t>(stream), report);
+  return run_scan<true>(dtype, index_dtype, align, p, workspace, workspace_bytes, static_cast<cudaStream_t>(stream), report);
 }
 
 }  // extern "C"

@@ -9,9 +9,10 @@
 // Both are first-order recurrences, one forward and one backward in t, whose
 // steps compose: rows r..s act on the state before them as H + A * state with
 // A the product of the gates.  Work is cut into slabs of rows by tiles of
-// columns, and every task belongs to one warp: 4 bytes of a row a lane (narrow
-// rows: several row groups side by side), down the rows in batches of 16.  No
-// block barrier, no exchange between lanes; warps hide each other's latency.
+// columns, and every task belongs to one warp: 8 or 4 bytes of a row a lane
+// (narrow rows: several row groups side by side), down the rows in batches of 8
+// or 16.  No block barrier, no exchange between lanes; warps hide each other's
+// latency.
 //
 //   fold   (A, H) of each slab.  Only the rows past its last segment start
 //          count, and none where its last row ends a segment.
@@ -50,7 +51,7 @@ namespace rgb {
 
 constexpr int kScanThreads = 256;
 constexpr int kScanWarps = kScanThreads / 32;
-constexpr int kScanBatch = 16;    // rows of a lane in flight; rows per recorded state
+constexpr int kScanBatch = 16;    // rows per recorded state
 constexpr int kJoinCols = 8;      // columns of a join's block
 constexpr int kJoinParts = 128;   // parts that it cuts the slabs into, a thread each
 constexpr int kJoinBatch = 8;     // pairs of a thread in flight
@@ -215,13 +216,19 @@ __device__ __forceinline__ void scan_mark(const OffT *__restrict__ offsets, int6
 // Words of shared memory of a warp's marks.
 __host__ __device__ constexpr int scan_marks_words(int rows) { return 2 * ((rows < 64 ? 64 : rows) / 32) + 2 * rows; }
 
-// 16 rows of a lane, `d` elements apart; of `count` rows (at least one), the
-// last stands in for those that are missing.
+// Rows of a lane in flight: 8 of 8 bytes or 16 of 4 (2) bytes of each input.
+template <typename T, int VEC>
+__host__ __device__ constexpr int scan_batch() {
+  return VEC * Elem<T>::kBytes == 8 ? 8 : 16;
+}
+
+// A batch of rows of a lane, `d` elements apart; of `count` rows (at least
+// one), the last stands in for those that are missing.
 template <typename T, int VEC>
 __device__ __forceinline__ void scan_rows(const T *__restrict__ at, int64_t d, int count,
-                                          typename VecIO<T, VEC>::Raw (&raw)[kScanBatch]) {
+                                          typename VecIO<T, VEC>::Raw (&raw)[scan_batch<T, VEC>()]) {
 #pragma unroll
-  for (int i = 0; i < kScanBatch; ++i) {
+  for (int i = 0; i < scan_batch<T, VEC>(); ++i) {
     raw[i] = VecIO<T, VEC>::load_raw(at);
     at += i + 1 < count ? d : 0;
   }
@@ -234,6 +241,7 @@ struct ScanWarp {
   using Raw = typename IO::Raw;
   using State = VecIO<float, VEC>;
   using Pair = ScanPair<VEC>;
+  static constexpr int BATCH = scan_batch<T, VEC>();
   const ScanArgs &p;
   const OffT *__restrict__ offsets;
   int lanes, rows, words, base;  // base: this lane's first row of a slab
@@ -275,7 +283,7 @@ struct ScanWarp {
     return (m.end_mask[last >> 5] >> (last & 31)) & 1;
   }
   __device__ __forceinline__ int row_count(int64_t row) const {  // rows of the batch at `row`
-    return static_cast<int>(min(max(p.n - row, int64_t{0}), int64_t{kScanBatch}));
+    return static_cast<int>(min(max(p.n - row, int64_t{0}), int64_t{BATCH}));
   }
   __device__ __forceinline__ void state_of(const float *states, int64_t seg, float (&x)[VEC]) const {
     if (states) {
@@ -289,7 +297,6 @@ struct ScanWarp {
   // Folds this lane's rows from the last segment start on (first end,
   // BACKWARD).  Returns whether there is one.
   __device__ __forceinline__ bool fold(Pair &f) const {
-    constexpr int BATCH = kScanBatch;
     f.clear();
     const uint64_t marks = lane_bits(BACKWARD ? m.end_mask : m.start_mask);
     if (!col_ok) return marks != 0;
@@ -306,7 +313,7 @@ struct ScanWarp {
       Raw ra[BATCH], rx[BATCH];
       scan_rows<T, VEC>(gates + row * p.d + col, p.d, count, ra);
       scan_rows<T, VEC>(second + row * p.d + col, p.d, count, rx);
-      const unsigned mark = static_cast<unsigned>(marks >> (batch * BATCH)) & 0xffffu;
+      const unsigned mark = static_cast<unsigned>(marks >> (batch * BATCH)) & ((1u << BATCH) - 1);
       const int *seg = (BACKWARD ? m.end_seg : m.start_seg) + base + batch * BATCH;
       const bool plain = mark == 0 && count == BATCH;
       auto step = [&](int i, bool alone) {
@@ -485,7 +492,7 @@ __global__ void __launch_bounds__(kJoinCols * kJoinParts) scan_join_kernel(const
 
 template <typename T, typename OffT, int VEC, bool BACKWARD>
 __global__ void __launch_bounds__(kScanThreads, BACKWARD ? 2 : 3) scan_walk_kernel(const ScanArgs p) {
-  constexpr int BATCH = kScanBatch;
+  constexpr int BATCH = scan_batch<T, VEC>();
   using IO = VecIO<T, VEC>;
   using Raw = typename IO::Raw;
   using State = VecIO<float, VEC>;
@@ -531,8 +538,8 @@ __global__ void __launch_bounds__(kScanThreads, BACKWARD ? 2 : 3) scan_walk_kern
         const int count = w.row_count(row);
         if (count <= 0 || !w.col_ok) continue;
         const int64_t at = row * p.d + w.col;
-        const unsigned start = static_cast<unsigned>(starts >> (batch * BATCH)) & 0xffffu;
-        const unsigned end = static_cast<unsigned>(ends >> (batch * BATCH)) & 0xffffu;
+        const unsigned start = static_cast<unsigned>(starts >> (batch * BATCH)) & ((1u << BATCH) - 1);
+        const unsigned end = static_cast<unsigned>(ends >> (batch * BATCH)) & ((1u << BATCH) - 1);
         const int *start_seg = w.m.start_seg + w.base + batch * BATCH;
         const int *end_seg = w.m.end_seg + w.base + batch * BATCH;
         const bool plain = (start | end) == 0 && count == BATCH;
@@ -548,7 +555,7 @@ __global__ void __launch_bounds__(kScanThreads, BACKWARD ? 2 : 3) scan_walk_kern
           for (int v = 0; v < VEC; ++v) s[v] = alone ? x[v] : fmaf(a[v], s[v], x[v]);
         };
         if constexpr (!BACKWARD) {
-          if (p.carries) State::store(p.carries + (row / BATCH) * p.d + w.col, h);
+          if (p.carries && row % kScanBatch == 0) State::store(p.carries + row / kScanBatch * p.d + w.col, h);
           T *to = static_cast<T *>(p.out) + at;
           if (plain) {
 #pragma unroll
@@ -584,7 +591,8 @@ __global__ void __launch_bounds__(kScanThreads, BACKWARD ? 2 : 3) scan_walk_kern
           Raw rg[BATCH];
           scan_rows<T, VEC>(grads + at, p.d, count, rg);
           float previous[BATCH][VEC], s[VEC];  // state before each row
-          State::load(p.carries + (row / BATCH) * p.d + w.col, s);
+          static_assert(!BACKWARD || BATCH == kScanBatch, "a batch starts at a recorded state");
+          State::load(p.carries + row / kScanBatch * p.d + w.col, s);
 #pragma unroll
           for (int i = 0; i < BATCH; ++i) {
             const bool is_first = (start >> i) & 1;
