@@ -279,8 +279,8 @@ int rg_run_noalloc(int op, int dtype, int index_dtype, int64_t d, int64_t n, int
  * always does).
  *
  * rg_scan_workspace_bytes gives the scratch of either call (256-byte aligned;
- * 0: none).  carries (f32 [ceil(N / 16), D]) receives
- * the state before every 16th row for rg_scan_backward, NULL if no backward pass
+ * 0: none).  carries (f32 [ceil(N / 8), D]) receives
+ * the state before every 8th row for rg_scan_backward, NULL if no backward pass
  * follows.  rg_scan_backward takes the forward call's inputs and carries and
  * the gradients of out and final_state (NULL: zero) and writes the gradients
  * that are not NULL; grad_initial (f32 [B, D]) needs `initial`.  Written

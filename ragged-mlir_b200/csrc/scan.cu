@@ -14,33 +14,28 @@ constexpr int64_t kMaxScanDim = 65536;
 
 
 struct ScanShape {
-  int vec, tiles;            // 4 bytes of a row a lane (one element where D is odd or a tensor is not aligned)
-  int wide_vec, wide_tiles;  // 8 bytes where they fill 32 lanes, else as vec
-  int shift, lane_rows, row_shift;
+  int vec, tiles, shift, lane_rows, row_shift;
   int64_t slabs, blocks;
 };
 
 constexpr int64_t kAloneRows = 256;  // rows up to which walk is the only launch
 
-// 32 lanes, or as many as cover a row, of one vector each.  8 bytes a lane take
-// two thirds of the instructions of 4 (B200, bf16 65536 x 1024: see the kernels);
-// a backward walk, which keeps 16 states of each column, has the registers for
-// 4.  A lane takes 64 rows of a slab, fewer where that would leave resident
-// warps without a task.  `align`: elements that all tensors are aligned for.
+// 32 lanes, or as many as cover a row, of one vector each: 8 bytes where they
+// fill the lanes, else 4 (one element where D is odd).  8 bytes take two thirds
+// of the instructions (f32 262k x 100: 127 -> 111 us).  A lane takes 64 rows of a
+// slab, fewer where that would leave resident warps without a task.  `align`:
+// elements that all tensors are aligned for.
 ScanShape make_shape(int dtype, int64_t d, int64_t n, int64_t b, int align) {
   ScanShape s;
-  s.vec = dtype == RG_DTYPE_BF16 && d % 2 == 0 && align >= 2 ? 2 : 1;
+  s.vec = 8 / elem_bytes(dtype);
+  while (s.vec > align || d % s.vec || (s.vec * elem_bytes(dtype) == 8 && d < 32 * s.vec)) s.vec /= 2;
   s.shift = 0;
   while ((int64_t{1} << s.shift) * s.vec < d && s.shift < 5) ++s.shift;
   s.tiles = static_cast<int>(ceil_div(d, (int64_t{1} << s.shift) * s.vec));
-  const int wide = 8 / elem_bytes(dtype);
-  s.wide_vec = d % wide == 0 && d >= 32 * wide && align >= wide ? wide : s.vec;
-  s.wide_tiles = static_cast<int>(ceil_div(d, (int64_t{1} << s.shift) * s.wide_vec));
   const int groups = 32 >> s.shift;
   constexpr int64_t warps = 148 * 24;
   s.lane_rows = 64;
-  while (s.lane_rows > 16 &&
-         (ceil_div(n, s.lane_rows * groups) * s.wide_tiles < warps || s.lane_rows * groups > 512))
+  while (s.lane_rows > 16 && (ceil_div(n, s.lane_rows * groups) * s.tiles < warps || s.lane_rows * groups > 512))
     s.lane_rows /= 2;
   s.row_shift = 0;
   while ((1 << s.row_shift) < s.lane_rows * groups) ++s.row_shift;
@@ -78,9 +73,8 @@ int aligned_elements(const TensorRange *r, int count) {
   return most;
 }
 
-// WIDE: of fold and of a forward walk.
-template <typename T, typename OffT, int WIDE, int VEC, bool BACKWARD>
-int launch(ScanArgs p, const ScanShape &s, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
+template <typename T, typename OffT, int VEC, bool BACKWARD>
+int launch(const ScanArgs &p, const ScanShape &s, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
   const int smem = kScanWarps * scan_marks_words(1 << s.row_shift) * 4;
   constexpr int usual = kScanWarps * scan_marks_words(64) * 4, limit = kScanWarps * scan_marks_words(512) * 4;
   // The second and third launch may start before the one before them ends.
@@ -98,35 +92,34 @@ int launch(ScanArgs p, const ScanShape &s, const DeviceProps &dev, cudaStream_t 
     record_launch(report, id, config.gridDim, threads, bytes);
     return check_cuda(cudaLaunchKernelEx(&config, kernel, p), "scan kernel launch");
   };
-  auto run = [&](void (*kernel)(ScanArgs), int id, int64_t slabs, int tiles, bool after) {
+  auto run = [&](void (*kernel)(ScanArgs), int id, int64_t slabs, bool after) {
     int per_sm = 0;
-    p.tiles = tiles;
     int status = prepare_kernel(reinterpret_cast<const void *>(kernel), dev.device, kScanThreads, usual, limit, &per_sm);
     if (status) return status;
-    return start(kernel, id, std::min(static_cast<int64_t>(per_sm) * dev.sm_count, ceil_div(slabs * tiles, kScanWarps)),
+    return start(kernel, id, std::min(static_cast<int64_t>(per_sm) * dev.sm_count, ceil_div(slabs * s.tiles, kScanWarps)),
                  kScanThreads, smem, after);
   };
   if (p.pairs) {
-    int status = run(scan_fold_kernel<T, OffT, WIDE, BACKWARD>, BACKWARD ? K_SCAN_FOLD_BACKWARD : K_SCAN_FOLD, s.slabs,
-                     s.wide_tiles, false);
+    int status = run(scan_fold_kernel<T, OffT, VEC, BACKWARD>, BACKWARD ? K_SCAN_FOLD_BACKWARD : K_SCAN_FOLD, s.slabs,
+                     false);
     if (status) return status;
     status = start(scan_join_kernel, K_SCAN_JOIN, ceil_div(p.d, kJoinCols), kJoinCols * kJoinParts, 0, true);
     if (status) return status;
   }
-  return run(scan_walk_kernel<T, OffT, BACKWARD ? VEC : WIDE, BACKWARD>, BACKWARD ? K_SCAN_BACKWARD : K_SCAN, s.blocks,
-             BACKWARD ? s.tiles : s.wide_tiles, p.pairs != nullptr);
+  return run(scan_walk_kernel<T, OffT, VEC, BACKWARD>, BACKWARD ? K_SCAN_BACKWARD : K_SCAN, s.blocks,
+             p.pairs != nullptr);
 }
 
 template <typename OffT, bool BACKWARD>
 int launch_vec(int dtype, const ScanArgs &p, const ScanShape &s, const DeviceProps &dev, cudaStream_t stream,
                rg_report *report) {
   if (dtype == RG_DTYPE_F32) {
-    if (s.wide_vec == 2) return launch<float, OffT, 2, 1, BACKWARD>(p, s, dev, stream, report);
-    return launch<float, OffT, 1, 1, BACKWARD>(p, s, dev, stream, report);
+    if (s.vec == 2) return launch<float, OffT, 2, BACKWARD>(p, s, dev, stream, report);
+    return launch<float, OffT, 1, BACKWARD>(p, s, dev, stream, report);
   }
-  if (s.wide_vec == 4) return launch<__nv_bfloat16, OffT, 4, 2, BACKWARD>(p, s, dev, stream, report);
-  if (s.vec == 2) return launch<__nv_bfloat16, OffT, 2, 2, BACKWARD>(p, s, dev, stream, report);
-  return launch<__nv_bfloat16, OffT, 1, 1, BACKWARD>(p, s, dev, stream, report);
+  if (s.vec == 4) return launch<__nv_bfloat16, OffT, 4, BACKWARD>(p, s, dev, stream, report);
+  if (s.vec == 2) return launch<__nv_bfloat16, OffT, 2, BACKWARD>(p, s, dev, stream, report);
+  return launch<__nv_bfloat16, OffT, 1, BACKWARD>(p, s, dev, stream, report);
 }
 
 template <bool BACKWARD>
@@ -140,12 +133,13 @@ int run_scan(int dtype, int index_dtype, int align, ScanArgs &p, void *workspace
   const int64_t need = layout_bytes(s, p.n, p.d);
   if (report) {
     report->workspace_bytes = need;
-    report->d_vector = BACKWARD ? s.vec : s.wide_vec;
+    report->d_vector = s.vec;
     report->d_tile = 1 << s.shift;
   }
   p.shift = s.shift;
   p.lane_rows = s.lane_rows;
   p.row_shift = s.row_shift;
+  p.tiles = s.tiles;
   p.slabs = s.slabs;
   p.blocks = s.blocks;
   p.per_block = ceil_div(p.b, s.blocks);

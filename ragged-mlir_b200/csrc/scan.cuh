@@ -10,8 +10,8 @@
 // steps compose: rows r..s act on the state before them as H + A * state with
 // A the product of the gates.  Work is cut into slabs of rows by tiles of
 // columns, and every task belongs to one warp: 8 or 4 bytes of a row a lane
-// (narrow rows: several row groups side by side), down the rows in batches of 8
-// or 16.  No block barrier, no exchange between lanes; warps hide each other's
+// (narrow rows: several row groups side by side), down the rows in batches of
+// 8.  No block barrier, no exchange between lanes; warps hide each other's
 // latency.
 //
 //   fold   (A, H) of each slab.  Only the rows past its last segment start
@@ -30,10 +30,12 @@
 // Up to 256 rows walk is the only launch: a lane whose rows go on from earlier
 // ones runs the recurrence over those itself.
 //
-// The backward pass needs the states again.  It recomputes 16 rows at a time
-// from values and gates, from the state before them that forward records in
-// f32 (4 bytes for 16 elements; reading `out` would cost as much as reading
-// values does): no rounded state enters a gradient.
+// The backward pass needs the states again.  It recomputes 8 rows at a time from
+// values and gates, from the state before them that forward records in f32 (4
+// bytes for 8 elements; reading `out` would cost as much as reading values
+// does): no rounded state enters a gradient.  16 rows at a time halve those
+// bytes, but their states leave registers for 4 bytes a lane and not 8: 219
+// instead of 184 us backward, 137 instead of 139 forward (bf16 65536 x 1024).
 //
 // States, products and sums are f32; results are rounded to the tensor's type
 // once, when they are written.  Segment starts cut the fold by a flag, never
@@ -51,7 +53,7 @@ namespace rgb {
 
 constexpr int kScanThreads = 256;
 constexpr int kScanWarps = kScanThreads / 32;
-constexpr int kScanBatch = 16;    // rows per recorded state
+constexpr int kScanBatch = 8;     // rows of a lane in flight; rows per recorded state
 constexpr int kJoinCols = 8;      // columns of a join's block
 constexpr int kJoinParts = 128;   // parts that it cuts the slabs into, a thread each
 constexpr int kJoinBatch = 8;     // pairs of a thread in flight
@@ -68,7 +70,7 @@ struct ScanArgs {
   int64_t slabs;       // slabs that hold rows
   int64_t blocks;      // slabs launched (more than `slabs` where many segments are empty)
   int64_t per_block;   // segments whose emptiness a slab looks at
-  float *carries;      // [N / 16, D] state before every 16th row (written by forward, read by backward)
+  float *carries;      // [N / 8, D] state before every 8th row (written by forward, read by backward)
   // forward
   void *out;
   float *final_state;  // [B, D] or null
@@ -216,19 +218,13 @@ __device__ __forceinline__ void scan_mark(const OffT *__restrict__ offsets, int6
 // Words of shared memory of a warp's marks.
 __host__ __device__ constexpr int scan_marks_words(int rows) { return 2 * ((rows < 64 ? 64 : rows) / 32) + 2 * rows; }
 
-// Rows of a lane in flight: 8 of 8 bytes or 16 of 4 (2) bytes of each input.
-template <typename T, int VEC>
-__host__ __device__ constexpr int scan_batch() {
-  return VEC * Elem<T>::kBytes == 8 ? 8 : 16;
-}
-
 // A batch of rows of a lane, `d` elements apart; of `count` rows (at least
 // one), the last stands in for those that are missing.
 template <typename T, int VEC>
 __device__ __forceinline__ void scan_rows(const T *__restrict__ at, int64_t d, int count,
-                                          typename VecIO<T, VEC>::Raw (&raw)[scan_batch<T, VEC>()]) {
+                                          typename VecIO<T, VEC>::Raw (&raw)[kScanBatch]) {
 #pragma unroll
-  for (int i = 0; i < scan_batch<T, VEC>(); ++i) {
+  for (int i = 0; i < kScanBatch; ++i) {
     raw[i] = VecIO<T, VEC>::load_raw(at);
     at += i + 1 < count ? d : 0;
   }
@@ -241,7 +237,7 @@ struct ScanWarp {
   using Raw = typename IO::Raw;
   using State = VecIO<float, VEC>;
   using Pair = ScanPair<VEC>;
-  static constexpr int BATCH = scan_batch<T, VEC>();
+  static constexpr int BATCH = kScanBatch;
   const ScanArgs &p;
   const OffT *__restrict__ offsets;
   int lanes, rows, words, base;  // base: this lane's first row of a slab
@@ -492,7 +488,7 @@ __global__ void __launch_bounds__(kJoinCols * kJoinParts) scan_join_kernel(const
 
 template <typename T, typename OffT, int VEC, bool BACKWARD>
 __global__ void __launch_bounds__(kScanThreads, BACKWARD ? 2 : 3) scan_walk_kernel(const ScanArgs p) {
-  constexpr int BATCH = scan_batch<T, VEC>();
+  constexpr int BATCH = kScanBatch;
   using IO = VecIO<T, VEC>;
   using Raw = typename IO::Raw;
   using State = VecIO<float, VEC>;
@@ -555,7 +551,7 @@ __global__ void __launch_bounds__(kScanThreads, BACKWARD ? 2 : 3) scan_walk_kern
           for (int v = 0; v < VEC; ++v) s[v] = alone ? x[v] : fmaf(a[v], s[v], x[v]);
         };
         if constexpr (!BACKWARD) {
-          if (p.carries && row % kScanBatch == 0) State::store(p.carries + row / kScanBatch * p.d + w.col, h);
+          if (p.carries) State::store(p.carries + row / BATCH * p.d + w.col, h);
           T *to = static_cast<T *>(p.out) + at;
           if (plain) {
 #pragma unroll
@@ -591,8 +587,7 @@ __global__ void __launch_bounds__(kScanThreads, BACKWARD ? 2 : 3) scan_walk_kern
           Raw rg[BATCH];
           scan_rows<T, VEC>(grads + at, p.d, count, rg);
           float previous[BATCH][VEC], s[VEC];  // state before each row
-          static_assert(!BACKWARD || BATCH == kScanBatch, "a batch starts at a recorded state");
-          State::load(p.carries + row / kScanBatch * p.d + w.col, s);
+          State::load(p.carries + row / BATCH * p.d + w.col, s);
 #pragma unroll
           for (int i = 0; i < BATCH; ++i) {
             const bool is_first = (start >> i) & 1;

@@ -25,7 +25,7 @@ from .runtime import CompiledProgram, _checked_devices, _torch
 from .validation import STATUS_BYTES
 
 
-CARRY_ROWS = 16  # rows per state that a scan records for its backward pass
+CARRY_ROWS = 8  # rows per state that a scan records for its backward pass
 
 
 class _LayerProgram:

@@ -114,7 +114,7 @@ def test_fake_shapes_and_refusals(monkeypatch):
     assert out.shape == (700, 24) and out.dtype == torch.bfloat16
     assert final.shape == (4, 24) and final.dtype == torch.float32
     ops = torch.ops.ragged_mlir
-    assert ops.segment_scan(values, values, offsets, None, "scan-24")[2].shape == (44, 24)
+    assert ops.segment_scan(values, values, offsets, None, "scan-24")[2].shape == (88, 24)
     assert ops.segment_scan(values, values, offsets, None, "scan-24", "validated", False)[2].shape == (0, 24)
     initial = torch.empty((4, 24), **meta)
     for bad in (dict(gates=values.float()), dict(gates=values[:5]), dict(initial=initial.bfloat16()),
