@@ -66,6 +66,7 @@ enum KernelId : int {
   K_MATMUL_SIMT = 19,
   K_MATMUL_TENSOR = 20,
   K_MATMUL_PACK = 21,
+  K_MATMUL_FEW = 22,
 };
 
 // Recording helper for rg_report.

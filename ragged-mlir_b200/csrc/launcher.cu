@@ -315,6 +315,7 @@ const char *rg_kernel_name(int kernel_id) {
     case K_MATMUL_SIMT: return "matmul_simt";
     case K_MATMUL_TENSOR: return "matmul_tensor";
     case K_MATMUL_PACK: return "matmul_pack";
+    case K_MATMUL_FEW: return "matmul_few";
   }
   return "";
 }

@@ -1,9 +1,10 @@
 // Launch code of the segmented matrix products (kernels: matmul_tensor.cuh for
-// bf16, matmul_simt.cuh for f32).
+// bf16, matmul_simt.cuh for f32, matmul_few.cuh for few rows a segment).
 #include <algorithm>
 #include <cstring>
 
 #include "internal.h"
+#include "matmul_few.cuh"
 #include "matmul_simt.cuh"
 #include "matmul_tensor.cuh"
 
@@ -26,6 +27,12 @@ int64_t status_bytes() { return 1024 * 8; }
 
 bool takes_tma(const void *p, int64_t cols) { return cols % 8 == 0 && aligned(p, 16); }
 
+// Whether a forward product goes row by row of the weights: up to four rows a
+// segment on average, and columns in whole 16-byte vectors.
+bool takes_few(int kind, int dtype, int64_t m, int64_t n, int64_t b, const void *right) {
+  return kind == MATMUL_FORWARD && n <= 4 * b && m % (16 / elem_bytes(dtype)) == 0 && aligned(right, 16);
+}
+
 MatmulShape make_shape(int kind, int dtype, int64_t k, int64_t m, int64_t n, int64_t b, const void *left,
                        const void *right) {
   MatmulShape s{};
@@ -38,7 +45,7 @@ MatmulShape make_shape(int kind, int dtype, int64_t k, int64_t m, int64_t n, int
   s.right_cols = m;
   s.left_pitch = s.left_cols;
   s.right_pitch = s.right_cols;
-  if (dtype == RG_DTYPE_F32) return s;
+  if (dtype == RG_DTYPE_F32 || takes_few(kind, dtype, m, n, b, right)) return s;
   s.bytes = status_bytes();
   if (!takes_tma(left, s.left_cols)) {
     s.pack_left = true;
@@ -171,9 +178,28 @@ int launch_tensor(const MatmulArgs &p, const DeviceProps &dev, cudaStream_t stre
   return launch_tensor_cols<OffT, KIND, 64>(p, dev, stream, report);
 }
 
+template <typename T, typename OffT>
+int launch_few(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
+  const auto kernel = matmul_few_kernel<T, OffT>;
+  constexpr int smem = kFewSmem;
+  int per_sm = 0;
+  const int status = prepare_kernel(reinterpret_cast<const void *>(kernel), dev.device, kFewThreads, smem, smem, &per_sm);
+  if (status) return status;
+  p.col_tiles = static_cast<int>(ceil_div(p.cols, few_cols<T>()));
+  const int64_t tiles = most_row_tiles(MATMUL_FORWARD, p, kFewRows) * p.col_tiles;
+  const dim3 grid(static_cast<unsigned>(std::min(tiles, static_cast<int64_t>(per_sm) * dev.sm_count)), 1, 1);
+  kernel<<<grid, kFewThreads, smem, stream>>>(p);
+  record_launch(report, K_MATMUL_FEW, grid, kFewThreads, smem);
+  return check_cuda(cudaGetLastError(), "matmul_few_kernel launch");
+}
+
 template <typename OffT>
 int launch_kind(int kind, int dtype, const MatmulArgs &p, const DeviceProps &dev, cudaStream_t stream,
                 rg_report *report) {
+  if (takes_few(kind, dtype, p.m, p.n, p.b, p.right)) {
+    if (dtype == RG_DTYPE_F32) return launch_few<float, OffT>(p, dev, stream, report);
+    return launch_few<__nv_bfloat16, OffT>(p, dev, stream, report);
+  }
   if (dtype == RG_DTYPE_F32) {
     if (kind == MATMUL_FORWARD) return launch_simt<OffT, MATMUL_FORWARD>(p, dev, stream, report);
     if (kind == MATMUL_GRAD_VALUES) return launch_simt<OffT, MATMUL_GRAD_VALUES>(p, dev, stream, report);

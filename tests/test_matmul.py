@@ -40,7 +40,7 @@ def test_abi_refuses_bad_arguments(native_library):
     lib = native_library
     one = ctypes.c_int64()
 
-    def sizes(kind=0, dtype=1, index=1, k=8, m=8, n=4, b=1, left=4096, right=4096):
+    def sizes(kind=0, dtype=1, index=1, k=8, m=8, n=64, b=1, left=4096, right=4096):
         return lib.rg_matmul_workspace_bytes(kind, dtype, index, k, m, n, b, left, right, ctypes.byref(one))
 
     assert sizes() == 0
