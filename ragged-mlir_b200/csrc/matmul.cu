@@ -160,7 +160,7 @@ int launch_tensor_cols(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream
   p.col_tiles = static_cast<int>(ceil_div(p.cols, COLS));
   p.row_tiles = static_cast<int>(ceil_div(p.k, kTensorRows));
   const int64_t tiles = most_row_tiles(KIND, p, kTensorRows) * p.col_tiles;
-  const dim3 grid(static_cast<unsigned>(std::min(tiles, static_cast<int64_t>(std::min(dev.sm_count, 1024)))), 1, 1);
+  const dim3 grid(static_cast<unsigned>(std::min(tiles, static_cast<int64_t>(std::min(dev.sm_count * tensor_ctas(COLS), 1024)))), 1, 1);
   kernel<<<grid, kTensorThreads, smem, stream>>>(p, maps);
   record_launch(report, K_MATMUL_TENSOR, grid, kTensorThreads, smem);
   return check_cuda(cudaGetLastError(), "matmul_tensor_kernel launch");

@@ -36,7 +36,9 @@ constexpr int kTensorDepth = 64;     // of a stage: 128 bytes of bf16
 constexpr int kLeftBytes = kTensorRows * 128;
 constexpr int kStoreBytes = 4 * 32 * 128;
 
-constexpr int tensor_stages(int cols) { return cols == 256 ? 4 : cols == 128 ? 6 : 8; }
+constexpr int tensor_stages(int cols) { return cols == 256 ? 4 : cols == 128 ? 6 : 3; }
+// Narrow tiles are small work each: two CTAs an SM overlap their starts and ends.
+constexpr int tensor_ctas(int cols) { return cols == 64 ? 2 : 1; }
 constexpr int tensor_smem_bytes(int cols) { return tensor_stages(cols) * (kLeftBytes + cols * 128) + kStoreBytes + 1024; }
 
 struct TensorMaps {
@@ -125,7 +127,7 @@ struct TensorGate {
 };
 
 template <typename OffT, int KIND, int COLS>
-__global__ void __launch_bounds__(kTensorThreads, 1)
+__global__ void __launch_bounds__(kTensorThreads, tensor_ctas(COLS))
 matmul_tensor_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps) {
   constexpr int STAGES = tensor_stages(COLS);
   constexpr int DEPTH = kTensorDepth, ROWS = kTensorRows;
