@@ -67,6 +67,7 @@ enum KernelId : int {
   K_MATMUL_TENSOR = 20,
   K_MATMUL_PACK = 21,
   K_MATMUL_FEW = 22,
+  K_MATMUL_PAIR = 23,
 };
 
 // Recording helper for rg_report.

@@ -5,6 +5,7 @@
 
 #include "internal.h"
 #include "matmul_few.cuh"
+#include "matmul_pair.cuh"
 #include "matmul_simt.cuh"
 #include "matmul_tensor.cuh"
 
@@ -115,25 +116,22 @@ int launch_simt(const MatmulArgs &p, const DeviceProps &dev, cudaStream_t stream
   return launch_simt_tile<OffT, KIND, 64, 1>(p, dev, stream, report);
 }
 
-template <typename OffT, int KIND, int COLS>
-int launch_tensor_cols(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
-  const auto kernel = matmul_tensor_kernel<OffT, KIND, COLS>;
-  const int smem = tensor_smem_bytes(COLS);
-  int per_sm = 0;
-  int status = prepare_kernel(reinterpret_cast<const void *>(kernel), dev.device, kTensorThreads, smem, smem, &per_sm);
-  if (status) return status;
-  TensorMaps maps;
+// Tensor maps of the operands: boxes of 128 rows of the left one (32 for the
+// last rows of a segment) and `right` columns of the right one.
+template <int KIND>
+int make_maps(TensorMaps &maps, const MatmulArgs &p, int right) {
+  int status = RG_OK;
   std::memset(&maps, 0, sizeof maps);
   constexpr bool weights = KIND == MATMUL_GRAD_WEIGHTS;
   const int64_t left_cols = KIND == MATMUL_GRAD_VALUES ? p.m : p.k;
   if (weights && left_cols % 64 == 0) {
     const int64_t dims[3] = {64, p.n, left_cols / 64}, strides[2] = {p.left_pitch, 64};
-    const int box[3] = {64, kTensorDepth, kTensorRows / 64};
+    const int box[3] = {64, kTensorDepth, 128 / 64};
     status = make_tensor_map(&maps.left, p.left, 3, dims, strides, box);
     maps.left_slabs = 1;
   } else {
     const int64_t dims[2] = {left_cols, p.n};
-    const int box[2] = {64, weights ? kTensorDepth : kTensorRows}, part[2] = {64, 32};
+    const int box[2] = {64, weights ? kTensorDepth : 128}, part[2] = {64, 32};
     status = make_tensor_map(&maps.left, p.left, 2, dims, &p.left_pitch, box);
     if (!status && !weights) status = make_tensor_map(&maps.left_part, p.left, 2, dims, &p.left_pitch, part);
   }
@@ -141,7 +139,7 @@ int launch_tensor_cols(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream
   maps.right_slabs = KIND != MATMUL_GRAD_VALUES && p.m % 64 == 0;
   if (weights && maps.right_slabs) {
     const int64_t dims[3] = {64, p.n, p.m / 64}, strides[2] = {p.right_pitch, 64};
-    const int box[3] = {64, kTensorDepth, COLS / 64};
+    const int box[3] = {64, kTensorDepth, right / 64};
     status = make_tensor_map(&maps.right, p.right, 3, dims, strides, box);
   } else if (weights) {
     const int64_t dims[2] = {p.m, p.n};
@@ -149,13 +147,25 @@ int launch_tensor_cols(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream
     status = make_tensor_map(&maps.right, p.right, 2, dims, &p.right_pitch, box);
   } else if (maps.right_slabs) {
     const int64_t dims[4] = {64, p.k, p.m / 64, p.b}, strides[3] = {p.right_pitch, 64, p.right_pitch * p.k};
-    const int box[4] = {64, kTensorDepth, COLS / 64, 1};
+    const int box[4] = {64, kTensorDepth, right / 64, 1};
     status = make_tensor_map(&maps.right, p.right, 4, dims, strides, box);
   } else {
     const int64_t dims[3] = {p.m, p.k, p.b}, strides[2] = {p.right_pitch, p.right_pitch * p.k};
-    const int box[3] = {64, KIND == MATMUL_FORWARD ? kTensorDepth : COLS, 1};
+    const int box[3] = {64, KIND == MATMUL_FORWARD ? kTensorDepth : right, 1};
     status = make_tensor_map(&maps.right, p.right, 3, dims, strides, box);
   }
+  if (status) return status;
+  return RG_OK;
+}
+
+template <typename OffT, int KIND, int COLS>
+int launch_tensor_cols(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
+  const auto kernel = matmul_tensor_kernel<OffT, KIND, COLS>;
+  const int smem = tensor_smem_bytes(COLS);
+  int per_sm = 0;
+  int status = prepare_kernel(reinterpret_cast<const void *>(kernel), dev.device, kTensorThreads, smem, smem, &per_sm);
+  TensorMaps maps;
+  if (!status) status = make_maps<KIND>(maps, p, COLS);
   if (status) return status;
   p.col_tiles = static_cast<int>(ceil_div(p.cols, COLS));
   p.row_tiles = static_cast<int>(ceil_div(p.k, kTensorRows));
@@ -166,11 +176,35 @@ int launch_tensor_cols(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream
   return check_cuda(cudaGetLastError(), "matmul_tensor_kernel launch");
 }
 
+template <typename OffT, int KIND>
+int launch_pair(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
+  const auto kernel = matmul_pair_kernel<OffT, KIND>;
+  int per_sm = 0;
+  int status =
+      prepare_kernel(reinterpret_cast<const void *>(kernel), dev.device, kTensorThreads, kPairSmem, kPairSmem, &per_sm);
+  TensorMaps maps;
+  if (!status) status = make_maps<KIND>(maps, p, kPairCols / 2);
+  if (status) return status;
+  p.col_tiles = static_cast<int>(ceil_div(p.cols, kPairCols));
+  p.row_tiles = static_cast<int>(ceil_div(p.k, kPairRows));
+  const int64_t tiles = most_row_tiles(KIND, p, kPairRows) * p.col_tiles;
+  const dim3 grid(static_cast<unsigned>(2 * std::min(tiles, static_cast<int64_t>(std::min(dev.sm_count, 1024) / 2))), 1, 1);
+  kernel<<<grid, kTensorThreads, kPairSmem, stream>>>(p, maps);
+  record_launch(report, K_MATMUL_PAIR, grid, kTensorThreads, kPairSmem);
+  return check_cuda(cudaGetLastError(), "matmul_pair_kernel launch");
+}
+
 // The widest tiles that give every SM one (a segment's last row tile counted half).
 template <typename OffT, int KIND>
 int launch_tensor(const MatmulArgs &p, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
   const int64_t row_tiles = KIND == MATMUL_GRAD_WEIGHTS ? p.b * ceil_div(p.k, kTensorRows)
                                                          : p.n / kTensorRows + std::max<int64_t>(std::min(p.n, p.b) / 2, 1);
+  // Pairs of SMs where 256 x 256 tiles keep all of them busy twice over and few
+  // of their rows are past a segment's end (segments of 768 rows on average).
+  const int64_t pair_rows = KIND == MATMUL_GRAD_WEIGHTS ? p.b * ceil_div(p.k, kPairRows) : p.n / kPairRows;
+  const bool full = KIND == MATMUL_GRAD_WEIGHTS ? p.k > 128 : p.n >= 768 * std::min(p.n, p.b);
+  if (p.cols > 128 && full && pair_rows * ceil_div(p.cols, kPairCols) >= dev.sm_count)
+    return launch_pair<OffT, KIND>(p, dev, stream, report);
   if (p.cols > 128 && row_tiles * ceil_div(p.cols, 256) >= dev.sm_count)
     return launch_tensor_cols<OffT, KIND, 256>(p, dev, stream, report);
   if (p.cols > 64 && row_tiles * ceil_div(p.cols, 128) >= dev.sm_count)

@@ -92,6 +92,15 @@ __device__ __forceinline__ void umma(uint32_t acc, uint64_t left, uint64_t right
       : "memory");
 }
 
+// Likewise on a pair of SMs (matmul_pair.cuh).
+__device__ __forceinline__ void umma_pair(uint32_t acc, uint64_t left, uint64_t right, uint32_t instruction, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(acc),
+      "l"(left), "l"(right), "r"(instruction), "r"(static_cast<uint32_t>(add))
+      : "memory");
+}
+
 // Arrives on `bar` when the products issued so far are done.
 __device__ __forceinline__ void umma_commit(uint64_t *bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar))
@@ -110,6 +119,52 @@ __device__ __forceinline__ void tmem_load_32(uint32_t at, uint32_t (&v)[32]) {
       : "r"(at));
 }
 
+// True in one lane of a converged warp, the same one each time.  Roles run their
+// inner loops in that lane alone: products that the compiler knows to come from
+// one thread are issued back to back, a branch on the lane's number costs a
+// hundred clocks around each.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+
+// Place in the ring of stages.
+template <int STAGES>
+struct RingPlace {
+  int stage;
+  uint32_t phase;
+  __device__ __forceinline__ void next() {
+    if (++stage == STAGES) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+  __device__ __forceinline__ void skip(uint32_t count) {
+    const uint32_t at = stage + count;
+    phase ^= at / STAGES & 1;
+    stage = static_cast<int>(at % STAGES);
+  }
+};
+
+// The products of a stage, `steps` times 16 of the contraction: 32 bytes along a
+// K-major row, 16 rows of an MN-major slab.
+template <bool PAIR, bool LEFT_MN, bool RIGHT_MN>
+__device__ __forceinline__ void umma_stage(uint32_t to, uint32_t left, uint32_t right, uint32_t slab,
+                                           uint32_t instruction, bool add, int steps) {
+  const uint64_t a = umma_operand(left, LEFT_MN ? slab : 16), b = umma_operand(right, RIGHT_MN ? slab : 16);
+#pragma unroll
+  for (int i = 0; i < kTensorDepth / 16; ++i) {
+    if (i < steps) {
+      const uint64_t ai = a + i * (LEFT_MN ? 2048 >> 4 : 32 >> 4), bi = b + i * (RIGHT_MN ? 2048 >> 4 : 32 >> 4);
+      if constexpr (PAIR)
+        umma_pair(to, ai, bi, instruction, add || i > 0);
+      else
+        umma(to, ai, bi, instruction, add || i > 0);
+    }
+  }
+}
+
 // Bounded wait by a role; on giving up marks the CTA so that all roles leave.
 // `status` is the CTA's own word.
 struct TensorGate {
@@ -123,6 +178,78 @@ struct TensorGate {
     *abandoned = 1;
     *status = 1;
     return false;
+  }
+};
+
+// Empties a warp's 32 rows (`quarter`: of the accumulator's 128, those this warp
+// can read) of a tile of COLS columns: rounds to bf16, turns 32 x 64 blocks
+// through shared memory, stores whole 128-byte lines.
+template <int KIND, int COLS>
+struct TensorStore {
+  const MatmulArgs &p;
+  unsigned char *turn;
+  int quarter;
+  __nv_bfloat16 *out;
+  bool whole;  // rows start at 16-byte boundaries
+  __device__ __forceinline__ TensorStore(const MatmulArgs &args, unsigned char *smem, int q)
+      : p(args), turn(smem + q * 32 * 128), quarter(q), out(static_cast<__nv_bfloat16 *>(args.out)) {
+    whole = p.out_pitch % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  }
+  // The accumulator's rows are the output's from `first` on, up to the tile's end.
+  __device__ __forceinline__ void tile(const MatmulTile &t, int64_t first, bool nothing, uint32_t acc) const {
+    const int lane = threadIdx.x & 31;
+    const int64_t row0 = first + quarter * 32;
+    const int rows = static_cast<int>(min(max(t.row_end - row0, int64_t{0}), int64_t{32}));
+    __nv_bfloat16 *to = out + (KIND == MATMUL_GRAD_WEIGHTS ? t.seg * p.rows + row0 : row0) * p.out_pitch;
+#pragma unroll 1
+    for (int c = 0; c < COLS; c += 64) {
+      const int64_t col0 = static_cast<int64_t>(t.col_tile) * COLS + c;
+      if (col0 >= p.cols) break;
+      uint32_t v[2][32];
+      if (nothing) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[0][i] = v[1][i] = 0;
+      } else {
+        const uint32_t at = acc + c + (static_cast<uint32_t>(quarter * 32) << 16);
+        tmem_load_32(at, v[0]);
+        tmem_load_32(at + 32, v[1]);
+        asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+      }
+      // Row `lane`, 8 pieces of 16 bytes, permuted so that neither this nor
+      // the reading across rows meets a bank twice.
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t *x = &v[i / 4][i % 4 * 8];
+        uint4 piece;
+        piece.x = pack_bf16x2(__uint_as_float(x[0]), __uint_as_float(x[1]));
+        piece.y = pack_bf16x2(__uint_as_float(x[2]), __uint_as_float(x[3]));
+        piece.z = pack_bf16x2(__uint_as_float(x[4]), __uint_as_float(x[5]));
+        piece.w = pack_bf16x2(__uint_as_float(x[6]), __uint_as_float(x[7]));
+        *reinterpret_cast<uint4 *>(turn + lane * 128 + ((i ^ (lane & 7)) * 16)) = piece;
+      }
+      __syncwarp();
+      if (whole) {
+        const int piece = lane & 7;
+        const bool col_ok = col0 + piece * 8 < p.cols;  // widths are multiples of 8 here
+#pragma unroll
+        for (int r = 0; r < 32; r += 4) {
+          const int row = r + lane / 8;
+          const uint4 x = *reinterpret_cast<const uint4 *>(turn + row * 128 + ((piece ^ (row & 7)) * 16));
+          if (row < rows && col_ok) *reinterpret_cast<uint4 *>(to + row * p.out_pitch + col0 + piece * 8) = x;
+        }
+      } else {
+        for (int row = 0; row < rows; ++row) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int col = half * 32 + lane;
+            const __nv_bfloat16 x = *reinterpret_cast<const __nv_bfloat16 *>(
+                turn + row * 128 + (((col / 8) ^ (row & 7)) * 16) + col % 8 * 2);
+            if (col0 + col < p.cols) to[row * p.out_pitch + col0 + col] = x;
+          }
+        }
+      }
+      __syncwarp();
+    }
   }
 };
 
@@ -167,6 +294,7 @@ matmul_tensor_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps
   asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
   const uint32_t tmem = tmem_base;
   const TensorGate gate{&abandoned, p.status + blockIdx.x};
+  auto abandoned_now = [&]() { return *gate.abandoned != 0; };
 
   MatmulWalk<OffT, KIND, ROWS> walk(p.offsets, p.b);
   MatmulTile t;
@@ -177,21 +305,21 @@ matmul_tensor_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps
 
   if (warp == 0) {
     // ------------------------------------------------------------ copies --
-    int stage = 0;
-    uint32_t phase = 1;
+    RingPlace<STAGES> at{0, 1};
     bool going = true;
     for (int64_t index = blockIdx.x; going && walk.find(p, index, t); index += gridDim.x) {
-      const int64_t count = slices(t);
+      const int count = static_cast<int>(slices(t));
       const int col0 = t.col_tile * COLS;
       const int boxes = LEFT_MN ? 2 : static_cast<int>((t.row_end - t.row + 31) / 32);
       const uint32_t bytes = (LEFT_MN ? kLeftBytes : boxes * 32 * 128) + kRight;
-      for (int64_t k = 0; k < count; ++k) {
-        going = gate.wait(&empty[stage], phase);
-        if (!going) break;
-        if (lane == 0) {
+      if (elect_lane()) {
+        RingPlace<STAGES> here = at;
+        for (int k = 0; k < count; ++k, here.next()) {
+          const int stage = here.stage;
+          if (!gate.wait(&empty[stage], here.phase)) break;
           unsigned char *left = smem + stage * kStage, *right = left + kLeftBytes;
           mbar_expect_tx(&full[stage], bytes);
-          const int d0 = static_cast<int>(k * DEPTH);
+          const int d0 = k * DEPTH;
           if constexpr (LEFT_MN) {
             const int row = static_cast<int>(t.begin) + d0;
             if (maps.left_slabs) {
@@ -225,12 +353,10 @@ matmul_tensor_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps
             }
           }
         }
-        __syncwarp();
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1;
-        }
       }
+      __syncwarp();
+      at.skip(static_cast<uint32_t>(count));
+      going = !abandoned_now();
     }
     // Given up: copies in flight write this CTA's shared memory, so they get
     // a millisecond to end before it does.
@@ -239,65 +365,66 @@ matmul_tensor_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps
   } else if (warp == 1) {
     // ---------------------------------------------------------- products --
     const uint32_t instruction = umma_instruction(ROWS, COLS, LEFT_MN, RIGHT_MN);
-    int stage = 0, acc = 0;
-    uint32_t phase = 0, acc_phase = 1;
+    RingPlace<STAGES> at{0, 0};
+    int acc = 0;
+    uint32_t acc_phase = 1;
     bool going = true;
     for (int64_t index = blockIdx.x; going && walk.find(p, index, t); index += gridDim.x) {
-      const int64_t count = slices(t);
+      const int count = static_cast<int>(slices(t));
       if (count == 0) continue;  // (weights kind: the stores write zeros)
-      going = gate.wait(&drained[acc], acc_phase);
-      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+      // Slices that are whole; in the weights kind the last one may not be.
+      const int whole = KIND == MATMUL_GRAD_WEIGHTS ? static_cast<int>((t.end - t.begin) / DEPTH) : count;
       const uint32_t to = tmem + acc * COLS;
-      for (int64_t k = 0; going && k < count; ++k) {
-        going = gate.wait(&full[stage], phase);
-        if (!going) break;
+      if (elect_lane()) {
+        bool there = gate.wait(&drained[acc], acc_phase);
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        unsigned char *left = smem + stage * kStage, *right = left + kLeftBytes;
-        int steps = DEPTH / 16;
-        if constexpr (KIND == MATMUL_GRAD_WEIGHTS) {
-          const int64_t there = t.end - t.begin - k * DEPTH;
-          if (there < DEPTH) {
-            steps = static_cast<int>(there + 15) / 16;
-            const int from = static_cast<int>(there), rows = steps * 16 - from;
-            for (int i = lane; i < rows * 8 * (2 + COLS / 64); i += 32) {
-              const int slab = i / (rows * 8), row = from + i / 8 % rows;
-              *reinterpret_cast<uint4 *>((slab < 2 ? left + slab * kSlab : right + (slab - 2) * kSlab) + row * 128 +
-                                         i % 8 * 16) = uint4{0, 0, 0, 0};
-            }
-            fence_proxy_async_shared();
-            __syncwarp();
-          }
+        RingPlace<STAGES> here = at;
+        for (int k = 0; there && k < whole; ++k, here.next()) {
+          there = gate.wait(&full[here.stage], here.phase);
+          if (!there) break;
+          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+          const uint32_t left = smem_u32(smem + here.stage * kStage);
+          umma_stage<false, LEFT_MN, RIGHT_MN>(to, left, left + kLeftBytes, kSlab, instruction, k > 0, DEPTH / 16);
+          umma_commit(&empty[here.stage]);
         }
-        if (lane == 0) {
-          const uint64_t a = umma_operand(smem_u32(left), LEFT_MN ? kSlab : 16);
-          const uint64_t b = umma_operand(smem_u32(right), RIGHT_MN ? kSlab : 16);
-          // 16 of the contraction: 32 bytes along a K-major row, 16 rows of an MN-major slab.
-          for (int i = 0; i < steps; ++i)
-            umma(to, a + i * (LEFT_MN ? 2048 >> 4 : 32 >> 4), b + i * (RIGHT_MN ? 2048 >> 4 : 32 >> 4), instruction,
-                 k > 0 || i > 0);
-          umma_commit(&empty[stage]);
-          if (k + 1 == count) umma_commit(&ready[acc]);
+        if (there && whole == count) umma_commit(&ready[acc]);
+      }
+      __syncwarp();
+      at.skip(static_cast<uint32_t>(whole));
+      going = !abandoned_now();
+      if (KIND == MATMUL_GRAD_WEIGHTS && going && whole < count) {
+        going = gate.wait(&full[at.stage], at.phase);
+        if (!going) break;
+        unsigned char *left = smem + at.stage * kStage, *right = left + kLeftBytes;
+        const int from = static_cast<int>(t.end - t.begin - int64_t{whole} * DEPTH), steps = (from + 15) / 16;
+        const int rows = steps * 16 - from;
+        for (int i = lane; i < rows * 8 * (2 + COLS / 64); i += 32) {
+          const int slab = i / (rows * 8), row = from + i / 8 % rows;
+          *reinterpret_cast<uint4 *>((slab < 2 ? left + slab * kSlab : right + (slab - 2) * kSlab) + row * 128 +
+                                     i % 8 * 16) = uint4{0, 0, 0, 0};
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (elect_lane()) {
+          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+          umma_stage<false, LEFT_MN, RIGHT_MN>(to, smem_u32(left), smem_u32(right), kSlab, instruction, whole > 0, steps);
+          umma_commit(&empty[at.stage]);
+          umma_commit(&ready[acc]);
         }
         __syncwarp();
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1;
-        }
+        at.next();
       }
       acc ^= 1;
       if (acc == 0) acc_phase ^= 1;
     }
     if (!going) {  // given up: the products in flight end before tensor memory is freed
-      if (lane == 0) umma_commit(&settled);
+      if (elect_lane()) umma_commit(&settled);
       __syncwarp();
       mbar_wait(&settled, 0);
     }
   } else {
     // ------------------------------------------------------------ stores --
-    const int quarter = warp & 3;  // of the accumulator's 128 rows: those this warp can read
-    unsigned char *turn = store_smem + quarter * 32 * 128;
-    __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out);
-    const bool whole = p.out_pitch % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+    TensorStore<KIND, COLS> store(p, store_smem, warp & 3);
     int acc = 0;
     uint32_t acc_phase = 0;
     bool going = true;
@@ -308,58 +435,7 @@ matmul_tensor_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps
         if (!going) break;
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
       }
-      const int64_t row0 = t.row + quarter * 32;
-      const int rows = static_cast<int>(min(max(t.row_end - row0, int64_t{0}), int64_t{32}));
-      __nv_bfloat16 *to = out + (KIND == MATMUL_GRAD_WEIGHTS ? t.seg * p.rows + row0 : row0) * p.out_pitch;
-#pragma unroll 1
-      for (int c = 0; c < COLS; c += 64) {
-        const int64_t col0 = static_cast<int64_t>(t.col_tile) * COLS + c;
-        if (col0 >= p.cols) break;
-        uint32_t v[2][32];
-        if (nothing) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[0][i] = v[1][i] = 0;
-        } else {
-          const uint32_t at = tmem + acc * COLS + c + (static_cast<uint32_t>(quarter * 32) << 16);
-          tmem_load_32(at, v[0]);
-          tmem_load_32(at + 32, v[1]);
-          asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
-        }
-        // Row `lane`, 8 pieces of 16 bytes, permuted so that neither this nor
-        // the reading across rows meets a bank twice.
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t *x = &v[i / 4][i % 4 * 8];
-          uint4 piece;
-          piece.x = pack_bf16x2(__uint_as_float(x[0]), __uint_as_float(x[1]));
-          piece.y = pack_bf16x2(__uint_as_float(x[2]), __uint_as_float(x[3]));
-          piece.z = pack_bf16x2(__uint_as_float(x[4]), __uint_as_float(x[5]));
-          piece.w = pack_bf16x2(__uint_as_float(x[6]), __uint_as_float(x[7]));
-          *reinterpret_cast<uint4 *>(turn + lane * 128 + ((i ^ (lane & 7)) * 16)) = piece;
-        }
-        __syncwarp();
-        if (whole) {
-          const int piece = lane & 7;
-          const bool col_ok = col0 + piece * 8 < p.cols;  // widths are multiples of 8 here
-#pragma unroll
-          for (int r = 0; r < 32; r += 4) {
-            const int row = r + lane / 8;
-            const uint4 x = *reinterpret_cast<const uint4 *>(turn + row * 128 + ((piece ^ (row & 7)) * 16));
-            if (row < rows && col_ok) *reinterpret_cast<uint4 *>(to + row * p.out_pitch + col0 + piece * 8) = x;
-          }
-        } else {
-          for (int row = 0; row < rows; ++row) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const int col = half * 32 + lane;
-              const __nv_bfloat16 x = *reinterpret_cast<const __nv_bfloat16 *>(
-                  turn + row * 128 + (((col / 8) ^ (row & 7)) * 16) + col % 8 * 2);
-              if (col0 + col < p.cols) to[row * p.out_pitch + col0 + col] = x;
-            }
-          }
-        }
-        __syncwarp();
-      }
+      store.tile(t, t.row, nothing, tmem + acc * COLS);
       if (!nothing) {
         asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
         if (lane == 0) mbar_arrive(&drained[acc]);

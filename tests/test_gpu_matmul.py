@@ -94,18 +94,25 @@ def test_widths(cuda, dtype, k, m):
     check(case, run(cuda, case, dtype, "i32"), dtype)
 
 
-@pytest.mark.parametrize("k,m,n,b", [(512, 2048, 9000, 8), (2048, 512, 9000, 8), (1024, 1024, 20_000, 40)])
-def test_wide_tiles(cuda, k, m, n, b):
-    """Enough tiles for the widest ones, several a CTA; sampled rows."""
+@pytest.mark.parametrize("k,m,lengths", [
+    (512, 2048, "routed 9000 8"), (2048, 512, "routed 9000 8"), (1024, 1024, "routed 20000 40"),
+    (520, 1544, "routed 9100 8"), (1544, 520, "routed 9100 8"), (777, 1290, "routed 6500 4"),
+    (1024, 1536, [0, 1, 129, 255, 257, 4000, 5000, 0, 300, 3000, 0]), (1536, 1024, [128, 6000, 0, 31, 256, 4097]),
+    (136, 4160, [5000, 16, 15, 17, 48, 0, 2500])])
+def test_wide_tiles(cuda, k, m, lengths):
+    """Enough tiles for the widest ones and for pairs of SMs, several a CTA."""
+    if isinstance(lengths, str):
+        n, b = map(int, lengths.split()[1:])
+        lengths = np.random.default_rng(n).multinomial(n, np.random.default_rng(b).dirichlet(np.full(b, 4.0)))
+    lengths = np.asarray(lengths)
+    n, b = int(lengths.sum()), len(lengths)
     torch = cuda
-    rng = np.random.default_rng(n)
-    lengths = rng.multinomial(n, rng.dirichlet(np.full(b, 4.0)))
     generator = torch.Generator(device="cuda").manual_seed(1)
     rand = lambda *s: torch.randn(s, generator=generator, device="cuda").bfloat16()  # noqa: E731
     values, weights, grad = rand(n, k), rand(b, k, m) / k ** 0.5, rand(n, m)
     offsets = torch.from_numpy(offsets_of(lengths)).to("cuda")
     program = matmul_program("bf16", k, m)
-    out, gv, gw = torch.empty_like(grad), torch.empty_like(values), torch.empty_like(weights)
+    out, gv, gw = (torch.full_like(x, SENTINEL) for x in (grad, values, weights))
     program.run(values, weights, offsets, out)
     program.run_backward(values, weights, offsets, grad, grad_values=gv, grad_weights=gw)
     bounds = offsets.tolist()
