@@ -286,6 +286,13 @@ class CompiledScan(_LayerProgram):
                 ("grad_initial", grad_initial, (b, d), torch.float32)]
         tensors = rows[:4] + [row for row in rows[4:] if row[1] is not None]
         self._tensors(torch, tensors, offsets, "validated", False)
+        return self._gradients(torch, values, gates, offsets, carries, grad_out, stream, initial, grad_final,
+                               grad_values, grad_gates, grad_initial)
+
+    def _gradients(self, torch, values, gates, offsets, carries, grad_out, stream, initial, grad_final, grad_values,
+                   grad_gates, grad_initial):
+        """``run_backward`` of tensors that are known to fit."""
+        spec, d, n, b = self.spec, self.spec.feature_dim, values.shape[0], offsets.numel() - 1
         pointers = (values.data_ptr(), gates.data_ptr(), offsets.data_ptr(), _address(initial), carries.data_ptr(),
                     grad_out.data_ptr(), _address(grad_final), _address(grad_values), _address(grad_gates),
                     _address(grad_initial))
@@ -293,7 +300,9 @@ class CompiledScan(_LayerProgram):
         def call(scratch, nbytes, on, report):
             _native.scan_backward(spec.dtype, spec.offsets_dtype, d, n, b, pointers, scratch, nbytes, on, report)
 
-        return self._launch(torch, offsets, n, b, stream, "validated", [t[1] for t in tensors] + [offsets],
+        used = [t for t in (values, gates, offsets, carries, grad_out, initial, grad_final, grad_values, grad_gates,
+                            grad_initial) if t is not None] if stream is not None else ()
+        return self._launch(torch, offsets, n, b, stream, "validated", used,
                             (((True, n, b) + _alignment(pointers), self._scratch(n, b), call),))
 
 
@@ -347,9 +356,15 @@ class CompiledMatmul(_LayerProgram):
         if grad_weights is not None:
             tensors.append(("grad_weights", grad_weights, (b, k, m), dtype))
         self._tensors(torch, tensors, offsets, "validated", False)
+        return self._gradients(torch, values, weights, offsets, grad_out, stream, grad_values, grad_weights)
+
+    def _gradients(self, torch, values, weights, offsets, grad_out, stream, grad_values, grad_weights):
+        """``run_backward`` of tensors that are known to fit."""
+        n, b = values.shape[0], offsets.numel() - 1
         work = []
         if grad_values is not None:
             work.append(self._product("grad_values", grad_out, weights, offsets, grad_values, n, b))
         if grad_weights is not None:
             work.append(self._product("grad_weights", values, grad_out, offsets, grad_weights, n, b))
-        return self._launch(torch, offsets, n, b, stream, "validated", [t[1] for t in tensors] + [offsets], work)
+        used = [t for t in (values, weights, offsets, grad_out, grad_values, grad_weights) if t is not None]
+        return self._launch(torch, offsets, n, b, stream, "validated", used, work)

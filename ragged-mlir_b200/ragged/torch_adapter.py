@@ -188,7 +188,7 @@ def _call(values, offsets, token: str, op: str, mode: str, mask=None):
 def _dense(*tensors):
     """The tensors, contiguous: a gradient arrives in whatever layout autograd
     made of it (an expanded sum, a transposed view)."""
-    return tuple(t.contiguous() if t is not None else None for t in tensors)
+    return [t if t is None or t.is_contiguous() else t.contiguous() for t in tensors]
 
 
 def _scan_shapes(values, offsets, record: bool) -> tuple:
@@ -208,15 +208,20 @@ def _scan_call(values, gates, offsets, initial, program, mode: str, record: bool
     return out, final, carries
 
 
-def _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final, program):
-    """The gradients of values, gates and initial, on the GPU."""
+def _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final, program, known=False):
+    """The gradients of values, gates and initial, on the GPU.  ``known``: the
+    tensors are those of a forward call and the gradients autograd made of its
+    outputs, so that they fit."""
     torch = _torch()
     values, gates, initial, grad_out, grad_final = _dense(values, gates, initial, grad_out, grad_final)
     grad_values, grad_gates = torch.empty_like(values), torch.empty_like(values)
-    grad_initial = torch.empty_like(initial) if initial is not None else carries.new_empty((0,))
-    program.run_backward(values, gates, offsets, carries, grad_out, initial=initial, grad_final=grad_final,
-                         grad_values=grad_values, grad_gates=grad_gates,
-                         grad_initial=grad_initial if initial is not None else None)
+    grad_initial = torch.empty_like(initial) if initial is not None else None
+    if known:
+        program._gradients(torch, values, gates, offsets, carries, grad_out, None, initial, grad_final, grad_values,
+                           grad_gates, grad_initial)
+    else:
+        program.run_backward(values, gates, offsets, carries, grad_out, initial=initial, grad_final=grad_final,
+                             grad_values=grad_values, grad_gates=grad_gates, grad_initial=grad_initial)
     return grad_values, grad_gates, grad_initial
 
 
@@ -230,8 +235,9 @@ def _register_scan(torch, library, contract) -> None:
         return _scan_call(values, gates, offsets, initial, _table.lookup(program, "scan"), mode, record)
 
     def scan_backward_kernel(values, gates, offsets, initial, carries, grad_out, grad_final, program):
-        return _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final,
-                                   _table.lookup(program, "scan"))
+        grads = _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final,
+                                    _table.lookup(program, "scan"))
+        return grads if initial is not None else (*grads[:2], carries.new_empty((0,)))
 
     for key in ("CPU", "CUDA"):
         library.impl("segment_scan", scan_kernel, key)
@@ -279,17 +285,21 @@ def _register_scan(torch, library, contract) -> None:
 def _matmul_call(values, weights, offsets, program, mode: str):
     """The output of segment_matmul, on the GPU."""
     values, weights = _dense(values, weights)
-    out = values.new_empty((values.shape[0], program.spec.out_dim))
+    out = _torch().empty((values.shape[0], program.spec.out_dim), dtype=values.dtype, device=values.device)
     program._run(values, weights, offsets, out, None, mode, False)
     return out
 
 
-def _matmul_backward_call(values, weights, offsets, grad_out, program, wanted):
-    """The gradients of values and weights (None: not wanted), on the GPU."""
+def _matmul_backward_call(values, weights, offsets, grad_out, program, wanted, known=False):
+    """The gradients of values and weights (None: not wanted), on the GPU;
+    ``known`` as for the scan."""
     torch = _torch()
     values, weights, grad_out = _dense(values, weights, grad_out)
     grads = [torch.empty_like(t) if want else None for t, want in zip((values, weights), wanted)]
-    program.run_backward(values, weights, offsets, grad_out, grad_values=grads[0], grad_weights=grads[1])
+    if known:
+        program._gradients(torch, values, weights, offsets, grad_out, None, *grads)
+    else:
+        program.run_backward(values, weights, offsets, grad_out, grad_values=grads[0], grad_weights=grads[1])
     return grads
 
 
@@ -328,8 +338,8 @@ def _autograd_functions(torch) -> dict[str, Any]:
             values, gates, offsets, carries, initial = ctx.saved_tensors
             if grad_out is None:
                 grad_out = torch.zeros_like(values)
-            grads = _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final, ctx.program)
-            return grads[0], grads[1], None, grads[2] if initial is not None else None, None, None
+            grads = _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final, ctx.program, True)
+            return grads[0], grads[1], None, grads[2], None, None
 
     class Matmul(torch.autograd.Function):
         @staticmethod
@@ -346,7 +356,7 @@ def _autograd_functions(torch) -> dict[str, Any]:
             if grad_out is None or not any(wanted):
                 return (None,) * 5
             values, weights, offsets = ctx.saved_tensors
-            return (*_matmul_backward_call(values, weights, offsets, grad_out, ctx.program, wanted), None, None, None)
+            return (*_matmul_backward_call(values, weights, offsets, grad_out, ctx.program, wanted, True), None, None, None)
 
     _functions.update(scan=Scan, matmul=Matmul)
     return _functions
