@@ -311,8 +311,10 @@ int rg_scan_backward(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b
  *
  * rg_matmul_workspace_bytes: scratch of a call (256-byte aligned; 0: none),
  * for tensors at these addresses: bf16 rows that do not start at 16-byte
- * boundaries are copied to some that do.  Where rg_report.status_offset is not
- * -1, a word for each CTA of the last launch is there (nonzero: a wait gave up). */
+ * boundaries are copied to some that do, and the gradients of few small weights
+ * of long segments are summed in parts.  Where rg_report.status_offset is not
+ * -1, a word for each CTA of the tensor-core launch is there (nonzero: a wait
+ * gave up). */
 enum rg_matmul_kind { RG_MATMUL_FORWARD = 0, RG_MATMUL_GRAD_VALUES = 1, RG_MATMUL_GRAD_WEIGHTS = 2 };
 int rg_matmul_workspace_bytes(int kind, int dtype, int index_dtype, int64_t k, int64_t m, int64_t n, int64_t b,
                               const void *left, const void *right, int64_t *bytes);

@@ -68,6 +68,7 @@ enum KernelId : int {
   K_MATMUL_PACK = 21,
   K_MATMUL_FEW = 22,
   K_MATMUL_PAIR = 23,
+  K_MATMUL_PARTS = 24,
 };
 
 // Recording helper for rg_report.

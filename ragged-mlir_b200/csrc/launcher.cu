@@ -317,6 +317,7 @@ const char *rg_kernel_name(int kernel_id) {
     case K_MATMUL_PACK: return "matmul_pack";
     case K_MATMUL_FEW: return "matmul_few";
     case K_MATMUL_PAIR: return "matmul_pair";
+    case K_MATMUL_PARTS: return "matmul_parts";
   }
   return "";
 }

@@ -21,17 +21,30 @@ struct MatmulShape {
   int64_t right_rows, right_cols;
   int64_t left_pitch, right_pitch;   // after packing
   bool pack_left, pack_right;
-  int64_t left_at, right_at, bytes;  // workspace
+  int splits;                        // of the segments' rows, in the weights kind
+  int64_t left_at, right_at, parts_at, bytes;  // workspace
 };
+
+// Columns of a tensor-core tile of the weights kind and tiles of 64 x 64 of the
+// f32 kernel decide how many tiles there are: with fewer than the SMs, each
+// segment's rows are split so that there are two a SM, into parts of 256 rows
+// at least.
+int splits_of(int kind, int dtype, int64_t k, int64_t m, int64_t n, int64_t b) {
+  if (kind != MATMUL_GRAD_WEIGHTS || b == 0) return 1;
+  const int64_t tiles = dtype == RG_DTYPE_F32 ? b * ceil_div(k, 64) * ceil_div(m, 64) : b * ceil_div(k, 128) * ceil_div(m, 64);
+  if (tiles >= 148) return 1;
+  return static_cast<int>(std::max<int64_t>(1, std::min(ceil_div(296, tiles), n / b / 256)));
+}
 
 int64_t status_bytes() { return 1024 * 8; }
 
 bool takes_tma(const void *p, int64_t cols) { return cols % 8 == 0 && aligned(p, 16); }
 
 // Whether a forward product goes row by row of the weights: up to four rows a
-// segment on average, and columns in whole 16-byte vectors.
+// segment on average, no more than 512 in all (each 8 rows of one segment read
+// its weights again), and columns in whole 16-byte vectors.
 bool takes_few(int kind, int dtype, int64_t m, int64_t n, int64_t b, const void *right) {
-  return kind == MATMUL_FORWARD && n <= 4 * b && m % (16 / elem_bytes(dtype)) == 0 && aligned(right, 16);
+  return kind == MATMUL_FORWARD && n <= 4 * b && n <= 512 && m % (16 / elem_bytes(dtype)) == 0 && aligned(right, 16);
 }
 
 MatmulShape make_shape(int kind, int dtype, int64_t k, int64_t m, int64_t n, int64_t b, const void *left,
@@ -46,8 +59,13 @@ MatmulShape make_shape(int kind, int dtype, int64_t k, int64_t m, int64_t n, int
   s.right_cols = m;
   s.left_pitch = s.left_cols;
   s.right_pitch = s.right_cols;
+  s.splits = splits_of(kind, dtype, k, m, n, b);
+  if (s.splits > 1) {
+    s.parts_at = status_bytes();
+    s.bytes = align256(s.parts_at + s.splits * b * k * m * 4);
+  }
   if (dtype == RG_DTYPE_F32 || takes_few(kind, dtype, m, n, b, right)) return s;
-  s.bytes = status_bytes();
+  if (!s.bytes) s.bytes = status_bytes();
   if (!takes_tma(left, s.left_cols)) {
     s.pack_left = true;
     s.left_pitch = (s.left_cols + 7) / 8 * 8;
@@ -81,7 +99,7 @@ int check_shape(int kind, int dtype, int index_dtype, int64_t k, int64_t m, int6
 
 // Row tiles of `tile` rows, at most: a segment has one that is not full.
 int64_t most_row_tiles(int kind, const MatmulArgs &p, int tile) {
-  return kind == MATMUL_GRAD_WEIGHTS ? p.b * ceil_div(p.k, tile) : p.n / tile + std::min(p.n, p.b);
+  return kind == MATMUL_GRAD_WEIGHTS ? p.splits * p.b * ceil_div(p.k, tile) : p.n / tile + std::min(p.n, p.b);
 }
 
 template <typename OffT, int KIND, int TILE, int SIZE>
@@ -107,7 +125,7 @@ template <typename OffT, int KIND>
 int launch_simt(const MatmulArgs &p, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
   const int64_t tiles =
       (KIND == MATMUL_GRAD_WEIGHTS ? p.b * ceil_div(p.k, 128) : ceil_div(p.n, 128)) * ceil_div(p.cols, 128);
-  const bool large = tiles >= dev.sm_count;
+  const bool large = tiles >= dev.sm_count && p.splits == 1;
   if (p.k % 4 == 0 && p.m % 4 == 0 && aligned(p.left, 16) && aligned(p.right, 16) && aligned(p.out, 16)) {
     if (large) return launch_simt_tile<OffT, KIND, 128, 4>(p, dev, stream, report);
     return launch_simt_tile<OffT, KIND, 64, 4>(p, dev, stream, report);
@@ -300,7 +318,7 @@ int rg_matmul(int kind, int dtype, int index_dtype, int64_t k, int64_t m, int64_
     report->workspace_bytes = s.bytes;
     report->d_vector = 1;
     report->d_tile = 1;
-    report->status_offset = s.bytes ? 0 : -1;
+    report->status_offset = dtype == RG_DTYPE_BF16 && s.bytes ? 0 : -1;
   }
   if (s.bytes) {
     if (!workspace || workspace_bytes < s.bytes) return fail(RG_ERR_WORKSPACE, "workspace missing or too small");
@@ -321,6 +339,8 @@ int rg_matmul(int kind, int dtype, int index_dtype, int64_t k, int64_t m, int64_
   p.left_pitch = s.left_pitch;
   p.right_pitch = s.right_pitch;
   p.out_pitch = s.cols;
+  p.splits = s.splits;
+  p.parts = s.splits > 1 ? reinterpret_cast<float *>(static_cast<char *>(workspace) + s.parts_at) : nullptr;
   p.status = static_cast<unsigned long long *>(workspace);
   char *scratch = static_cast<char *>(workspace);
   if (s.pack_left) {
@@ -333,8 +353,17 @@ int rg_matmul(int kind, int dtype, int index_dtype, int64_t k, int64_t m, int64_
     status = pack(right, scratch + s.right_at, s.right_rows, s.right_cols, s.right_pitch, dev, on, report);
     if (status) return status;
   }
-  if (index_dtype == RG_INDEX_I32) return launch_kind<int32_t>(kind, dtype, p, dev, on, report);
-  return launch_kind<int64_t>(kind, dtype, p, dev, on, report);
+  status = index_dtype == RG_INDEX_I32 ? launch_kind<int32_t>(kind, dtype, p, dev, on, report)
+                                       : launch_kind<int64_t>(kind, dtype, p, dev, on, report);
+  if (status || s.splits == 1) return status;
+  const int64_t count = b * k * m;
+  const dim3 grid(static_cast<unsigned>(std::min(ceil_div(count, 256), static_cast<int64_t>(dev.sm_count) * 8)), 1, 1);
+  if (dtype == RG_DTYPE_F32)
+    matmul_parts_kernel<float><<<grid, 256, 0, on>>>(p.parts, static_cast<float *>(out), count, s.splits);
+  else
+    matmul_parts_kernel<__nv_bfloat16><<<grid, 256, 0, on>>>(p.parts, static_cast<__nv_bfloat16 *>(out), count, s.splits);
+  record_launch(report, K_MATMUL_PARTS, grid, 256, 0);
+  return check_cuda(cudaGetLastError(), "matmul_parts_kernel launch");
 }
 
 }  // extern "C"

@@ -28,6 +28,10 @@ struct MatmulArgs {
   int64_t left_pitch, right_pitch, out_pitch;  // elements between rows
   int col_tiles;
   int row_tiles;             // weights kind: row tiles of a segment
+  // Weights kind, where there are few tiles and long segments: each segment's
+  // rows in `splits` parts, with a sum each in `parts` (f32 [splits][B][K][M]).
+  int splits;
+  float *parts;
   unsigned long long *status;
 };
 
@@ -35,7 +39,7 @@ struct MatmulArgs {
 // weights kind), and the segment's rows [begin, end).
 struct MatmulTile {
   int64_t seg, row, row_end, begin, end;
-  int col_tile;
+  int col_tile, split;
 };
 
 // Walks a CTA's tiles, in ascending order.  Forward and values: the tiles of a
@@ -54,12 +58,19 @@ struct MatmulWalk {
     t.col_tile = static_cast<int>(index % p.col_tiles);
     const int64_t tile = index / p.col_tiles;
     if constexpr (KIND == MATMUL_GRAD_WEIGHTS) {
-      t.seg = tile / p.row_tiles;
-      if (t.seg >= b) return false;
-      t.row = (tile - t.seg * p.row_tiles) * TILE;
+      const int64_t part = tile / p.row_tiles;
+      t.split = static_cast<int>(part / b);
+      if (t.split >= p.splits) return false;
+      t.seg = part - t.split * b;
+      t.row = (tile - part * p.row_tiles) * TILE;
       t.row_end = min(t.row + TILE, p.rows);
       t.begin = min(max(static_cast<int64_t>(offsets[t.seg]), int64_t{0}), p.n);
       t.end = max(min(static_cast<int64_t>(offsets[t.seg + 1]), p.n), t.begin);
+      if (p.splits > 1) {  // (parts of whole slices of 64)
+        const int64_t per = ((t.end - t.begin + p.splits - 1) / p.splits + 63) / 64 * 64;
+        t.begin = min(t.begin + t.split * per, t.end);
+        t.end = min(t.begin + per, t.end);
+      }
       return true;
     } else {
       const int lane = threadIdx.x & 31;
@@ -95,5 +106,17 @@ struct MatmulWalk {
     }
   }
 };
+
+// The parts' sums, in order, rounded once.
+template <typename T>
+__global__ void __launch_bounds__(256) matmul_parts_kernel(const float *__restrict__ parts, T *__restrict__ out,
+                                                           int64_t count, int splits) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += int64_t{gridDim.x} * 256) {
+    float sum[1] = {0.0f};
+#pragma unroll 4
+    for (int z = 0; z < splits; ++z) sum[0] += parts[z * count + i];
+    VecIO<T, 1>::store(out + i, sum);
+  }
+}
 
 }  // namespace rgb

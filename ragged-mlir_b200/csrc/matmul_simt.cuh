@@ -136,7 +136,8 @@ __global__ void __launch_bounds__(kSimtThreads, TILE == 128 ? 2 : 3) matmul_simt
         }
       }
     }
-    float *to = out + (KIND == MATMUL_GRAD_WEIGHTS ? t.seg * p.k * p.m : int64_t{0});
+    float *to = out;
+    if constexpr (KIND == MATMUL_GRAD_WEIGHTS) to = (p.parts ? p.parts + t.split * p.b * p.k * p.m : out) + t.seg * p.k * p.m;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int64_t row = t.row + (i / 4) * 64 + ty * 4 + i % 4;

@@ -215,6 +215,17 @@ struct TensorStore {
         tmem_load_32(at + 32, v[1]);
         asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
       }
+      if constexpr (KIND == MATMUL_GRAD_WEIGHTS) {
+        if (p.parts) {  // a part's sum, f32: a row a lane (few and small tiles alone are split)
+          float *row = p.parts + ((t.split * p.b + t.seg) * p.rows + row0 + lane) * p.cols;
+          if (lane < rows) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              if (col0 + i < p.cols) row[col0 + i] = __uint_as_float(v[i / 32][i % 32]);
+          }
+          continue;
+        }
+      }
       // Row `lane`, 8 pieces of 16 bytes, permuted so that neither this nor
       // the reading across rows meets a bank twice.
 #pragma unroll

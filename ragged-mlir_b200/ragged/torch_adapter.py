@@ -208,14 +208,15 @@ def _scan_call(values, gates, offsets, initial, program, mode: str, record: bool
     return out, final, carries
 
 
-def _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final, program, known=False):
+def _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final, program, known=None):
     """The gradients of values, gates and initial, on the GPU.  ``known``: the
     tensors are those of a forward call and the gradients autograd made of its
-    outputs, so that they fit."""
+    outputs, so that they fit, and these gradients are wanted."""
     torch = _torch()
     values, gates, initial, grad_out, grad_final = _dense(values, gates, initial, grad_out, grad_final)
-    grad_values, grad_gates = torch.empty_like(values), torch.empty_like(values)
-    grad_initial = torch.empty_like(initial) if initial is not None else None
+    wanted = known or (True, True, initial is not None)
+    grad_values, grad_gates, grad_initial = (torch.empty_like(t) if want else None
+                                             for t, want in zip((values, values, initial), wanted))
     if known:
         program._gradients(torch, values, gates, offsets, carries, grad_out, None, initial, grad_final, grad_values,
                            grad_gates, grad_initial)
@@ -338,7 +339,9 @@ def _autograd_functions(torch) -> dict[str, Any]:
             values, gates, offsets, carries, initial = ctx.saved_tensors
             if grad_out is None:
                 grad_out = torch.zeros_like(values)
-            grads = _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final, ctx.program, True)
+            wanted = ctx.needs_input_grad
+            grads = _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final, ctx.program,
+                                        (wanted[0], wanted[1], wanted[3]))
             return grads[0], grads[1], None, grads[2], None, None
 
     class Matmul(torch.autograd.Function):

@@ -126,6 +126,20 @@ def test_wide_tiles(cuda, k, m, lengths):
             assert ((got.double() - want).abs() <= limit).all().item(), s
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("k,m,lengths", [(64, 64, [20_000]), (33, 100, [9000, 0, 5, 3001]), (200, 72, [64 * 40, 64 * 41 + 1]),
+                                         (1, 8, [100_000]), (256, 64, [0, 6000, 0, 7777])])
+def test_gradients_of_small_weights_of_long_segments(cuda, dtype, k, m, lengths):
+    """Few tiles: the sums over a segment's rows are taken in parts."""
+    torch = cuda
+    case = make_case(lengths, k, m, dtype, seed=k)
+    check(case, run(torch, case, dtype), dtype)
+    t = device(torch, case, dtype)
+    report = matmul_program(dtype, k, m).run_backward(t["values"], t["weights"], t["offsets"], t["grad_out"],
+                                                      grad_weights=torch.empty_like(t["weights"]))
+    assert "matmul_parts" in report.kernel_names
+
+
 @pytest.mark.parametrize("k,m", [(8, 8), (7, 64), (100, 136), (1024, 264), (2500, 40)])
 @pytest.mark.parametrize("lengths", [[1], [3], [8, 1], [0, 1, 2, 0, 4, 0, 5], [1] * 30, [0] * 60 + [100, 9, 16, 17] + [0] * 40])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -349,6 +363,47 @@ def test_operands_beyond_32_bits_of_elements(cuda):
     out = torch.empty((n, m), dtype=torch.bfloat16, device="cuda")
     program.run(values, weights, torch.from_numpy(offsets_of(lengths)).to("cuda"), out)
     assert torch.all(out[-3:, 5] == k / 2).item() and out.count_nonzero().item() == 3
+
+
+def test_a_captured_training_step(cuda):
+    """Projection, recurrence and their gradients by autograd, inside one graph,
+    replayed on new inputs; no eager graph of the leaves is alive."""
+    torch = cuda
+    from ragged import ArtifactCache, Compiler, ScanSpec, torch_adapter
+    offsets = torch.from_numpy(offsets_of([300, 0, 41, 700])).to("cuda")
+    n, k, d = 1041, 40, 64
+    scan = Compiler().compile(ScanSpec("bf16", d), ArtifactCache(_cache_dir(), max_specializations=4096))
+    project = matmul_program("bf16", k, d)
+    generator = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *s: torch.randn(s, generator=generator, device="cuda").bfloat16()  # noqa: E731
+    x, w, gates, grad = rand(n, k), rand(4, k, d), torch.sigmoid(rand(n, d)), rand(n, d)
+    leaves = [t.requires_grad_() for t in (x, w, gates)]
+
+    def step():
+        h, _ = torch_adapter.segment_scan(torch_adapter.segment_matmul(x, w, offsets, program=project), gates, offsets,
+                                          program=scan)
+        return torch.autograd.grad(h, leaves, grad)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for _ in range(2):
+        with torch.no_grad():
+            x.copy_(rand(n, k))
+            w.copy_(rand(4, k, d))
+            grad.copy_(rand(n, d))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [g.clone() for g in captured]
+        for a, b in zip(kept, step()):
+            assert torch.equal(a, b)
+    del graph
 
 
 def test_a_run_of_the_operators_together(cuda):

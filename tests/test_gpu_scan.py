@@ -340,6 +340,56 @@ def test_autograd_layouts_and_missing_gradients(cuda):
     assert not out.requires_grad
 
 
+@pytest.mark.parametrize("wanted", [(0,), (1,), (2,), (0, 2)])
+def test_gradients_of_some_inputs(cuda, wanted):
+    """Gradients that no one asks for are not computed; the others are the same."""
+    torch = cuda
+    from ragged import torch_adapter
+    case = make_case(LENGTHS["mixed"], 48, "bf16", True)
+    all_of_them = run(torch, case, "bf16")
+    t = device(torch, case, "bf16", "i64")
+    names = ("values", "gates", "initial")
+    leaves = [t[names[i]].requires_grad_() for i in wanted]
+    out, final = torch_adapter.segment_scan(t["values"], t["gates"], t["offsets"], program=scan_program("bf16", 48),
+                                            initial=t["initial"])
+    grads = torch.autograd.grad((out, final), leaves, (t["grad_out"], t["grad_final"]))
+    for i, grad in zip(wanted, grads):
+        assert np.array_equal(host(grad), all_of_them["grad_" + names[i]]), names[i]
+
+
+_FIRST_CALL = """
+import sys
+sys.path[:0] = {paths!r}
+import tempfile, torch
+from ragged import ArtifactCache, Compiler, MatmulSpec, ScanSpec
+cache = ArtifactCache(tempfile.mkdtemp())
+scan = Compiler().compile(ScanSpec("f32", 32), cache)
+product = Compiler().compile(MatmulSpec("bf16", 64, 64), cache)
+v, g = torch.ones(3000, 32, device="cuda"), torch.full((3000, 32), 0.5, device="cuda")
+o, out = torch.tensor([0, 1, 3000], device="cuda"), torch.empty(3000, 32, device="cuda")
+x, w = torch.ones(3000, 64, device="cuda").bfloat16(), torch.ones(2, 64, 64, device="cuda").bfloat16()
+y = torch.empty_like(x)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    scan.run(v, g, o, out)
+    product.run(x, w, o, y)
+graph.replay()
+torch.cuda.synchronize()
+assert out[0, 0].item() == 1 and abs(out[2999, 5].item() - 2) < 1e-6 and torch.all(y == 64).item()
+print("captured")
+"""
+
+
+def test_the_first_call_may_be_captured(cuda):
+    """A process whose first calls are inside a graph capture."""
+    import subprocess
+    import sys
+    from conftest import PACKAGE, REPO
+    code = _FIRST_CALL.format(paths=[str(REPO), str(PACKAGE)])
+    result = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert result.returncode == 0 and "captured" in result.stdout, result.stderr[-2000:]
+
+
 def test_gradients_are_the_differences_of_the_outputs(cuda):
     """The loss <grad_out, out> + <grad_final, final> is linear in values and
     initial, and in each single row of the gates, so its differences over
