@@ -25,26 +25,50 @@ struct MatmulShape {
   int64_t left_at, right_at, parts_at, bytes;  // workspace
 };
 
-// Columns of a tensor-core tile of the weights kind and tiles of 64 x 64 of the
-// f32 kernel decide how many tiles there are: with fewer than the SMs, each
-// segment's rows are split so that there are two a SM, into parts of 256 rows
-// at least.
-int splits_of(int kind, int dtype, int64_t k, int64_t m, int64_t n, int64_t b) {
-  if (kind != MATMUL_GRAD_WEIGHTS || b == 0) return 1;
-  const int64_t tiles = dtype == RG_DTYPE_F32 ? b * ceil_div(k, 64) * ceil_div(m, 64) : b * ceil_div(k, 128) * ceil_div(m, 64);
-  if (tiles >= 148) return 1;
-  return static_cast<int>(std::max<int64_t>(1, std::min(ceil_div(296, tiles), n / b / 256)));
+// The weights kind's tiles, `tile` rows by `cols` columns (f32: tile by tile),
+// and the parts that each segment's rows are split into.  A few tiles of long
+// segments leave SMs idle: parts give each SM one (bf16) or two (f32), of 1024
+// rows at least (bf16; 256, f32), since each costs a write and a read of its f32
+// sums.  Of one segment of 65536 rows, 512 x 512: 61 us in 9 parts, 260 in one,
+// bf16; 622 in 18 parts, 2240 in one, f32.  8 segments of 1024 rows, 128 x 128:
+// 22 us in parts of 512 rows, 14 in one, bf16.
+struct WeightsPlan {
+  int tile, cols, splits;
+};
+
+int parts_of(int64_t slots, int64_t tiles, int64_t rows, int64_t least) {
+  return static_cast<int>(std::max<int64_t>(1, std::min(slots / tiles, rows / least)));
+}
+
+WeightsPlan plan_weights(int dtype, int64_t k, int64_t m, int64_t n, int64_t b) {
+  if (dtype == RG_DTYPE_BF16) {
+    const int cols = m > 64 ? 128 : 64;
+    return {128, cols, parts_of(148, b * ceil_div(k, 128) * ceil_div(m, cols), n / b, 1024)};
+  }
+  const int64_t large = b * ceil_div(k, 128) * ceil_div(m, 128), small = b * ceil_div(k, 64) * ceil_div(m, 64);
+  if (large >= 148) return {128, 128, 1};
+  if (small >= 296) return {64, 64, 1};
+  // 128 x 128 in parts that fill three quarters of the SMs, else 64 x 64 (one
+  // segment as above: 872 us; 8 segments of 1024 rows, 128 x 128: 22 and 43 us).
+  const int parts = parts_of(296, large, n / b, 256);
+  if (large * parts >= 111) return {128, 128, parts};
+  return {64, 64, parts_of(296, small, n / b, 256)};
 }
 
 int64_t status_bytes() { return 1024 * 8; }
 
 bool takes_tma(const void *p, int64_t cols) { return cols % 8 == 0 && aligned(p, 16); }
 
-// Whether a forward product goes row by row of the weights: up to four rows a
-// segment on average, no more than 512 in all (each 8 rows of one segment read
-// its weights again), and columns in whole 16-byte vectors.
+// Whether a forward product goes row by row of the weights (columns in whole
+// 16-byte vectors).  f32: up to 16 rows a segment on average.  1024 x 2048
+// weights, 16 segments: 32 rows 37 us, 137 with tiles of 64; 256 rows 72 and 137;
+// 1024 rows 225 and 219; all of 1024 rows in one segment 213 and 150.  bf16: up
+// to two rows a segment, 256 in all.  There 16 rows 20.5 us, 26.6 with tensor-core
+// tiles; 32 rows 24.6 and 28.7; 48 rows 30.7 and 28.7; 512 rows in 256 segments of
+// 512 x 512 43 and 37; 512 rows in one segment 94 and 14.
 bool takes_few(int kind, int dtype, int64_t m, int64_t n, int64_t b, const void *right) {
-  return kind == MATMUL_FORWARD && n <= 4 * b && n <= 512 && m % (16 / elem_bytes(dtype)) == 0 && aligned(right, 16);
+  if (kind != MATMUL_FORWARD || m % (16 / elem_bytes(dtype)) || !aligned(right, 16)) return false;
+  return dtype == RG_DTYPE_F32 ? n <= 16 * b : n <= 2 * b && n <= 256;
 }
 
 MatmulShape make_shape(int kind, int dtype, int64_t k, int64_t m, int64_t n, int64_t b, const void *left,
@@ -59,7 +83,7 @@ MatmulShape make_shape(int kind, int dtype, int64_t k, int64_t m, int64_t n, int
   s.right_cols = m;
   s.left_pitch = s.left_cols;
   s.right_pitch = s.right_cols;
-  s.splits = splits_of(kind, dtype, k, m, n, b);
+  s.splits = kind == MATMUL_GRAD_WEIGHTS && b ? plan_weights(dtype, k, m, n, b).splits : 1;
   if (s.splits > 1) {
     s.parts_at = status_bytes();
     s.bytes = align256(s.parts_at + s.splits * b * k * m * 4);
@@ -119,13 +143,16 @@ int launch_simt_tile(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream, 
   return check_cuda(cudaGetLastError(), "matmul_simt_kernel launch");
 }
 
-// 128 x 128 tiles where they give every SM one, 64 x 64 where they do not;
-// 16-byte pieces where all rows start at 16-byte boundaries.
+// 128 x 128 tiles where they give two thirds of the SMs one, else 64 x 64: 8192
+// rows x 512 x 512 in 16 segments 104 us, 150 with tiles of 64; 4096 rows in 8
+// segments 57 and 80; 1024 rows in 8 segments (32 tiles) 55 and 43; 2048 rows in
+// 64 segments (64 tiles, a quarter full) 98 and 76.  16-byte pieces where all
+// rows start at 16-byte boundaries.
 template <typename OffT, int KIND>
 int launch_simt(const MatmulArgs &p, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
-  const int64_t tiles =
-      (KIND == MATMUL_GRAD_WEIGHTS ? p.b * ceil_div(p.k, 128) : ceil_div(p.n, 128)) * ceil_div(p.cols, 128);
-  const bool large = tiles >= dev.sm_count && p.splits == 1;
+  const bool large = KIND == MATMUL_GRAD_WEIGHTS
+                         ? plan_weights(RG_DTYPE_F32, p.k, p.m, p.n, p.b).tile == 128
+                         : ceil_div(p.n, 128) * ceil_div(p.cols, 128) >= dev.sm_count * 2 / 3;
   if (p.k % 4 == 0 && p.m % 4 == 0 && aligned(p.left, 16) && aligned(p.right, 16) && aligned(p.out, 16)) {
     if (large) return launch_simt_tile<OffT, KIND, 128, 4>(p, dev, stream, report);
     return launch_simt_tile<OffT, KIND, 64, 4>(p, dev, stream, report);
@@ -212,21 +239,27 @@ int launch_pair(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream, rg_re
   return check_cuda(cudaGetLastError(), "matmul_pair_kernel launch");
 }
 
-// The widest tiles that give every SM one (a segment's last row tile counted half).
+// Pairs of SMs where their tiles of 256 x 256 keep all SMs busy twice over and few
+// of a tile's rows are past a segment's end; else the widest tiles of one SM that
+// give every SM one (128 columns: half of the SMs, which computes 2048 rows x 512
+// x 512 in 8 segments in 10 us, 12 with 64).  In us, for pairs, 256 and 128
+// columns: 65536 rows x 2048 x 2048 in 16 segments 360, 379, 526; 16384 rows x 1024
+// x 2048 in 8 segments 64, 68, 88; in 32 segments 72, 74, 98; 8192 rows in 32
+// segments 55, 53, 61.
 template <typename OffT, int KIND>
 int launch_tensor(const MatmulArgs &p, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
+  // (a segment's last row tile is counted half)
   const int64_t row_tiles = KIND == MATMUL_GRAD_WEIGHTS ? p.b * ceil_div(p.k, kTensorRows)
                                                          : p.n / kTensorRows + std::max<int64_t>(std::min(p.n, p.b) / 2, 1);
-  // Pairs of SMs where 256 x 256 tiles keep all of them busy twice over and few
-  // of their rows are past a segment's end (segments of 768 rows on average).
   const int64_t pair_rows = KIND == MATMUL_GRAD_WEIGHTS ? p.b * ceil_div(p.k, kPairRows) : p.n / kPairRows;
-  const bool full = KIND == MATMUL_GRAD_WEIGHTS ? p.k > 128 : p.n >= 768 * std::min(p.n, p.b);
+  const bool full = KIND == MATMUL_GRAD_WEIGHTS ? p.k > 128 : p.n >= 512 * std::min(p.n, p.b);
   if (p.cols > 128 && full && pair_rows * ceil_div(p.cols, kPairCols) >= dev.sm_count)
     return launch_pair<OffT, KIND>(p, dev, stream, report);
   if (p.cols > 128 && row_tiles * ceil_div(p.cols, 256) >= dev.sm_count)
     return launch_tensor_cols<OffT, KIND, 256>(p, dev, stream, report);
-  if (p.cols > 64 && row_tiles * ceil_div(p.cols, 128) >= dev.sm_count)
-    return launch_tensor_cols<OffT, KIND, 128>(p, dev, stream, report);
+  const bool wide = KIND == MATMUL_GRAD_WEIGHTS ? plan_weights(RG_DTYPE_BF16, p.k, p.m, p.n, p.b).cols == 128
+                                                 : p.cols > 64 && row_tiles * ceil_div(p.cols, 128) >= dev.sm_count / 2;
+  if (wide) return launch_tensor_cols<OffT, KIND, 128>(p, dev, stream, report);
   return launch_tensor_cols<OffT, KIND, 64>(p, dev, stream, report);
 }
 

@@ -12,19 +12,25 @@ namespace {
 
 constexpr int64_t kMaxScanDim = 65536;
 
-
 struct ScanShape {
   int vec, tiles, shift, lane_rows, row_shift;
   int64_t slabs, blocks;
 };
 
-constexpr int64_t kAloneRows = 256;  // rows up to which walk is the only launch
+// Whether walk is the only launch: up to 128 rows, or 512 of up to four a segment
+// on average, where catching up costs less than two more launches.  In us, alone
+// and in three launches, 1024 columns of bf16: 256 rows in 256 segments 16 and 27
+// (backward 29 and 37), 512 in 128 14 and 21; 128 in 4 14 and 16; 256 in 4 18 and
+// 16 (23 and 18); 512 in 4, the most that rows of unlike lengths can lose, 35 and 16.
+bool walks_alone(int64_t n, int64_t b) { return n <= 128 || (n <= 512 && n <= 4 * b); }
 
 // 32 lanes, or as many as cover a row, of one vector each: 8 bytes where they
 // fill the lanes, else 4 (one element where D is odd).  8 bytes take two thirds
-// of the instructions (f32 262k x 100: 127 -> 111 us).  A lane takes 64 rows of a
-// slab, fewer where that would leave resident warps without a task.  `align`:
-// elements that all tensors are aligned for.
+// of the instructions: bf16 65536 x 1024 139 us (backward 186), 166 (227) with 4;
+// f32 262144 x 100 117 (158) and 131 (326).  A lane takes 64 rows of a slab, fewer
+// where that would leave resident warps without a task: f32 262144 x 100 117 us,
+// 158 with 16; 4096 x 512 20 (23) with 16, 29 (35) with 64.  `align`: elements that
+// all tensors are aligned for.
 ScanShape make_shape(int dtype, int64_t d, int64_t n, int64_t b, int align) {
   ScanShape s;
   s.vec = 8 / elem_bytes(dtype);
@@ -48,7 +54,9 @@ ScanShape make_shape(int dtype, int64_t d, int64_t n, int64_t b, int align) {
 }
 
 // Pairs, then states of each slab.
-int64_t layout_bytes(const ScanShape &s, int64_t n, int64_t d) { return n <= kAloneRows ? 0 : align256(s.slabs * d * 12); }
+int64_t layout_bytes(const ScanShape &s, int64_t n, int64_t d, int64_t b) {
+  return walks_alone(n, b) ? 0 : align256(s.slabs * d * 12);
+}
 
 int check_shape(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b) {
   if (dtype != RG_DTYPE_F32 && dtype != RG_DTYPE_BF16) return fail(RG_ERR_INVALID_ARGUMENT, "dtype must be f32 or bf16");
@@ -130,7 +138,7 @@ int run_scan(int dtype, int index_dtype, int align, ScanArgs &p, void *workspace
   if (status) return status;
   const ScanShape s = make_shape(dtype, p.d, p.n, p.b, align);
   if (s.blocks > 2000000000LL / s.tiles) return fail(RG_ERR_INVALID_ARGUMENT, "the call needs more than 2e9 tasks");
-  const int64_t need = layout_bytes(s, p.n, p.d);
+  const int64_t need = layout_bytes(s, p.n, p.d, p.b);
   if (report) {
     report->workspace_bytes = need;
     report->d_vector = s.vec;
@@ -168,7 +176,7 @@ int rg_scan_workspace_bytes(int dtype, int index_dtype, int64_t d, int64_t n, in
   // (the slabs go by the tensors' alignment)
   *bytes = 0;
   for (int align = 1; align <= 4; align *= 2)
-    *bytes = std::max(*bytes, layout_bytes(make_shape(dtype, d, n, b, align), n, d));
+    *bytes = std::max(*bytes, layout_bytes(make_shape(dtype, d, n, b, align), n, d, b));
   return RG_OK;
 }
 

@@ -27,8 +27,8 @@
 // in a backward pass), so that it meets first what fold left in L2.  The
 // arithmetic is one FMA an element, about 10 instructions an element in all.
 //
-// Up to 256 rows walk is the only launch: a lane whose rows go on from earlier
-// ones runs the recurrence over those itself.
+// For few rows walk is the only launch: a lane whose rows go on from earlier ones
+// runs the recurrence over those itself.
 //
 // The backward pass needs the states again.  It recomputes 8 rows at a time from
 // values and gates, from the state before them that forward records in f32 (4
@@ -79,7 +79,7 @@ struct ScanArgs {
   const float *grad_final;  // [B, D] or null
   void *grad_values, *grad_gates;
   float *grad_initial;  // [B, D] or null
-  // workspace (null up to 256 rows)
+  // workspace (null where walk is the only launch)
   float2 *pairs;    // (A, H) of each slab: [slabs][D]; A is NaN-boxed where the pair starts at a segment
   float *states;    // state before each slab: [slabs][D]
 };
