@@ -295,7 +295,7 @@ matmul_pair_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps) 
     for (int64_t index = first; going && walk.find(p, index, t); index += stride) {
       const bool nothing = KIND == MATMUL_GRAD_WEIGHTS && t.end == t.begin;
       if (!nothing) {
-        going = gate.wait(&ready[acc], acc_phase);
+        going = gate.wait(&ready[acc], acc_phase, slices(t));
         if (!going) break;
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
       }

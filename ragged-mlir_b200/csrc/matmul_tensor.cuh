@@ -166,12 +166,13 @@ __device__ __forceinline__ void umma_stage(uint32_t to, uint32_t left, uint32_t 
 }
 
 // Bounded wait by a role; on giving up marks the CTA so that all roles leave.
-// `status` is the CTA's own word.
+// `status` is the CTA's own word.  `slices`: what the wait may have to see
+// through, where that has no bound of its own.
 struct TensorGate {
   volatile int *abandoned;
   unsigned long long *status;
-  __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity) const {
-    for (int i = 0; i < kMbarWaitLimit; ++i) {
+  __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, int64_t slices = 0) const {
+    for (int64_t left = kMbarWaitLimit * (1 + (slices >> 14)); left > 0; --left) {
       if (mbar_try_wait(bar, parity)) return true;
       if (*abandoned) return false;
     }
@@ -218,7 +219,13 @@ struct TensorStore {
       if constexpr (KIND == MATMUL_GRAD_WEIGHTS) {
         if (p.parts) {  // a part's sum, f32: a row a lane (few and small tiles alone are split)
           float *row = p.parts + ((t.split * p.b + t.seg) * p.rows + row0 + lane) * p.cols;
-          if (lane < rows) {
+          if (lane < rows && p.cols % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < 64; i += 4) {
+              const uint32_t *x = &v[i / 32][i % 32];
+              if (col0 + i < p.cols) *reinterpret_cast<uint4 *>(row + col0 + i) = uint4{x[0], x[1], x[2], x[3]};
+            }
+          } else if (lane < rows) {
 #pragma unroll
             for (int i = 0; i < 64; ++i)
               if (col0 + i < p.cols) row[col0 + i] = __uint_as_float(v[i / 32][i % 32]);
@@ -442,7 +449,7 @@ matmul_tensor_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps
     for (int64_t index = blockIdx.x; going && walk.find(p, index, t); index += gridDim.x) {
       const bool nothing = KIND == MATMUL_GRAD_WEIGHTS && t.end == t.begin;
       if (!nothing) {
-        going = gate.wait(&ready[acc], acc_phase);
+        going = gate.wait(&ready[acc], acc_phase, slices(t));
         if (!going) break;
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
       }

@@ -189,14 +189,20 @@ struct ScanMarks {
   int *start_seg, *end_seg;         // rows each
 };
 
+// Returns the segment of row `row0`.
 template <typename OffT>
-__device__ __forceinline__ void scan_mark(const OffT *__restrict__ offsets, int64_t b, int64_t first, int64_t row0,
-                                          int rows, const ScanMarks &m) {
+__device__ __forceinline__ int64_t scan_mark(const OffT *__restrict__ offsets, int64_t b, int64_t row0, int rows,
+                                             const ScanMarks &m) {
   const int lane = threadIdx.x & 31;
   const int words = (rows < 64 ? 64 : rows) / 32;
   for (int i = lane; i < 2 * words; i += 32) m.start_mask[i] = 0;
   __syncwarp();
-  for (int64_t s = first + lane;; s += 32) {
+  int64_t first = -1, next = 0, row = row0;
+  bool search = true;
+  for (;;) {
+    if (search) next = max(next, scan_find(offsets, b, row));
+    if (first < 0) first = next;
+    const int64_t s = next + lane;
     const bool there = s < b;
     const int64_t begin = there ? static_cast<int64_t>(offsets[s]) - row0 : rows;
     const int64_t end = there ? static_cast<int64_t>(offsets[s + 1]) - 1 - row0 : rows;
@@ -211,8 +217,12 @@ __device__ __forceinline__ void scan_mark(const OffT *__restrict__ offsets, int6
       }
     }
     if (__any_sync(~0u, begin >= rows)) break;
+    next += 32;
+    search = !__any_sync(~0u, begin <= end);  // 32 segments without rows: on to the last one that starts there
+    row = row0 + __shfl_sync(~0u, begin, 31);
   }
   __syncwarp();
+  return first;
 }
 
 // Words of shared memory of a warp's marks.
@@ -241,6 +251,7 @@ struct ScanWarp {
   const ScanArgs &p;
   const OffT *__restrict__ offsets;
   int lanes, rows, words, base;  // base: this lane's first row of a slab
+  int limit;                     // rows of the slab before the last segment's end; those behind it are left alone
   int64_t pos, row0, col, seg0;  // slab in the order of the recurrence, its first row, this lane's column
   bool col_ok;
   ScanMarks m;
@@ -260,13 +271,13 @@ struct ScanWarp {
   __device__ __forceinline__ void go(int64_t slab, int tile) {
     pos = slab;
     row0 = (BACKWARD ? p.slabs - 1 - pos : pos) << p.row_shift;
+    limit = static_cast<int>(min(max(min(static_cast<int64_t>(offsets[p.b]), p.n) - row0, int64_t{0}), int64_t{rows}));
     col = (static_cast<int64_t>(tile) * lanes + (threadIdx.x & (lanes - 1))) * VEC;
     col_ok = col < p.d;
   }
   __device__ __forceinline__ void mark() {
     __syncwarp();
-    seg0 = scan_find(offsets, p.b, row0);
-    scan_mark(offsets, p.b, seg0, row0, rows, m);
+    seg0 = scan_mark(offsets, p.b, row0, rows, m);
   }
   __device__ __forceinline__ uint64_t lane_bits(const unsigned *mask) const {  // of this lane's rows
     if (p.lane_rows == 64) return mask[base >> 5] | (static_cast<uint64_t>(mask[(base >> 5) + 1]) << 32);
@@ -275,11 +286,11 @@ struct ScanWarp {
   }
   __device__ __forceinline__ bool starts_at_first() const { return m.start_mask[0] & 1; }
   __device__ __forceinline__ bool ends_at_last() const {
-    const int last = static_cast<int>(min(static_cast<int64_t>(rows), p.n - row0)) - 1;
-    return (m.end_mask[last >> 5] >> (last & 31)) & 1;
+    const int last = limit - 1;
+    return last >= 0 && (m.end_mask[last >> 5] >> (last & 31)) & 1;
   }
-  __device__ __forceinline__ int row_count(int64_t row) const {  // rows of the batch at `row`
-    return static_cast<int>(min(max(p.n - row, int64_t{0}), int64_t{BATCH}));
+  __device__ __forceinline__ int row_count(int batch) const {  // rows of this lane's batch
+    return min(max(limit - base - batch * BATCH, 0), BATCH);
   }
   __device__ __forceinline__ void state_of(const float *states, int64_t seg, float (&x)[VEC]) const {
     if (states) {
@@ -304,7 +315,7 @@ struct ScanWarp {
 #pragma unroll 1
     for (int batch = enter; BACKWARD ? batch >= 0 : batch < batches; batch += BACKWARD ? -1 : 1) {
       const int64_t row = row0 + base + batch * BATCH;
-      const int count = row_count(row);
+      const int count = row_count(batch);
       if (count <= 0) continue;
       Raw ra[BATCH], rx[BATCH];
       scan_rows<T, VEC>(gates + row * p.d + col, p.d, count, ra);
@@ -349,11 +360,11 @@ struct ScanWarp {
 #pragma unroll
     for (int v = 0; v < VEC; ++v) h[v] = 0.0f;
     const int64_t mine = row0 + base;
-    if (mine >= p.n || !col_ok) return;
+    if (base >= limit || !col_ok) return;
     const T *__restrict__ gates = static_cast<const T *>(p.gates);
     const T *__restrict__ second = static_cast<const T *>(BACKWARD ? p.grad_out : p.values);
     int64_t seg = seg0;  // the segment of this lane's first (last, BACKWARD) row
-    const int64_t here = BACKWARD ? min(mine + p.lane_rows, p.n) - 1 : mine;
+    const int64_t here = BACKWARD ? row0 + min(base + p.lane_rows, limit) - 1 : mine;
     const int at = static_cast<int>(here - row0);
     for (int i = at >> 5; i >= 0; --i) {
       const unsigned bits = m.start_mask[i] & (i == at >> 5 ? (2u << (at & 31)) - 1 : ~0u);
@@ -531,7 +542,7 @@ __global__ void __launch_bounds__(kScanThreads, BACKWARD ? 2 : 3) scan_walk_kern
       for (int k = 0; k < batches; ++k) {
         const int batch = BACKWARD ? batches - 1 - k : k;
         const int64_t row = w.row0 + w.base + batch * BATCH;
-        const int count = w.row_count(row);
+        const int count = w.row_count(batch);
         if (count <= 0 || !w.col_ok) continue;
         const int64_t at = row * p.d + w.col;
         const unsigned start = static_cast<unsigned>(starts >> (batch * BATCH)) & ((1u << BATCH) - 1);

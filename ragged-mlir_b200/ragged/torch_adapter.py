@@ -226,6 +226,14 @@ def _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad
     return grad_values, grad_gates, grad_initial
 
 
+def _no_tangents(torch, *tensors) -> None:
+    """Refuses forward-mode derivatives, which a call would drop unnoticed."""
+    forward = torch.autograd.forward_ad
+    if forward._current_level >= 0 and any(t is not None and forward.unpack_dual(t).tangent is not None
+                                           for t in tensors):
+        raise ValidationError("forward-mode derivatives are not supported")
+
+
 def _first_derivative(torch) -> None:
     if torch.is_grad_enabled():
         raise ValidationError("second derivatives are not supported (create_graph)")
@@ -473,6 +481,7 @@ def segment_scan(values, gates, offsets, *, program: CompiledScan, initial=None,
     gradients with ``torch.autograd.grad``, or drop earlier graphs first."""
     torch = _torch()
     record = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (values, gates, initial))
+    _no_tangents(torch, values, gates, initial)
     if _plain(torch, values, gates, offsets, initial):
         if record:
             return _autograd_functions(torch)["scan"].apply(values, gates, offsets, initial, program, mode)
@@ -488,6 +497,7 @@ def segment_matmul(values, weights, offsets, *, program: CompiledMatmul, mode: s
     differentiable (once) in values and weights.  (On captured backward
     passes: see ``segment_scan``.)"""
     torch = _torch()
+    _no_tangents(torch, values, weights)
     if _plain(torch, values, weights, offsets):
         if torch.is_grad_enabled() and (values.requires_grad or weights.requires_grad):
             return _autograd_functions(torch)["matmul"].apply(values, weights, offsets, program, mode)

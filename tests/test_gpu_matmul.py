@@ -128,7 +128,8 @@ def test_wide_tiles(cuda, k, m, lengths):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("k,m,lengths", [(64, 64, [20_000]), (33, 100, [9000, 0, 5, 3001]), (200, 72, [64 * 40, 64 * 41 + 1]),
-                                         (1, 8, [100_000]), (256, 64, [0, 6000, 0, 7777])])
+                                         (1, 8, [100_000]), (256, 64, [0, 6000, 0, 7777]),
+                                         (40, 30, [9000]), (136, 257, [5000])])
 def test_gradients_of_small_weights_of_long_segments(cuda, dtype, k, m, lengths):
     """Few tiles: the sums over a segment's rows are taken in parts."""
     torch = cuda
@@ -179,6 +180,30 @@ def test_no_rows(cuda, dtype, lengths):
     case = make_case(lengths, 24, 40, dtype)
     got = run(cuda, case, dtype)
     assert not got["grad_weights"].any()
+
+
+@pytest.mark.parametrize("k,m", [(40, 72), (33, 9)])
+@pytest.mark.parametrize("lengths,behind", [([3, 0, 9], 20), ([300, 0, 700, 0], 5), ([0, 0], 90)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_behind_the_last_segment_stay(cuda, dtype, lengths, behind, k, m):
+    """Neither read nor written: NaN in the inputs there reaches nothing."""
+    torch = cuda
+    case = make_case(lengths, k, m, dtype, seed=behind)
+    t = device(torch, case, dtype)
+    used = case["offsets"][-1]
+    for name in ("values", "grad_out"):
+        t[name] = torch.cat([t[name], torch.full((behind, t[name].shape[1]), float("nan"), device="cuda",
+                                                 dtype=t[name].dtype)])
+    program = matmul_program(dtype, k, m)
+    o = dict(out=torch.full_like(t["grad_out"], SENTINEL), grad_values=torch.full_like(t["values"], SENTINEL),
+             grad_weights=torch.full_like(t["weights"], SENTINEL))
+    program.run(t["values"], t["weights"], t["offsets"], o["out"])
+    program.run_backward(t["values"], t["weights"], t["offsets"], t["grad_out"], grad_values=o["grad_values"],
+                         grad_weights=o["grad_weights"])
+    for name in ("out", "grad_values"):
+        assert torch.all(o[name][used:] == SENTINEL).item(), name
+        o[name] = o[name][:used]
+    check(case, {name: host(x) for name, x in o.items()}, dtype)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])

@@ -182,6 +182,38 @@ def test_few_rows_among_many_empty_segments(cuda):
     check(case, run(cuda, case, "f32", "i32"), "f32")
 
 
+@pytest.mark.parametrize("initial", [False, True])
+@pytest.mark.parametrize("lengths,behind", [([3, 0, 9], 20), ([300, 0, 700, 0], 5), ([65, 2000, 1], 1500), ([0, 0], 900)])
+@pytest.mark.parametrize("dtype,d", [("f32", 12), ("bf16", 128)])
+def test_rows_behind_the_last_segment_stay(cuda, dtype, d, lengths, behind, initial):
+    """Neither read nor written: NaN in the inputs there reaches nothing."""
+    torch = cuda
+    case = make_case(lengths, d, dtype, initial, seed=behind)
+    t = device(torch, case, dtype, "i64")
+    used, b = case["offsets"][-1], len(lengths)
+    for name in ("values", "gates", "grad_out"):
+        t[name] = torch.cat([t[name], torch.full((behind, d), float("nan"), device="cuda", dtype=t[name].dtype)])
+    program = scan_program(dtype, d)
+    o = {name: torch.full_like(t["values"], SENTINEL) for name in ("out", "grad_values", "grad_gates")}
+    o["final"], o["grad_initial"] = (torch.full((b, d), SENTINEL, device="cuda") for _ in range(2))
+    carries = torch.empty((program.carry_rows(used + behind), d), device="cuda")
+    program.run(t["values"], t["gates"], t["offsets"], o["out"], initial=t["initial"], final=o["final"], carries=carries)
+    program.run_backward(t["values"], t["gates"], t["offsets"], carries, t["grad_out"], initial=t["initial"],
+                         grad_final=t["grad_final"], grad_values=o["grad_values"], grad_gates=o["grad_gates"],
+                         grad_initial=o["grad_initial"] if initial else None)
+    for name in ("out", "grad_values", "grad_gates"):
+        assert torch.all(o[name][used:] == SENTINEL).item(), name
+        o[name] = o[name][:used]
+    check(case, {name: host(x) for name, x in o.items()}, dtype)
+
+
+def test_many_empty_segments_in_the_middle_of_a_slab(cuda):
+    lengths = [3] + [0] * 9000 + [5] + [0] * 40 + [600, 0, 1] + [0] * 70 + [2]
+    for d in (8, 100):
+        case = make_case(lengths, d, "f32", True)
+        check(case, run(cuda, case, "f32"), "f32")
+
+
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 @pytest.mark.parametrize("where", ["values", "initial", "grad_out", "grad_final"])
 def test_nothing_crosses_segments(cuda, where, bad):

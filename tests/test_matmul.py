@@ -126,3 +126,16 @@ def test_reference_gradients_are_differences():
                 y[at] += sign * 0.5
                 moved.append((ref.products(*other(y), offsets)["out"][0] * grad).sum())
             assert abs(moved[0] - moved[1] - found[name][0][at]) < 1e-9
+
+
+def test_forward_mode_is_refused(native_library, tmp_path):
+    from ragged import ArtifactCache, Compiler, MatmulSpec, ScanSpec, ValidationError, torch_adapter
+    cache, offsets = ArtifactCache(tmp_path), torch.tensor([0, 4])
+    scan, product = (Compiler().compile(spec, cache) for spec in (ScanSpec("f32", 8), MatmulSpec("f32", 8, 8)))
+    x, w = torch.ones(4, 8), torch.ones(1, 8, 8)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, x)
+        with pytest.raises(ValidationError, match="forward-mode"):
+            torch_adapter.segment_scan(x, dual, offsets, program=scan)
+        with pytest.raises(ValidationError, match="forward-mode"):
+            torch_adapter.segment_matmul(dual, w, offsets, program=product)
