@@ -1,6 +1,6 @@
 /*
  * ragged_b200.h -- C ABI of the B200 (sm_100a) segmented sum / max / softmax
- * library, libragged_b200.so.
+ * library, libragged_b200.so, and of its segmented scan and matrix product.
  *
  * It replaces the reference's native launcher (simon-jd/ragged-mlir):
  * the nanobind module `ragged._native.DriverModule` declared in
@@ -284,8 +284,9 @@ int rg_run_noalloc(int op, int dtype, int index_dtype, int64_t d, int64_t n, int
  * follows.  rg_scan_backward takes the forward call's inputs and carries and
  * the gradients of out and final_state (NULL: zero) and writes the gradients
  * that are not NULL; grad_initial (f32 [B, D]) needs `initial`.  Written
- * tensors overlap nothing.  Results do not depend on timing: equal inputs give
- * equal bits. */
+ * tensors overlap nothing.  Rows behind offsets[B] are neither read nor written
+ * (a caller may keep N fixed).  Results do not depend on timing: equal inputs
+ * give equal bits. */
 int rg_scan_workspace_bytes(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, int64_t *bytes);
 int rg_scan(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, const void *values, const void *gates,
             const void *offsets, const float *initial, void *out, float *final_state, float *carries,
@@ -307,6 +308,7 @@ int rg_scan_backward(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b
  *   RG_MATMUL_GRAD_WEIGHTS        values [N, K]     grad_out [N, M]  [B, K, M]
  * Sums are f32, rounded once.  A segment without rows has zeros for the
  * gradient of its weights; its weights are not read.  out overlaps nothing.
+ * Rows behind offsets[B] reach no result and are not written.
  * bf16 runs on the tensor cores, f32 in f32 arithmetic.
  *
  * rg_matmul_workspace_bytes: scratch of a call (256-byte aligned; 0: none),

@@ -6,7 +6,12 @@
 // slices of 16 of the contraction in a ring of shared-memory stages that
 // asynchronous copies fill three slices ahead; two CTAs an SM fill each other's
 // waits.  Bound: 128 FMAs a clock and SM; a thread loads 16 values from shared
-// memory for 64 FMAs, so the pipes and not the loads set the pace.
+// memory for 64 FMAs, so the pipes and not the loads set the pace.  Packed FMAs
+// (two columns at once) leave issue slots to the loads.
+//
+// 8192 rows x 512 x 512 in 8 segments: 104 us forward, 115 and 127 for the gradients
+// of values and weights: 41 TFLOP/s of the pipes' 74, the rest being rows past the
+// segments' ends and 288 tiles on 296 places.
 #pragma once
 
 #include "matmul.cuh"

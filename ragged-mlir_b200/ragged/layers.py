@@ -8,6 +8,9 @@ unless ``stream`` is given, no synchronisation in validated mode, and
 ``mode="checked"`` to validate the offsets on the device first.  ``run``
 records no gradient; ``run_backward`` computes the gradients of a call, and
 ``torch_adapter.segment_scan`` / ``segment_matmul`` put both behind autograd.
+Rows behind the last offset are left as they are and reach no result, so a
+caller of ``run`` may keep N fixed while the offsets change (autograd gives no
+gradients for them: there offsets end at N, as everywhere else).
 
 Neither operation exists in the reference, whose programs end at sums, maxima
 and softmaxes of packed rows.
