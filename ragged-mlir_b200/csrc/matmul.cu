@@ -203,6 +203,22 @@ int make_maps(TensorMaps &maps, const MatmulArgs &p, int right) {
   return RG_OK;
 }
 
+// After a pack launch the product may start before that ends (its copies wait).
+int launch_after_pack(void (*kernel)(MatmulArgs, TensorMaps), dim3 grid, int smem, const MatmulArgs &p,
+                      const TensorMaps &maps, cudaStream_t stream) {
+  cudaLaunchAttribute serial;
+  serial.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  serial.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(kTensorThreads, 1, 1);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = &serial;
+  config.numAttrs = p.packed ? 1 : 0;
+  return check_cuda(cudaLaunchKernelEx(&config, kernel, p, maps), "segmented product launch");
+}
+
 template <typename OffT, int KIND, int COLS>
 int launch_tensor_cols(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
   const auto kernel = matmul_tensor_kernel<OffT, KIND, COLS>;
@@ -216,9 +232,8 @@ int launch_tensor_cols(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream
   p.row_tiles = static_cast<int>(ceil_div(p.k, kTensorRows));
   const int64_t tiles = most_row_tiles(KIND, p, kTensorRows) * p.col_tiles;
   const dim3 grid(static_cast<unsigned>(std::min(tiles, static_cast<int64_t>(std::min(dev.sm_count * tensor_ctas(COLS), 1024)))), 1, 1);
-  kernel<<<grid, kTensorThreads, smem, stream>>>(p, maps);
   record_launch(report, K_MATMUL_TENSOR, grid, kTensorThreads, smem);
-  return check_cuda(cudaGetLastError(), "matmul_tensor_kernel launch");
+  return launch_after_pack(kernel, grid, smem, p, maps, stream);
 }
 
 template <typename OffT, int KIND>
@@ -234,9 +249,8 @@ int launch_pair(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream, rg_re
   p.row_tiles = static_cast<int>(ceil_div(p.k, kPairRows));
   const int64_t tiles = most_row_tiles(KIND, p, kPairRows) * p.col_tiles;
   const dim3 grid(static_cast<unsigned>(2 * std::min(tiles, static_cast<int64_t>(std::min(dev.sm_count, 1024) / 2))), 1, 1);
-  kernel<<<grid, kTensorThreads, kPairSmem, stream>>>(p, maps);
   record_launch(report, K_MATMUL_PAIR, grid, kTensorThreads, kPairSmem);
-  return check_cuda(cudaGetLastError(), "matmul_pair_kernel launch");
+  return launch_after_pack(kernel, grid, kPairSmem, p, maps, stream);
 }
 
 // Pairs of SMs where their tiles of 256 x 256 keep all SMs busy twice over and few
@@ -295,12 +309,11 @@ int launch_kind(int kind, int dtype, const MatmulArgs &p, const DeviceProps &dev
   return launch_tensor<OffT, MATMUL_GRAD_WEIGHTS>(p, dev, stream, report);
 }
 
-int pack(const void *from, void *to, int64_t rows, int64_t cols, int64_t pitch, const DeviceProps &dev,
-         cudaStream_t stream, rg_report *report) {
+int pack(const PackArgs &left, const PackArgs &right, const DeviceProps &dev, cudaStream_t stream, rg_report *report) {
+  const int64_t rows = left.rows + right.rows;
   if (rows == 0) return RG_OK;
   const dim3 grid(static_cast<unsigned>(std::min(ceil_div(rows, 8), static_cast<int64_t>(dev.sm_count) * 8)), 1, 1);
-  matmul_pack_kernel<<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16 *>(from),
-                                               static_cast<__nv_bfloat16 *>(to), rows, cols, pitch);
+  matmul_pack_kernel<<<grid, 256, 0, stream>>>(left, right);
   record_launch(report, K_MATMUL_PACK, grid, 256, 0);
   return check_cuda(cudaGetLastError(), "matmul_pack_kernel launch");
 }
@@ -375,15 +388,21 @@ int rg_matmul(int kind, int dtype, int index_dtype, int64_t k, int64_t m, int64_
   p.splits = s.splits;
   p.parts = s.splits > 1 ? reinterpret_cast<float *>(static_cast<char *>(workspace) + s.parts_at) : nullptr;
   p.status = static_cast<unsigned long long *>(workspace);
+  p.packed = s.pack_left || s.pack_right;
   char *scratch = static_cast<char *>(workspace);
-  if (s.pack_left) {
-    p.left = scratch + s.left_at;
-    status = pack(left, scratch + s.left_at, s.left_rows, s.left_cols, s.left_pitch, dev, on, report);
-    if (status) return status;
-  }
-  if (s.pack_right) {
-    p.right = scratch + s.right_at;
-    status = pack(right, scratch + s.right_at, s.right_rows, s.right_cols, s.right_pitch, dev, on, report);
+  if (s.pack_left || s.pack_right) {
+    PackArgs packed[2] = {};
+    if (s.pack_left) {
+      p.left = scratch + s.left_at;
+      packed[0] = {static_cast<const __nv_bfloat16 *>(left), reinterpret_cast<__nv_bfloat16 *>(scratch + s.left_at),
+                   s.left_rows, s.left_cols, s.left_pitch};
+    }
+    if (s.pack_right) {
+      p.right = scratch + s.right_at;
+      packed[1] = {static_cast<const __nv_bfloat16 *>(right), reinterpret_cast<__nv_bfloat16 *>(scratch + s.right_at),
+                   s.right_rows, s.right_cols, s.right_pitch};
+    }
+    status = pack(packed[0], packed[1], dev, on, report);
     if (status) return status;
   }
   status = index_dtype == RG_INDEX_I32 ? launch_kind<int32_t>(kind, dtype, p, dev, on, report)

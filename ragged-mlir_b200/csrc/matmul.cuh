@@ -33,6 +33,7 @@ struct MatmulArgs {
   int splits;
   float *parts;
   unsigned long long *status;
+  bool packed;               // a pack launch comes right before
 };
 
 // One output tile: rows [row, row_end) of the output (of segment `seg` for the

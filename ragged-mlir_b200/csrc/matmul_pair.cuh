@@ -155,6 +155,8 @@ matmul_pair_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps) 
 
   if (warp == 0) {
     // ------------------------------------------------------------ copies --
+    grid_dependency_wait();  // on operands that are being packed
+    fence_proxy_async_global();
     RingPlace<STAGES> at{0, 1};
     bool going = true;
     for (int64_t index = first; going && walk.find(p, index, t); index += stride) {
