@@ -15,6 +15,7 @@ from __future__ import annotations
 from contextlib import nullcontext
 from dataclasses import replace
 import importlib
+import sys
 import threading
 import time
 from typing import Any
@@ -39,6 +40,9 @@ _device_l2_mib: dict[int, float | None] = {}
 
 
 def _torch():
+    loaded = sys.modules.get("torch")  # (import_module costs most of a microsecond a call)
+    if loaded is not None:
+        return loaded
     try:
         return importlib.import_module("torch")
     except ImportError as exc:

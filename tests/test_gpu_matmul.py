@@ -483,3 +483,75 @@ def test_a_run_of_the_operators_together(cuda):
     sums = torch.zeros((24, k), dtype=torch.float64, device="cuda")
     sums.index_add_(0, torch.repeat_interleave(torch.arange(24, device="cuda"), by_sequence.diff()), y.detach().double())
     near(pooled, sums)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_chained_calls_of_unaligned_rows(cuda, captured):
+    """Each call packs what the one before it wrote, back to back and in a
+    replayed graph: the same bits as with a synchronisation after each."""
+    torch = cuda
+    torch.manual_seed(5)
+    offsets = torch.tensor([0, 700, 701, 701, 1500, 2111], device="cuda")
+    x = torch.randn(2111, 77, device="cuda").bfloat16()
+    widths = [77, 131, 64, 201, 77]
+    weights = [(torch.randn(5, k, m, device="cuda") / k ** 0.5).bfloat16() for k, m in zip(widths, widths[1:])]
+    rows = [torch.empty(2111, m, device="cuda", dtype=torch.bfloat16) for m in widths[1:]]
+    grads = [torch.empty_like(w) for w in weights]
+    programs = [matmul_program("bf16", k, m) for k, m in zip(widths, widths[1:])]
+
+    def chain(wait):
+        source = x
+        for program, w, out, grad in zip(programs, weights, rows, grads):
+            program.run(source, w, offsets, out)
+            if wait:
+                torch.cuda.synchronize()
+            program.run_backward(source, w, offsets, out, grad_weights=grad)
+            if wait:
+                torch.cuda.synchronize()
+            source = out
+
+    results = lambda: [t.clone() for t in rows + grads]  # noqa: E731
+    graph = None
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        chain(True)
+        with torch.cuda.graph(graph):
+            chain(False)
+    for turn in range(4):
+        x.copy_(torch.randn(2111, 77, device="cuda").bfloat16())
+        chain(True)
+        want = results()
+        for t in rows + grads:
+            t.fill_(SENTINEL)
+        if graph is not None:
+            graph.replay()
+        else:
+            chain(False)
+        torch.cuda.synchronize()
+        for got, expected in zip(results(), want):
+            assert torch.equal(got, expected), turn
+
+
+def test_calls_on_two_streams_at_once(cuda):
+    """One program from two streams: scratch is a call's own."""
+    torch = cuda
+    torch.manual_seed(6)
+    offsets = torch.tensor([0, 900, 1700, 3001], device="cuda")
+    program = matmul_program("bf16", 75, 131)
+    cases = [(torch.randn(3001, 75, device="cuda").bfloat16(), torch.randn(3, 75, 131, device="cuda").bfloat16())
+             for _ in range(2)]
+    want = []
+    for x, w in cases:
+        out = torch.empty(3001, 131, device="cuda", dtype=torch.bfloat16)
+        program.run(x, w, offsets, out)
+        torch.cuda.synchronize()
+        want.append(out)
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs = [[torch.empty_like(want[0]) for _ in range(10)] for _ in cases]
+    torch.cuda.synchronize()
+    for i in range(10):
+        for s, stream in enumerate(streams):
+            program.run(*cases[s], offsets, outs[s][i], stream)
+    torch.cuda.synchronize()
+    for s in range(2):
+        assert all(torch.equal(out, want[s]) for out in outs[s])

@@ -484,3 +484,39 @@ def test_offsets_beyond_32_bits_of_elements(cuda):
     assert torch.equal(tail, torch.tensor([[0.0], [1.0], [1.0], [2.0]], device="cuda").expand(4, d))
     assert torch.equal(final, torch.tensor([[1.0], [2.0]], device="cuda").expand(2, d))
     assert not out[:-3].any().item()
+
+
+def test_chained_calls_and_two_streams_at_once(cuda):
+    """Calls whose launches may overlap, back to back on the rows before and
+    from two streams: the same bits as with a synchronisation after each."""
+    torch = cuda
+    torch.manual_seed(7)
+    offsets = torch.tensor([0, 900, 901, 5000, 20_011], device="cuda")
+    program = scan_program("bf16", 200)
+    gates = torch.rand(20_011, 200, device="cuda").bfloat16()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    first = [torch.randn(20_011, 200, device="cuda").bfloat16() for _ in streams]
+    rows = [[torch.empty_like(x) for _ in range(6)] for x in first]
+
+    def chain(s, wait):
+        source = first[s]
+        for out in rows[s]:
+            program.run(source, gates, offsets, out, streams[s])
+            if wait:
+                torch.cuda.synchronize()
+            source = out
+
+    torch.cuda.synchronize()
+    for s in range(2):
+        chain(s, True)
+    want = [[t.clone() for t in row] for row in rows]
+    for _ in range(5):
+        for row in rows:
+            for t in row:
+                t.fill_(SENTINEL)
+        torch.cuda.synchronize()
+        for s in range(2):
+            chain(s, False)
+        torch.cuda.synchronize()
+        for s in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(rows[s], want[s]))
