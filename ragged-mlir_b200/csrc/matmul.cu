@@ -20,6 +20,7 @@ struct MatmulShape {
   int64_t left_rows, left_cols;      // operands as matrices
   int64_t right_rows, right_cols;
   int64_t left_pitch, right_pitch;   // after packing
+  bool few;                          // the few-rows kernel computes it
   bool pack_left, pack_right;
   int splits;                        // of the segments' rows, in the weights kind
   int64_t left_at, right_at, parts_at, bytes;  // workspace
@@ -66,6 +67,8 @@ bool takes_tma(const void *p, int64_t cols) { return cols % 8 == 0 && aligned(p,
 // to two rows a segment, 256 in all.  There 16 rows 20.5 us, 26.6 with tensor-core
 // tiles; 32 rows 24.6 and 28.7; 48 rows 30.7 and 28.7; 512 rows in 256 segments of
 // 512 x 512 43 and 37; 512 rows in one segment 94 and 14.
+// (Decided once, on the caller's operands: a copy of them is aligned and has
+// another pitch.)
 bool takes_few(int kind, int dtype, int64_t m, int64_t n, int64_t b, const void *right) {
   if (kind != MATMUL_FORWARD || m % (16 / elem_bytes(dtype)) || !aligned(right, 16)) return false;
   return dtype == RG_DTYPE_F32 ? n <= 16 * b : n <= 2 * b && n <= 256;
@@ -88,7 +91,8 @@ MatmulShape make_shape(int kind, int dtype, int64_t k, int64_t m, int64_t n, int
     s.parts_at = status_bytes();
     s.bytes = align256(s.parts_at + s.splits * b * k * m * 4);
   }
-  if (dtype == RG_DTYPE_F32 || takes_few(kind, dtype, m, n, b, right)) return s;
+  s.few = takes_few(kind, dtype, m, n, b, right);
+  if (dtype == RG_DTYPE_F32 || s.few) return s;
   if (!s.bytes) s.bytes = status_bytes();
   if (!takes_tma(left, s.left_cols)) {
     s.pack_left = true;
@@ -293,9 +297,9 @@ int launch_few(MatmulArgs p, const DeviceProps &dev, cudaStream_t stream, rg_rep
 }
 
 template <typename OffT>
-int launch_kind(int kind, int dtype, const MatmulArgs &p, const DeviceProps &dev, cudaStream_t stream,
+int launch_kind(int kind, int dtype, bool few, const MatmulArgs &p, const DeviceProps &dev, cudaStream_t stream,
                 rg_report *report) {
-  if (takes_few(kind, dtype, p.m, p.n, p.b, p.right)) {
+  if (few) {
     if (dtype == RG_DTYPE_F32) return launch_few<float, OffT>(p, dev, stream, report);
     return launch_few<__nv_bfloat16, OffT>(p, dev, stream, report);
   }
@@ -364,7 +368,7 @@ int rg_matmul(int kind, int dtype, int index_dtype, int64_t k, int64_t m, int64_
     report->workspace_bytes = s.bytes;
     report->d_vector = 1;
     report->d_tile = 1;
-    report->status_offset = dtype == RG_DTYPE_BF16 && s.bytes ? 0 : -1;
+    report->status_offset = dtype == RG_DTYPE_BF16 && !s.few ? 0 : -1;
   }
   if (s.bytes) {
     if (!workspace || workspace_bytes < s.bytes) return fail(RG_ERR_WORKSPACE, "workspace missing or too small");
@@ -405,8 +409,8 @@ int rg_matmul(int kind, int dtype, int index_dtype, int64_t k, int64_t m, int64_
     status = pack(packed[0], packed[1], dev, on, report);
     if (status) return status;
   }
-  status = index_dtype == RG_INDEX_I32 ? launch_kind<int32_t>(kind, dtype, p, dev, on, report)
-                                       : launch_kind<int64_t>(kind, dtype, p, dev, on, report);
+  status = index_dtype == RG_INDEX_I32 ? launch_kind<int32_t>(kind, dtype, s.few, p, dev, on, report)
+                                       : launch_kind<int64_t>(kind, dtype, s.few, p, dev, on, report);
   if (status || s.splits == 1) return status;
   const int64_t count = b * k * m;
   const dim3 grid(static_cast<unsigned>(std::min(ceil_div(count, 256), static_cast<int64_t>(dev.sm_count) * 8)), 1, 1);

@@ -39,7 +39,7 @@ __device__ __forceinline__ void few_tile(const MatmulArgs &p, const MatmulTile &
   const int64_t col = static_cast<int64_t>(t.col_tile) * COLS + lane * VEC;
   const bool live = col < p.cols;
   const int rows = static_cast<int>(t.row_end - t.row);
-  const T *values = static_cast<const T *>(p.left) + t.row * p.k;
+  const T *values = static_cast<const T *>(p.left) + t.row * p.left_pitch;
   const T *weights = static_cast<const T *>(p.right) + t.seg * p.k * p.m + (live ? col : 0);
   float sum[ROWS][VEC];
 #pragma unroll
@@ -68,7 +68,7 @@ __device__ __forceinline__ void few_tile(const MatmulArgs &p, const MatmulTile &
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
         float x[1] = {0.0f};
-        if (r < rows) VecIO<T, 1>::load(values + r * p.k + k0 + k, x);
+        if (r < rows) VecIO<T, 1>::load(values + r * p.left_pitch + k0 + k, x);
         x_smem[k * ROWS + r] = x[0];
       }
     }

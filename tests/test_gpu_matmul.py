@@ -555,3 +555,32 @@ def test_calls_on_two_streams_at_once(cuda):
     torch.cuda.synchronize()
     for s in range(2):
         assert all(torch.equal(out, want[s]) for out in outs[s])
+
+
+def dirty_allocator(torch, *byte_counts):
+    """Leaves NaN (and, as 64-bit words, nonzero values) in the memory that the
+    next allocations of these sizes get."""
+    for count in byte_counts:
+        blocks = [torch.full((-(-count // 4),), float("nan"), device="cuda") for _ in range(3)]
+        torch.cuda.synchronize()
+        del blocks
+
+
+@pytest.mark.parametrize("mode", ["validated", "checked"])
+@pytest.mark.parametrize("shift", range(1, 8))
+@pytest.mark.parametrize("k,m", [(7, 64), (33, 8), (100, 64), (64, 40), (1100, 136)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_few_rows_with_weights_inside_a_buffer(cuda, dtype, k, m, shift, mode):
+    """Calls of few rows a segment whose weights start anywhere in a flat buffer
+    of parameters; the columns fill 16-byte vectors, the rows of values do not."""
+    torch = cuda
+    program = matmul_program(dtype, k, m)
+    for lengths in ([1, 1, 1, 1], [2, 0, 3, 1], [0, 7, 0, 0, 0, 1]):
+        case = make_case(lengths, k, m, dtype, seed=shift)
+        t = device(torch, case, dtype)
+        weights = torch.zeros(t["weights"].numel() + shift, dtype=t["weights"].dtype, device="cuda")[shift:]
+        weights = weights.view_as(t["weights"]).copy_(t["weights"])
+        out = torch.full_like(t["grad_out"], SENTINEL)
+        dirty_allocator(torch, 8192 + 2 * (k + 8) * (len(out) + len(lengths) * (m + 8)))
+        program.run(t["values"], weights, t["offsets"], out, mode=mode)
+        check(case, dict(out=host(out)), dtype)
