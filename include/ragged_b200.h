@@ -285,8 +285,10 @@ int rg_run_noalloc(int op, int dtype, int index_dtype, int64_t d, int64_t n, int
  * the gradients of out and final_state (NULL: zero) and writes the gradients
  * that are not NULL; grad_initial (f32 [B, D]) needs `initial`.  Written
  * tensors overlap nothing.  Rows behind offsets[B] are neither read nor written
- * (a caller may keep N fixed).  Results do not depend on timing: equal inputs
- * give equal bits. */
+ * (a caller may keep N fixed), unless RG_CLEAR_REST is or'ed to dtype: then
+ * those rows of out, grad_values and grad_gates are set to zero.  Results do not
+ * depend on timing: equal inputs give equal bits. */
+enum rg_rest { RG_CLEAR_REST = 256 }; /* or'ed to the dtype of rg_scan, rg_scan_backward and rg_matmul */
 int rg_scan_workspace_bytes(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, int64_t *bytes);
 int rg_scan(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, const void *values, const void *gates,
             const void *offsets, const float *initial, void *out, float *final_state, float *carries,
@@ -308,7 +310,8 @@ int rg_scan_backward(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b
  *   RG_MATMUL_GRAD_WEIGHTS        values [N, K]     grad_out [N, M]  [B, K, M]
  * Sums are f32, rounded once.  A segment without rows has zeros for the
  * gradient of its weights; its weights are not read.  out overlaps nothing.
- * Rows behind offsets[B] reach no result and are not written.
+ * Rows behind offsets[B] reach no result and are not written, or with
+ * RG_CLEAR_REST or'ed to dtype are set to zero.
  * bf16 runs on the tensor cores, f32 in f32 arithmetic.
  *
  * rg_matmul_workspace_bytes: scratch of a call (256-byte aligned; 0: none),

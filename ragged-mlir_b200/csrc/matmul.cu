@@ -343,6 +343,8 @@ int rg_matmul(int kind, int dtype, int index_dtype, int64_t k, int64_t m, int64_
               const void *right, const void *offsets, void *out, void *workspace, int64_t workspace_bytes,
               void *stream, rg_report *report) {
   clear_report(report);
+  const bool clear_rest = dtype & RG_CLEAR_REST;
+  dtype &= ~RG_CLEAR_REST;
   int status = check_shape(kind, dtype, index_dtype, k, m, n, b);
   if (status) return status;
   const MatmulShape s = make_shape(kind, dtype, k, m, n, b, left, right);
@@ -393,6 +395,7 @@ int rg_matmul(int kind, int dtype, int index_dtype, int64_t k, int64_t m, int64_
   p.parts = s.splits > 1 ? reinterpret_cast<float *>(static_cast<char *>(workspace) + s.parts_at) : nullptr;
   p.status = static_cast<unsigned long long *>(workspace);
   p.packed = s.pack_left || s.pack_right;
+  p.clear_rest = clear_rest && kind != MATMUL_GRAD_WEIGHTS;
   char *scratch = static_cast<char *>(workspace);
   if (s.pack_left || s.pack_right) {
     PackArgs packed[2] = {};

@@ -34,6 +34,7 @@ struct MatmulArgs {
   float *parts;
   unsigned long long *status;
   bool packed;               // a pack launch comes right before
+  bool clear_rest;           // rows of the output behind the last segment: set to zero, else left alone
 };
 
 // One output tile: rows [row, row_end) of the output (of segment `seg` for the
@@ -107,6 +108,25 @@ struct MatmulWalk {
     }
   }
 };
+
+// Rows of the output behind the last segment: zeros, by `count` threads of which
+// this is number `at`.  They are one range of memory, written in 16-byte pieces.
+template <typename T, typename OffT>
+__device__ __forceinline__ void matmul_clear_rest(const MatmulArgs &p, int64_t at, int64_t count) {
+  if (!p.clear_rest) return;
+  const int64_t used = min(max(static_cast<int64_t>(static_cast<const OffT *>(p.offsets)[p.b]), int64_t{0}), p.n);
+  T *from = static_cast<T *>(p.out) + used * p.out_pitch, *to = static_cast<T *>(p.out) + p.n * p.out_pitch;
+  const int64_t elements = to - from;
+  constexpr int kPiece = 16 / static_cast<int>(sizeof(T));
+  const int64_t head = min(static_cast<int64_t>((16 - (reinterpret_cast<uintptr_t>(from) & 15)) & 15) / int64_t{sizeof(T)},
+                           elements);
+  const int64_t pieces = (elements - head) / kPiece;
+  uint4 *body = reinterpret_cast<uint4 *>(from + head);
+  for (int64_t i = at; i < pieces; i += count) body[i] = uint4{0, 0, 0, 0};
+  const T zero = static_cast<T>(0.0f);
+  if (at < head) from[at] = zero;
+  if (at < elements - head - pieces * kPiece) to[-1 - at] = zero;
+}
 
 // The parts' sums, in order, rounded once.
 template <typename T>

@@ -129,6 +129,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) matmul_few_kernel(const Matmul
     else
       few_tile<T, 8>(p, t, few_smem);
   }
+  matmul_clear_rest<T, OffT>(p, int64_t{blockIdx.x} * kFewThreads + threadIdx.x, int64_t{gridDim.x} * kFewThreads);
 }
 
 }  // namespace rgb

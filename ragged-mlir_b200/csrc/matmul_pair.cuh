@@ -316,6 +316,10 @@ matmul_pair_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps) 
         if (acc == 0) acc_phase ^= 1;
       }
     }
+    if constexpr (KIND != MATMUL_GRAD_WEIGHTS)
+      matmul_clear_rest<__nv_bfloat16, OffT>(
+          p, int64_t{blockIdx.x} * kStoreThreads + threadIdx.x - (kTensorThreads - kStoreThreads),
+          int64_t{gridDim.x} * kStoreThreads);
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();

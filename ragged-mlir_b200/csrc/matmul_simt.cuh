@@ -166,6 +166,8 @@ __global__ void __launch_bounds__(kSimtThreads, TILE == 128 ? 2 : 3) matmul_simt
     cp_async_wait<0>();
     __syncthreads();  // the last slice has been read
   }
+  if constexpr (KIND != MATMUL_GRAD_WEIGHTS)
+    matmul_clear_rest<float, OffT>(p, int64_t{blockIdx.x} * kSimtThreads + threadIdx.x, int64_t{gridDim.x} * kSimtThreads);
 }
 
 }  // namespace rgb

@@ -37,6 +37,7 @@
 namespace rgb {
 
 constexpr int kTensorThreads = 192;  // warps: copies, products, 4 x stores
+constexpr int kStoreThreads = 128;
 constexpr int kTensorRows = 128;
 constexpr int kTensorDepth = 64;     // of a stage: 128 bytes of bf16
 constexpr int kLeftBytes = kTensorRows * 128;
@@ -473,6 +474,10 @@ matmul_tensor_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps
         if (acc == 0) acc_phase ^= 1;
       }
     }
+    if constexpr (KIND != MATMUL_GRAD_WEIGHTS)
+      matmul_clear_rest<__nv_bfloat16, OffT>(
+          p, int64_t{blockIdx.x} * kStoreThreads + threadIdx.x - (kTensorThreads - kStoreThreads),
+          int64_t{gridDim.x} * kStoreThreads);
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();

@@ -130,6 +130,13 @@ int launch_vec(int dtype, const ScanArgs &p, const ScanShape &s, const DevicePro
   return launch<__nv_bfloat16, OffT, 1, BACKWARD>(p, s, dev, stream, report);
 }
 
+// Takes RG_CLEAR_REST out of a dtype.
+bool take_clear_rest(int &dtype) {
+  const bool clear = dtype & RG_CLEAR_REST;
+  dtype &= ~RG_CLEAR_REST;
+  return clear;
+}
+
 template <bool BACKWARD>
 int run_scan(int dtype, int index_dtype, int align, ScanArgs &p, void *workspace, int64_t workspace_bytes,
              cudaStream_t stream, rg_report *report) {
@@ -184,6 +191,7 @@ int rg_scan(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, const v
             const void *offsets, const float *initial, void *out, float *final_state, float *carries, void *workspace,
             int64_t workspace_bytes, void *stream, rg_report *report) {
   clear_report(report);
+  const bool clear_rest = take_clear_rest(dtype);
   int status = check_shape(dtype, index_dtype, d, n, b);
   if (status) return status;
   if (b == 0) return RG_OK;
@@ -208,6 +216,7 @@ int rg_scan(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b, const v
   p.n = n;
   p.d = d;
   p.b = b;
+  p.clear_rest = clear_rest;
   p.carries = carries;
   p.out = out;
   p.final_state = final_state;
@@ -220,6 +229,7 @@ int rg_scan_backward(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b
                      float *grad_initial, void *workspace, int64_t workspace_bytes, void *stream,
                      rg_report *report) {
   clear_report(report);
+  const bool clear_rest = take_clear_rest(dtype);
   int status = check_shape(dtype, index_dtype, d, n, b);
   if (status) return status;
   if (b == 0) return RG_OK;
@@ -248,6 +258,7 @@ int rg_scan_backward(int dtype, int index_dtype, int64_t d, int64_t n, int64_t b
   p.n = n;
   p.d = d;
   p.b = b;
+  p.clear_rest = clear_rest;
   p.carries = const_cast<float *>(carries);
   p.grad_out = grad_out;
   p.grad_final = grad_final;

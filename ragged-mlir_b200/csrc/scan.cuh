@@ -75,6 +75,7 @@ struct ScanArgs {
   int64_t slabs;       // slabs that hold rows
   int64_t blocks;      // slabs launched (more than `slabs` where many segments are empty)
   int64_t per_block;   // segments whose emptiness a slab looks at
+  bool clear_rest;     // rows of the results behind the last segment: set to zero, else left alone
   float *carries;      // [N / 8, D] state before every 8th row (written by forward, read by backward)
   // forward
   void *out;
@@ -652,6 +653,19 @@ __global__ void __launch_bounds__(kScanThreads, BACKWARD ? 2 : 3) scan_walk_kern
     // Segments without rows: the state passes through (as does its gradient).
     float *to = BACKWARD ? p.grad_initial : p.final_state;
     w.go(block, tile);
+    if (block < p.slabs && p.clear_rest && w.col_ok) {
+      const int stop = static_cast<int>(min(p.n - w.row0, static_cast<int64_t>(w.base + p.lane_rows)));
+      const float zero[VEC] = {};
+      for (int i = max(w.base, w.limit); i < stop; ++i) {
+        const int64_t at = (w.row0 + i) * p.d + w.col;
+        if constexpr (BACKWARD) {
+          if (p.grad_values) IO::store(static_cast<T *>(p.grad_values) + at, zero);
+          if (p.grad_gates) IO::store(static_cast<T *>(p.grad_gates) + at, zero);
+        } else {
+          IO::store(static_cast<T *>(p.out) + at, zero);
+        }
+      }
+    }
     if (to && w.col_ok) {
       const int64_t stop = min(p.b, (block + 1) * p.per_block);
       for (int64_t s = block * p.per_block + ((threadIdx.x & 31) >> p.shift); s < stop; s += 32 >> p.shift) {

@@ -28,6 +28,7 @@ FLAG_NO_VECTORIZE = 1
 FLAG_IN_PLACE = 2
 FLAG_NO_POINTWISE_FUSION = 4
 MAX_LAUNCHES = 8
+CLEAR_REST = 256
 PRODUCTS = {"forward": 0, "grad_values": 1, "grad_weights": 2}
 
 # Every symbol include/ragged_b200.h declares.
@@ -353,20 +354,25 @@ def scan_workspace_bytes(dtype: str, index: str, d: int, n: int, b: int) -> int:
     return out.value
 
 
+def _rest(dtype: str, clear_rest: bool) -> int:
+    return DTYPES[dtype] | CLEAR_REST if clear_rest else DTYPES[dtype]
+
+
 def scan(dtype: str, index: str, d: int, n: int, b: int, pointers: tuple, workspace_ptr: int, workspace_bytes: int,
-         stream: int, report: Report | None) -> None:
-    """``pointers``: values, gates, offsets, initial, out, final, carries (0: none)."""
-    status = library().rg_scan(DTYPES[dtype], INDEX[index], d, n, b, *pointers, workspace_ptr, workspace_bytes, stream,
+         stream: int, report: Report | None, clear_rest: bool = False) -> None:
+    """``pointers``: values, gates, offsets, initial, out, final, carries (0: none).
+    ``clear_rest``: rows behind the last segment are set to zero."""
+    status = library().rg_scan(_rest(dtype, clear_rest), INDEX[index], d, n, b, *pointers, workspace_ptr, workspace_bytes, stream,
                                report)
     if status:
         raise_for(status, "rg_scan")
 
 
 def scan_backward(dtype: str, index: str, d: int, n: int, b: int, pointers: tuple, workspace_ptr: int,
-                  workspace_bytes: int, stream: int, report: Report | None) -> None:
+                  workspace_bytes: int, stream: int, report: Report | None, clear_rest: bool = False) -> None:
     """``pointers``: values, gates, offsets, initial, carries, grad_out,
     grad_final, grad_values, grad_gates, grad_initial (0: none)."""
-    status = library().rg_scan_backward(DTYPES[dtype], INDEX[index], d, n, b, *pointers, workspace_ptr,
+    status = library().rg_scan_backward(_rest(dtype, clear_rest), INDEX[index], d, n, b, *pointers, workspace_ptr,
                                         workspace_bytes, stream, report)
     if status:
         raise_for(status, "rg_scan_backward")
@@ -383,8 +389,8 @@ def matmul_workspace_bytes(kind: str, dtype: str, index: str, k: int, m: int, n:
 
 def matmul(kind: str, dtype: str, index: str, k: int, m: int, n: int, b: int, left_ptr: int, right_ptr: int,
            offsets_ptr: int, out_ptr: int, workspace_ptr: int, workspace_bytes: int, stream: int,
-           report: Report | None) -> None:
-    status = library().rg_matmul(PRODUCTS[kind], DTYPES[dtype], INDEX[index], k, m, n, b, left_ptr, right_ptr,
+           report: Report | None, clear_rest: bool = False) -> None:
+    status = library().rg_matmul(PRODUCTS[kind], _rest(dtype, clear_rest), INDEX[index], k, m, n, b, left_ptr, right_ptr,
                                  offsets_ptr, out_ptr, workspace_ptr, workspace_bytes, stream, report)
     if status:
         raise_for(status, "rg_matmul")

@@ -8,9 +8,10 @@ unless ``stream`` is given, no synchronisation in validated mode, and
 ``mode="checked"`` to validate the offsets on the device first.  ``run``
 records no gradient; ``run_backward`` computes the gradients of a call, and
 ``torch_adapter.segment_scan`` / ``segment_matmul`` put both behind autograd.
-Rows behind the last offset are left as they are and reach no result, so a
-caller of ``run`` may keep N fixed while the offsets change (autograd gives no
-gradients for them: there offsets end at N, as everywhere else).
+Rows behind the last offset reach no result, so N may stay fixed while the
+offsets change (in validated mode; checked mode asks for offsets that end at N).
+``run`` and ``run_backward`` leave those rows of what they write as they are;
+the functions of ``torch_adapter``, which allocate their results, give zeros.
 
 Neither operation exists in the reference, whose programs end at sums, maxima
 and softmaxes of packed rows.
@@ -248,7 +249,7 @@ class CompiledScan(_LayerProgram):
         outputs overlap nothing."""
         return self._run(values, gates, offsets, out, initial, final, carries, stream, mode, True)
 
-    def _run(self, values, gates, offsets, out, initial, final, carries, stream, mode, gradless):
+    def _run(self, values, gates, offsets, out, initial, final, carries, stream, mode, gradless, clear_rest=False):
         torch = _torch()
         spec, d = self.spec, self.spec.feature_dim
         b, n = self._segments(torch, offsets), self._rows(values, torch)
@@ -265,7 +266,7 @@ class CompiledScan(_LayerProgram):
                     _address(final), _address(carries))
 
         def call(scratch, nbytes, on, report):
-            _native.scan(spec.dtype, spec.offsets_dtype, d, n, b, pointers, scratch, nbytes, on, report)
+            _native.scan(spec.dtype, spec.offsets_dtype, d, n, b, pointers, scratch, nbytes, on, report, clear_rest)
 
         return self._launch(torch, offsets, n, b, stream, mode, [t[1] for t in tensors] + [offsets],
                             (((False, n, b) + _alignment(pointers), self._scratch(n, b), call),))
@@ -276,6 +277,11 @@ class CompiledScan(_LayerProgram):
         outputs (``grad_final`` f32 [B, D]; None: zero).  Writes those of
         ``grad_values``, ``grad_gates`` [N, D] and ``grad_initial`` (f32
         [B, D], with ``initial``) that are given."""
+        return self._run_backward(values, gates, offsets, carries, grad_out, stream, initial, grad_final, grad_values,
+                                  grad_gates, grad_initial)
+
+    def _run_backward(self, values, gates, offsets, carries, grad_out, stream, initial, grad_final, grad_values,
+                      grad_gates, grad_initial, clear_rest=False):
         torch = _torch()
         spec, d = self.spec, self.spec.feature_dim
         b, n = self._segments(torch, offsets), self._rows(values, torch)
@@ -290,10 +296,10 @@ class CompiledScan(_LayerProgram):
         tensors = rows[:4] + [row for row in rows[4:] if row[1] is not None]
         self._tensors(torch, tensors, offsets, "validated", False)
         return self._gradients(torch, values, gates, offsets, carries, grad_out, stream, initial, grad_final,
-                               grad_values, grad_gates, grad_initial)
+                               grad_values, grad_gates, grad_initial, clear_rest)
 
     def _gradients(self, torch, values, gates, offsets, carries, grad_out, stream, initial, grad_final, grad_values,
-                   grad_gates, grad_initial):
+                   grad_gates, grad_initial, clear_rest):
         """``run_backward`` of tensors that are known to fit."""
         spec, d, n, b = self.spec, self.spec.feature_dim, values.shape[0], offsets.numel() - 1
         pointers = (values.data_ptr(), gates.data_ptr(), offsets.data_ptr(), _address(initial), carries.data_ptr(),
@@ -301,7 +307,8 @@ class CompiledScan(_LayerProgram):
                     _address(grad_initial))
 
         def call(scratch, nbytes, on, report):
-            _native.scan_backward(spec.dtype, spec.offsets_dtype, d, n, b, pointers, scratch, nbytes, on, report)
+            _native.scan_backward(spec.dtype, spec.offsets_dtype, d, n, b, pointers, scratch, nbytes, on, report,
+                                  clear_rest)
 
         used = [t for t in (values, gates, offsets, carries, grad_out, initial, grad_final, grad_values, grad_gates,
                             grad_initial) if t is not None] if stream is not None else ()
@@ -317,7 +324,7 @@ class CompiledMatmul(_LayerProgram):
     def _status_words(self, launch) -> int:
         return launch.grids[-1][0]  # one for each CTA
 
-    def _product(self, kind, left, right, offsets, out, n, b):
+    def _product(self, kind, left, right, offsets, out, n, b, clear_rest):
         """(key, scratch bytes, call) of one product."""
         spec = self.spec
         shape = (kind, spec.dtype, spec.offsets_dtype, spec.feature_dim, spec.out_dim, n, b)
@@ -325,7 +332,8 @@ class CompiledMatmul(_LayerProgram):
         pointers = (left, right, offsets.data_ptr(), out.data_ptr())
         key = (kind, n, b) + _alignment(pointers)
         nbytes = self._cached(key, lambda: _native.matmul_workspace_bytes(*shape, left, right))
-        return key, nbytes, lambda scratch, size, on, report: _native.matmul(*shape, *pointers, scratch, size, on, report)
+        return key, nbytes, lambda scratch, size, on, report: _native.matmul(*shape, *pointers, scratch, size, on,
+                                                                             report, clear_rest)
 
     def run(self, values, weights, offsets, out, stream=None, mode: str = "validated") -> ExecutionReport:
         """Writes ``out`` [N, out_dim] from ``values`` [N, feature_dim] and
@@ -333,7 +341,7 @@ class CompiledMatmul(_LayerProgram):
         contiguous.  ``out`` overlaps nothing."""
         return self._run(values, weights, offsets, out, stream, mode, True)
 
-    def _run(self, values, weights, offsets, out, stream, mode, gradless):
+    def _run(self, values, weights, offsets, out, stream, mode, gradless, clear_rest=False):
         torch = _torch()
         k, m = self.spec.feature_dim, self.spec.out_dim
         b, n = self._segments(torch, offsets), self._rows(values, torch)
@@ -341,13 +349,16 @@ class CompiledMatmul(_LayerProgram):
         tensors = (("values", values, (n, k), dtype), ("weights", weights, (b, k, m), dtype), ("out", out, (n, m), dtype))
         self._tensors(torch, tensors, offsets, mode, gradless)
         return self._launch(torch, offsets, n, b, stream, mode, (values, weights, offsets, out),
-                            (self._product("forward", values, weights, offsets, out, n, b),))
+                            (self._product("forward", values, weights, offsets, out, n, b, clear_rest),))
 
     def run_backward(self, values, weights, offsets, grad_out, stream=None, *, grad_values=None,
                      grad_weights=None) -> ExecutionReport:
         """Gradients of ``run`` from that of ``out``: those of ``grad_values``
         and ``grad_weights`` that are given (zero for the weights of a segment
         without rows)."""
+        return self._run_backward(values, weights, offsets, grad_out, stream, grad_values, grad_weights)
+
+    def _run_backward(self, values, weights, offsets, grad_out, stream, grad_values, grad_weights, clear_rest=False):
         torch = _torch()
         k, m = self.spec.feature_dim, self.spec.out_dim
         b, n = self._segments(torch, offsets), self._rows(values, torch)
@@ -359,15 +370,15 @@ class CompiledMatmul(_LayerProgram):
         if grad_weights is not None:
             tensors.append(("grad_weights", grad_weights, (b, k, m), dtype))
         self._tensors(torch, tensors, offsets, "validated", False)
-        return self._gradients(torch, values, weights, offsets, grad_out, stream, grad_values, grad_weights)
+        return self._gradients(torch, values, weights, offsets, grad_out, stream, grad_values, grad_weights, clear_rest)
 
-    def _gradients(self, torch, values, weights, offsets, grad_out, stream, grad_values, grad_weights):
+    def _gradients(self, torch, values, weights, offsets, grad_out, stream, grad_values, grad_weights, clear_rest):
         """``run_backward`` of tensors that are known to fit."""
         n, b = values.shape[0], offsets.numel() - 1
         work = []
         if grad_values is not None:
-            work.append(self._product("grad_values", grad_out, weights, offsets, grad_values, n, b))
+            work.append(self._product("grad_values", grad_out, weights, offsets, grad_values, n, b, clear_rest))
         if grad_weights is not None:
-            work.append(self._product("grad_weights", values, grad_out, offsets, grad_weights, n, b))
+            work.append(self._product("grad_weights", values, grad_out, offsets, grad_weights, n, b, False))
         used = [t for t in (values, weights, offsets, grad_out, grad_values, grad_weights) if t is not None]
         return self._launch(torch, offsets, n, b, stream, "validated", used, work)

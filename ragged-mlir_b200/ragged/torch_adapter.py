@@ -204,7 +204,7 @@ def _scan_call(values, gates, offsets, initial, program, mode: str, record: bool
     shapes = _scan_shapes(values, offsets, record)
     out = torch.empty_like(values)
     final, carries = (torch.empty(shape, dtype=torch.float32, device=values.device) for shape in shapes[1:])
-    program._run(values, gates, offsets, out, initial, final, carries if record else None, None, mode, False)
+    program._run(values, gates, offsets, out, initial, final, carries if record else None, None, mode, False, True)
     return out, final, carries
 
 
@@ -219,10 +219,10 @@ def _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad
                                              for t, want in zip((values, values, initial), wanted))
     if known:
         program._gradients(torch, values, gates, offsets, carries, grad_out, None, initial, grad_final, grad_values,
-                           grad_gates, grad_initial)
+                           grad_gates, grad_initial, True)
     else:
-        program.run_backward(values, gates, offsets, carries, grad_out, initial=initial, grad_final=grad_final,
-                             grad_values=grad_values, grad_gates=grad_gates, grad_initial=grad_initial)
+        program._run_backward(values, gates, offsets, carries, grad_out, None, initial, grad_final, grad_values,
+                              grad_gates, grad_initial, True)
     return grad_values, grad_gates, grad_initial
 
 
@@ -295,7 +295,7 @@ def _matmul_call(values, weights, offsets, program, mode: str):
     """The output of segment_matmul, on the GPU."""
     values, weights = _dense(values, weights)
     out = _torch().empty((values.shape[0], program.spec.out_dim), dtype=values.dtype, device=values.device)
-    program._run(values, weights, offsets, out, None, mode, False)
+    program._run(values, weights, offsets, out, None, mode, False, True)
     return out
 
 
@@ -306,9 +306,9 @@ def _matmul_backward_call(values, weights, offsets, grad_out, program, wanted, k
     values, weights, grad_out = _dense(values, weights, grad_out)
     grads = [torch.empty_like(t) if want else None for t, want in zip((values, weights), wanted)]
     if known:
-        program._gradients(torch, values, weights, offsets, grad_out, None, *grads)
+        program._gradients(torch, values, weights, offsets, grad_out, None, *grads, True)
     else:
-        program.run_backward(values, weights, offsets, grad_out, grad_values=grads[0], grad_weights=grads[1])
+        program._run_backward(values, weights, offsets, grad_out, None, *grads, True)
     return grads
 
 
@@ -473,7 +473,8 @@ def segment_softmax(values, offsets, *, program: CompiledProgram, mode: str = "v
 def segment_scan(values, gates, offsets, *, program: CompiledScan, initial=None, mode: str = "validated"):
     """(out [N, D], final f32 [B, D]) of the recurrence out[t] = gates[t] *
     out[t - 1] + values[t] within each segment, differentiable (once) in
-    values, gates and initial.
+    values, gates and initial.  Rows behind the last offset (a padded batch) are
+    zero in out and in the gradients, whatever the inputs hold there.
 
     Under a CUDA graph capture of a backward pass, autograd itself must not
     have an eager graph of the same leaves alive: its accumulation nodes stay
@@ -494,7 +495,8 @@ def segment_scan(values, gates, offsets, *, program: CompiledScan, initial=None,
 
 def segment_matmul(values, weights, offsets, *, program: CompiledMatmul, mode: str = "validated"):
     """[N, out] of values[t] @ weights[s] for the rows t of segment s,
-    differentiable (once) in values and weights.  (On captured backward
+    differentiable (once) in values and weights.  Rows behind the last offset
+    are zero, as are the gradients of those values.  (On captured backward
     passes: see ``segment_scan``.)"""
     torch = _torch()
     _no_tangents(torch, values, weights)

@@ -584,3 +584,40 @@ def test_few_rows_with_weights_inside_a_buffer(cuda, dtype, k, m, shift, mode):
         dirty_allocator(torch, 8192 + 2 * (k + 8) * (len(out) + len(lengths) * (m + 8)))
         program.run(t["values"], weights, t["offsets"], out, mode=mode)
         check(case, dict(out=host(out)), dtype)
+
+
+@pytest.mark.parametrize("route", ["call", "operator"])
+@pytest.mark.parametrize("dtype,k,m,lengths,behind", [
+    ("f32", 40, 72, [3, 0, 9], 20), ("bf16", 40, 72, [3, 0, 9], 20),              # few rows and tiles
+    ("f32", 33, 9, [300, 0, 700, 0], 5), ("bf16", 33, 9, [300, 0, 700, 0], 5),    # rows off 16-byte boundaries
+    ("f32", 16, 8, [1, 0, 1, 2], 60), ("bf16", 16, 8, [1, 0, 0, 0, 0, 0, 0, 0], 13),  # few rows a segment, padded
+    ("f32", 24, 200, [0, 0], 700), ("bf16", 24, 200, [0, 0], 700),                # no rows at all
+    ("bf16", 512, 2048, [4000, 100, 6000], 9000), ("f32", 512, 512, [4000, 100, 3000], 999)])  # wide tiles, pairs
+def test_padded_rows_of_results_are_zero(cuda, dtype, k, m, lengths, behind, route):
+    """Rows behind the last offset, NaN in the inputs: zeros in what the call
+    allocates, in fresh memory that holds NaN, and no gradient of the weights."""
+    torch = cuda
+    from ragged import torch_adapter
+    generator = torch.Generator(device="cuda").manual_seed(behind)
+    offsets = torch.from_numpy(offsets_of(np.asarray(lengths))).to("cuda")
+    used, n, b = sum(lengths), sum(lengths) + behind, len(lengths)
+    kind = torch.float32 if dtype == "f32" else torch.bfloat16
+    rand = lambda *s: torch.randn(s, generator=generator, device="cuda").to(kind)  # noqa: E731
+    values, grad, weights = rand(n, k), rand(n, m), rand(b, k, m)
+    values[used:], grad[used:] = float("nan"), float("nan")
+    program = matmul_program(dtype, k, m)
+    want = dict(out=torch.zeros_like(grad), grad_values=torch.zeros_like(values), grad_weights=torch.empty_like(weights))
+    program.run(values, weights, offsets, want["out"])
+    program.run_backward(values, weights, offsets, grad, grad_values=want["grad_values"],
+                         grad_weights=want["grad_weights"])
+    leaves = [values.requires_grad_(), weights.requires_grad_()]
+    size = kind.itemsize
+    dirty_allocator(torch, n * m * size, n * k * size)
+    if route == "call":
+        out = torch_adapter.segment_matmul(*leaves, offsets, program=program)
+    else:
+        torch_adapter.register_torch_ops()
+        out = torch.ops.ragged_mlir.segment_matmul(*leaves, offsets, torch_adapter.register_program(program))
+    dirty_allocator(torch, n * k * size)
+    gv, gw = torch.autograd.grad(out, leaves, grad)
+    assert torch.equal(out, want["out"]) and torch.equal(gv, want["grad_values"]) and torch.equal(gw, want["grad_weights"])

@@ -520,3 +520,49 @@ def test_chained_calls_and_two_streams_at_once(cuda):
         torch.cuda.synchronize()
         for s in range(2):
             assert all(torch.equal(a, b) for a, b in zip(rows[s], want[s]))
+
+
+@pytest.mark.parametrize("route", ["call", "operator"])
+@pytest.mark.parametrize("initial", [False, True])
+@pytest.mark.parametrize("lengths,behind", [([3, 0, 9], 20), ([300, 0, 700, 0], 5), ([65, 2000, 1], 1500), ([0, 0], 900),
+                                            ([1] * 60, 200), ([64, 64], 64)])
+@pytest.mark.parametrize("dtype,d", [("f32", 12), ("f32", 100), ("bf16", 128), ("bf16", 7)])
+def test_padded_rows_of_results_are_zero(cuda, dtype, d, lengths, behind, initial, route):
+    """Rows behind the last offset, NaN in the inputs: zeros in what the call
+    allocates, in fresh memory that holds NaN; the rest is what run() writes."""
+    torch = cuda
+    from ragged import torch_adapter
+    case = make_case(lengths, d, dtype, initial, seed=behind)
+    t = device(torch, case, dtype, "i64")
+    used = int(case["offsets"][-1])
+    for name in ("values", "gates", "grad_out"):
+        t[name] = torch.cat([t[name], torch.full((behind, d), float("nan"), device="cuda", dtype=t[name].dtype)])
+    program = scan_program(dtype, d)
+    want = {name: torch.zeros_like(t["values"]) for name in ("out", "grad_values", "grad_gates")}
+    want["final"] = torch.empty((len(lengths), d), device="cuda")
+    want["grad_initial"] = torch.empty_like(want["final"]) if initial else None
+    carries = torch.empty((program.carry_rows(used + behind), d), device="cuda")
+    program.run(t["values"], t["gates"], t["offsets"], want["out"], initial=t["initial"], final=want["final"],
+                carries=carries)
+    program.run_backward(t["values"], t["gates"], t["offsets"], carries, t["grad_out"], initial=t["initial"],
+                         grad_final=t["grad_final"], grad_values=want["grad_values"], grad_gates=want["grad_gates"],
+                         grad_initial=want["grad_initial"])
+    names = ["values", "gates"] + (["initial"] if initial else [])
+    leaves = [t[name].requires_grad_() for name in names]
+
+    def dirty():
+        blocks = [torch.full(t["values"].shape, float("nan"), device="cuda", dtype=t["values"].dtype) for _ in range(4)]
+        torch.cuda.synchronize()
+        del blocks
+
+    dirty()
+    if route == "call":
+        out, final = torch_adapter.segment_scan(*leaves[:2], t["offsets"], program=program, initial=t["initial"])
+    else:
+        torch_adapter.register_torch_ops()
+        out, final, _ = torch.ops.ragged_mlir.segment_scan(*leaves[:2], t["offsets"], t["initial"],
+                                                           torch_adapter.register_program(program))
+    dirty()
+    grads = torch.autograd.grad((out, final), leaves, (t["grad_out"], t["grad_final"]))
+    for got, name in zip((out, final, *grads), ("out", "final", "grad_values", "grad_gates", "grad_initial")):
+        assert torch.equal(got, want[name]), name
