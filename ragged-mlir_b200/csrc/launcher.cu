@@ -176,10 +176,22 @@ int make_tensor_map(CUtensorMap *map, const void *base, int rank, const int64_t 
     boxes[i] = static_cast<cuuint32_t>(box[i]);
     if (i + 1 < rank) pitches[i] = static_cast<cuuint64_t>(strides[i] * 2);
   }
-  const CUresult result = reinterpret_cast<Encode>(entry)(
-      map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank), const_cast<void *>(base), sizes, pitches,
-      boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&]() {
+    return reinterpret_cast<Encode>(entry)(
+        map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank), const_cast<void *>(base), sizes, pitches,
+        boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult result = encode();
+  if (result == CUDA_ERROR_INVALID_CONTEXT) {
+    // A thread that has called the runtime for queries alone has no context yet;
+    // setting its device, even to what it is, gives it one.
+    int device = 0;
+    int status = check_cuda(cudaGetDevice(&device), "cudaGetDevice");
+    if (!status) status = check_cuda(cudaSetDevice(device), "cudaSetDevice");
+    if (status) return status;
+    result = encode();
+  }
   if (result != CUDA_SUCCESS) {
     char buffer[96];
     std::snprintf(buffer, sizeof buffer, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(result));

@@ -621,3 +621,53 @@ def test_padded_rows_of_results_are_zero(cuda, dtype, k, m, lengths, behind, rou
     dirty_allocator(torch, n * k * size)
     gv, gw = torch.autograd.grad(out, leaves, grad)
     assert torch.equal(out, want["out"]) and torch.equal(gv, want["grad_values"]) and torch.equal(gw, want["grad_weights"])
+
+
+@pytest.mark.parametrize("call", ["forward", "backward", "autograd"])
+def test_the_first_call_of_a_thread(cuda, call):
+    """A new thread whose first use of the GPU is a product that another thread
+    has made before: a serving thread, or autograd's own."""
+    import threading
+    torch = cuda
+    from ragged import torch_adapter
+    case = make_case([300, 0, 41], 72, 136, "bf16")
+    t = device(torch, case, "bf16")
+    program = matmul_program("bf16", 72, 136)
+    leaves = [t["values"].requires_grad_(), t["weights"].requires_grad_()]
+    grads = [torch.empty_like(x) for x in leaves]
+    out = torch.empty_like(t["grad_out"])
+
+    def forward():
+        with torch.no_grad():
+            program.run(*leaves, t["offsets"], out)
+
+    def backward():
+        program.run_backward(*leaves, t["offsets"], t["grad_out"], grad_values=grads[0], grad_weights=grads[1])
+
+    forward()
+    backward()
+    want = [x.clone() for x in (out, *grads)]
+    graph = torch_adapter.segment_matmul(*leaves, t["offsets"], program=program)
+    for x in (out, *grads):
+        x.fill_(SENTINEL)
+    torch.cuda.synchronize()
+    raised = []
+
+    def work():
+        try:
+            if call == "autograd":
+                grads[:] = torch.autograd.grad(graph, leaves, t["grad_out"])
+            else:
+                (forward if call == "forward" else backward)()
+        except BaseException as error:  # noqa: BLE001 - shown by the assertion below
+            raised.append(error)
+
+    thread = threading.Thread(target=work)
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert not raised, raised
+    if call == "forward":
+        assert torch.equal(out, want[0])
+    else:
+        assert torch.equal(grads[0], want[1]) and torch.equal(grads[1], want[2])
