@@ -5,9 +5,11 @@ matrix product.
 ``MatmulSpec`` a ``CompiledMatmul``.  Both follow ``CompiledProgram.run``: CUDA
 tensors on one device, outputs that the caller allocates, the current stream
 unless ``stream`` is given, no synchronisation in validated mode, and
-``mode="checked"`` to validate the offsets on the device first.  ``run``
-records no gradient; ``run_backward`` computes the gradients of a call, and
-``torch_adapter.segment_scan`` / ``segment_matmul`` put both behind autograd.
+``mode="checked"`` to validate the offsets on the device first and to raise
+where a bounded wait inside a launch gave up.  ``run`` records no gradient;
+``run_backward`` computes the gradients of a call, and
+``torch_adapter.segment_scan`` / ``segment_matmul`` put both behind autograd, the
+gradients in the mode of the call.
 Rows behind the last offset reach no result, so N may stay fixed while the
 offsets change (in validated mode; checked mode asks for offsets that end at N).
 ``run`` and ``run_backward`` leave those rows of what they write as they are;
@@ -271,16 +273,17 @@ class CompiledScan(_LayerProgram):
         return self._launch(torch, offsets, n, b, stream, mode, [t[1] for t in tensors] + [offsets],
                             (((False, n, b) + _alignment(pointers), self._scratch(n, b), call),))
 
-    def run_backward(self, values, gates, offsets, carries, grad_out, stream=None, *, initial=None, grad_final=None,
-                     grad_values=None, grad_gates=None, grad_initial=None) -> ExecutionReport:
+    def run_backward(self, values, gates, offsets, carries, grad_out, stream=None, mode: str = "validated", *,
+                     initial=None, grad_final=None, grad_values=None, grad_gates=None,
+                     grad_initial=None) -> ExecutionReport:
         """Gradients of a ``run`` that recorded ``carries``, from those of its
         outputs (``grad_final`` f32 [B, D]; None: zero).  Writes those of
         ``grad_values``, ``grad_gates`` [N, D] and ``grad_initial`` (f32
         [B, D], with ``initial``) that are given."""
-        return self._run_backward(values, gates, offsets, carries, grad_out, stream, initial, grad_final, grad_values,
-                                  grad_gates, grad_initial)
+        return self._run_backward(values, gates, offsets, carries, grad_out, stream, mode, initial, grad_final,
+                                  grad_values, grad_gates, grad_initial)
 
-    def _run_backward(self, values, gates, offsets, carries, grad_out, stream, initial, grad_final, grad_values,
+    def _run_backward(self, values, gates, offsets, carries, grad_out, stream, mode, initial, grad_final, grad_values,
                       grad_gates, grad_initial, clear_rest=False):
         torch = _torch()
         spec, d = self.spec, self.spec.feature_dim
@@ -294,12 +297,12 @@ class CompiledScan(_LayerProgram):
                 ("grad_values", grad_values, (n, d), dtype), ("grad_gates", grad_gates, (n, d), dtype),
                 ("grad_initial", grad_initial, (b, d), torch.float32)]
         tensors = rows[:4] + [row for row in rows[4:] if row[1] is not None]
-        self._tensors(torch, tensors, offsets, "validated", False)
-        return self._gradients(torch, values, gates, offsets, carries, grad_out, stream, initial, grad_final,
+        self._tensors(torch, tensors, offsets, mode, False)
+        return self._gradients(torch, values, gates, offsets, carries, grad_out, stream, mode, initial, grad_final,
                                grad_values, grad_gates, grad_initial, clear_rest)
 
-    def _gradients(self, torch, values, gates, offsets, carries, grad_out, stream, initial, grad_final, grad_values,
-                   grad_gates, grad_initial, clear_rest):
+    def _gradients(self, torch, values, gates, offsets, carries, grad_out, stream, mode, initial, grad_final,
+                   grad_values, grad_gates, grad_initial, clear_rest):
         """``run_backward`` of tensors that are known to fit."""
         spec, d, n, b = self.spec, self.spec.feature_dim, values.shape[0], offsets.numel() - 1
         pointers = (values.data_ptr(), gates.data_ptr(), offsets.data_ptr(), _address(initial), carries.data_ptr(),
@@ -312,7 +315,7 @@ class CompiledScan(_LayerProgram):
 
         used = [t for t in (values, gates, offsets, carries, grad_out, initial, grad_final, grad_values, grad_gates,
                             grad_initial) if t is not None] if stream is not None else ()
-        return self._launch(torch, offsets, n, b, stream, "validated", used,
+        return self._launch(torch, offsets, n, b, stream, mode, used,
                             (((True, n, b) + _alignment(pointers), self._scratch(n, b), call),))
 
 
@@ -322,7 +325,10 @@ class CompiledMatmul(_LayerProgram):
     kind = MatmulSpec
 
     def _status_words(self, launch) -> int:
-        return launch.grids[-1][0]  # one for each CTA
+        """One for each CTA of the tensor-core launch (before it operands may be
+        packed, after it parts be summed)."""
+        return next(grid[0] for name, grid in zip(launch.names, launch.grids)
+                    if name in ("matmul_tensor", "matmul_pair"))
 
     def _product(self, kind, left, right, offsets, out, n, b, clear_rest):
         """(key, scratch bytes, call) of one product."""
@@ -351,14 +357,15 @@ class CompiledMatmul(_LayerProgram):
         return self._launch(torch, offsets, n, b, stream, mode, (values, weights, offsets, out),
                             (self._product("forward", values, weights, offsets, out, n, b, clear_rest),))
 
-    def run_backward(self, values, weights, offsets, grad_out, stream=None, *, grad_values=None,
-                     grad_weights=None) -> ExecutionReport:
+    def run_backward(self, values, weights, offsets, grad_out, stream=None, mode: str = "validated", *,
+                     grad_values=None, grad_weights=None) -> ExecutionReport:
         """Gradients of ``run`` from that of ``out``: those of ``grad_values``
         and ``grad_weights`` that are given (zero for the weights of a segment
         without rows)."""
-        return self._run_backward(values, weights, offsets, grad_out, stream, grad_values, grad_weights)
+        return self._run_backward(values, weights, offsets, grad_out, stream, mode, grad_values, grad_weights)
 
-    def _run_backward(self, values, weights, offsets, grad_out, stream, grad_values, grad_weights, clear_rest=False):
+    def _run_backward(self, values, weights, offsets, grad_out, stream, mode, grad_values, grad_weights,
+                      clear_rest=False):
         torch = _torch()
         k, m = self.spec.feature_dim, self.spec.out_dim
         b, n = self._segments(torch, offsets), self._rows(values, torch)
@@ -369,10 +376,11 @@ class CompiledMatmul(_LayerProgram):
             tensors.append(("grad_values", grad_values, (n, k), dtype))
         if grad_weights is not None:
             tensors.append(("grad_weights", grad_weights, (b, k, m), dtype))
-        self._tensors(torch, tensors, offsets, "validated", False)
-        return self._gradients(torch, values, weights, offsets, grad_out, stream, grad_values, grad_weights, clear_rest)
+        self._tensors(torch, tensors, offsets, mode, False)
+        return self._gradients(torch, values, weights, offsets, grad_out, stream, mode, grad_values, grad_weights,
+                               clear_rest)
 
-    def _gradients(self, torch, values, weights, offsets, grad_out, stream, grad_values, grad_weights, clear_rest):
+    def _gradients(self, torch, values, weights, offsets, grad_out, stream, mode, grad_values, grad_weights, clear_rest):
         """``run_backward`` of tensors that are known to fit."""
         n, b = values.shape[0], offsets.numel() - 1
         work = []
@@ -381,4 +389,4 @@ class CompiledMatmul(_LayerProgram):
         if grad_weights is not None:
             work.append(self._product("grad_weights", values, grad_out, offsets, grad_weights, n, b, False))
         used = [t for t in (values, weights, offsets, grad_out, grad_values, grad_weights) if t is not None]
-        return self._launch(torch, offsets, n, b, stream, "validated", used, work)
+        return self._launch(torch, offsets, n, b, stream, mode, used, work)

@@ -41,12 +41,14 @@ SCHEMAS = {
     "segment_scan": 'segment_scan(Tensor values, Tensor gates, Tensor offsets, Tensor? initial, str program, '
                     'str mode="validated", bool record=True) -> (Tensor, Tensor, Tensor)',
     "segment_scan_backward": 'segment_scan_backward(Tensor values, Tensor gates, Tensor offsets, Tensor? initial, '
-                             'Tensor carries, Tensor grad_out, Tensor? grad_final, str program) '
+                             'Tensor carries, Tensor grad_out, Tensor? grad_final, str program, '
+                             'str mode="validated") '
                              '-> (Tensor, Tensor, Tensor)',
     "segment_matmul": 'segment_matmul(Tensor values, Tensor weights, Tensor offsets, str program, '
                       'str mode="validated") -> Tensor',
     "segment_matmul_backward": 'segment_matmul_backward(Tensor values, Tensor weights, Tensor offsets, '
-                               'Tensor grad_out, str program, bool[2] wanted) -> (Tensor, Tensor)',
+                               'Tensor grad_out, str program, bool[2] wanted, str mode="validated") '
+                               '-> (Tensor, Tensor)',
 }
 
 
@@ -208,7 +210,7 @@ def _scan_call(values, gates, offsets, initial, program, mode: str, record: bool
     return out, final, carries
 
 
-def _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final, program, known=None):
+def _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final, program, mode, known=None):
     """The gradients of values, gates and initial, on the GPU.  ``known``: the
     tensors are those of a forward call and the gradients autograd made of its
     outputs, so that they fit, and these gradients are wanted."""
@@ -218,10 +220,10 @@ def _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad
     grad_values, grad_gates, grad_initial = (torch.empty_like(t) if want else None
                                              for t, want in zip((values, values, initial), wanted))
     if known:
-        program._gradients(torch, values, gates, offsets, carries, grad_out, None, initial, grad_final, grad_values,
-                           grad_gates, grad_initial, True)
+        program._gradients(torch, values, gates, offsets, carries, grad_out, None, mode, initial, grad_final,
+                           grad_values, grad_gates, grad_initial, True)
     else:
-        program._run_backward(values, gates, offsets, carries, grad_out, None, initial, grad_final, grad_values,
+        program._run_backward(values, gates, offsets, carries, grad_out, None, mode, initial, grad_final, grad_values,
                               grad_gates, grad_initial, True)
     return grad_values, grad_gates, grad_initial
 
@@ -243,9 +245,9 @@ def _register_scan(torch, library, contract) -> None:
     def scan_kernel(values, gates, offsets, initial, program, mode="validated", record=True):
         return _scan_call(values, gates, offsets, initial, _table.lookup(program, "scan"), mode, record)
 
-    def scan_backward_kernel(values, gates, offsets, initial, carries, grad_out, grad_final, program):
+    def scan_backward_kernel(values, gates, offsets, initial, carries, grad_out, grad_final, program, mode="validated"):
         grads = _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final,
-                                    _table.lookup(program, "scan"))
+                                    _table.lookup(program, "scan"), mode)
         return grads if initial is not None else (*grads[:2], carries.new_empty((0,)))
 
     for key in ("CPU", "CUDA"):
@@ -262,14 +264,15 @@ def _register_scan(torch, library, contract) -> None:
                 torch.empty(carries, **state))
 
     @torch.library.register_fake("ragged_mlir::segment_scan_backward", lib=library)
-    def scan_backward_fake(values, gates, offsets, initial, carries, grad_out, grad_final, program):
+    def scan_backward_fake(values, gates, offsets, initial, carries, grad_out, grad_final, program, mode="validated"):
+        contract.mode(mode)
         grad = torch.empty(values.shape, dtype=values.dtype, device=values.device)
         state = torch.empty(initial.shape if initial is not None else (0,), dtype=torch.float32, device=values.device)
         return grad, torch.empty_like(grad), state
 
     def setup(ctx, inputs, output):
-        values, gates, offsets, initial, program, _, record = inputs
-        ctx.record, ctx.program, ctx.has_initial = record, program, initial is not None
+        values, gates, offsets, initial, program, mode, record = inputs
+        ctx.record, ctx.program, ctx.mode, ctx.has_initial = record, program, mode, initial is not None
         ctx.save_for_backward(values, gates, offsets, output[2], *([initial] if initial is not None else []))
         ctx.mark_non_differentiable(output[2])
         ctx.set_materialize_grads(False)
@@ -285,7 +288,7 @@ def _register_scan(torch, library, contract) -> None:
             grad_out = torch.zeros_like(values)
         grads = torch.ops.ragged_mlir.segment_scan_backward(
             values, gates, offsets, initial[0] if ctx.has_initial else None, carries, grad_out, grad_final,
-            ctx.program)
+            ctx.program, ctx.mode)
         return grads[0], grads[1], None, grads[2] if ctx.has_initial else None, None, None, None
 
     torch.library.register_autograd("ragged_mlir::segment_scan", backward, setup_context=setup, lib=library)
@@ -299,16 +302,16 @@ def _matmul_call(values, weights, offsets, program, mode: str):
     return out
 
 
-def _matmul_backward_call(values, weights, offsets, grad_out, program, wanted, known=False):
+def _matmul_backward_call(values, weights, offsets, grad_out, program, wanted, mode, known=False):
     """The gradients of values and weights (None: not wanted), on the GPU;
     ``known`` as for the scan."""
     torch = _torch()
     values, weights, grad_out = _dense(values, weights, grad_out)
     grads = [torch.empty_like(t) if want else None for t, want in zip((values, weights), wanted)]
     if known:
-        program._gradients(torch, values, weights, offsets, grad_out, None, *grads, True)
+        program._gradients(torch, values, weights, offsets, grad_out, None, mode, *grads, True)
     else:
-        program._run_backward(values, weights, offsets, grad_out, None, *grads, True)
+        program._run_backward(values, weights, offsets, grad_out, None, mode, *grads, True)
     return grads
 
 
@@ -335,7 +338,7 @@ def _autograd_functions(torch) -> dict[str, Any]:
         def forward(ctx, values, gates, offsets, initial, program, mode):
             out, final, carries = _scan_call(values, gates, offsets, initial, program, mode, True)
             ctx.save_for_backward(values, gates, offsets, carries, initial)
-            ctx.program = program
+            ctx.program, ctx.mode = program, mode
             ctx.set_materialize_grads(False)
             return out, final
 
@@ -349,14 +352,14 @@ def _autograd_functions(torch) -> dict[str, Any]:
                 grad_out = torch.zeros_like(values)
             wanted = ctx.needs_input_grad
             grads = _scan_backward_call(values, gates, offsets, initial, carries, grad_out, grad_final, ctx.program,
-                                        (wanted[0], wanted[1], wanted[3]))
+                                        ctx.mode, (wanted[0], wanted[1], wanted[3]))
             return grads[0], grads[1], None, grads[2], None, None
 
     class Matmul(torch.autograd.Function):
         @staticmethod
         def forward(ctx, values, weights, offsets, program, mode):
             ctx.save_for_backward(values, weights, offsets)
-            ctx.program = program
+            ctx.program, ctx.mode = program, mode
             ctx.set_materialize_grads(False)
             return _matmul_call(values, weights, offsets, program, mode)
 
@@ -367,7 +370,8 @@ def _autograd_functions(torch) -> dict[str, Any]:
             if grad_out is None or not any(wanted):
                 return (None,) * 5
             values, weights, offsets = ctx.saved_tensors
-            return (*_matmul_backward_call(values, weights, offsets, grad_out, ctx.program, wanted, True), None, None, None)
+            return (*_matmul_backward_call(values, weights, offsets, grad_out, ctx.program, wanted, ctx.mode, True),
+                    None, None, None)
 
     _functions.update(scan=Scan, matmul=Matmul)
     return _functions
@@ -377,8 +381,8 @@ def _register_matmul(torch, library, contract) -> None:
     def matmul_kernel(values, weights, offsets, program, mode="validated"):
         return _matmul_call(values, weights, offsets, _table.lookup(program, "matmul"), mode)
 
-    def matmul_backward_kernel(values, weights, offsets, grad_out, program, wanted):
-        grads = _matmul_backward_call(values, weights, offsets, grad_out, _table.lookup(program, "matmul"), wanted)
+    def matmul_backward_kernel(values, weights, offsets, grad_out, program, wanted, mode="validated"):
+        grads = _matmul_backward_call(values, weights, offsets, grad_out, _table.lookup(program, "matmul"), wanted, mode)
         return tuple(values.new_empty((0,)) if g is None else g for g in grads)
 
     for key in ("CPU", "CUDA"):
@@ -392,11 +396,12 @@ def _register_matmul(torch, library, contract) -> None:
         return values.new_empty((values.shape[0], weights.shape[2]))
 
     @torch.library.register_fake("ragged_mlir::segment_matmul_backward", lib=library)
-    def matmul_backward_fake(values, weights, offsets, grad_out, program, wanted):
+    def matmul_backward_fake(values, weights, offsets, grad_out, program, wanted, mode="validated"):
+        contract.mode(mode)
         return tuple(t.new_empty(t.shape if want else (0,)) for t, want in zip((values, weights), wanted))
 
     def setup(ctx, inputs, output):
-        values, weights, offsets, ctx.program, _ = inputs
+        values, weights, offsets, ctx.program, ctx.mode = inputs
         ctx.save_for_backward(values, weights, offsets)
         ctx.set_materialize_grads(False)
 
@@ -406,7 +411,8 @@ def _register_matmul(torch, library, contract) -> None:
         if grad_out is None or not any(wanted):
             return (None,) * 5
         values, weights, offsets = ctx.saved_tensors
-        grads = torch.ops.ragged_mlir.segment_matmul_backward(values, weights, offsets, grad_out, ctx.program, wanted)
+        grads = torch.ops.ragged_mlir.segment_matmul_backward(values, weights, offsets, grad_out, ctx.program, wanted,
+                                                              ctx.mode)
         return grads[0] if wanted[0] else None, grads[1] if wanted[1] else None, None, None, None
 
     torch.library.register_autograd("ragged_mlir::segment_matmul", backward, setup_context=setup, lib=library)

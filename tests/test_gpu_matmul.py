@@ -671,3 +671,80 @@ def test_the_first_call_of_a_thread(cuda, call):
         assert torch.equal(out, want[0])
     else:
         assert torch.equal(grads[0], want[1]) and torch.equal(grads[1], want[2])
+
+
+@pytest.mark.parametrize("k,m,lengths", [(64, 64, [20_000]), (33, 100, [9000, 0, 5, 3001]), (136, 257, [5000]),
+                                         (72, 136, [3, 0, 200]), (1024, 1544, [9000, 0, 700])])
+def test_checked_backward(cuda, k, m, lengths):
+    """The offsets are validated first; parts of sums and packed operands in the
+    scratch are not taken for words of waits that gave up."""
+    torch = cuda
+    from ragged import ValidationError
+    case = make_case(lengths, k, m, "bf16", seed=k)
+    t = device(torch, case, "bf16")
+    program = matmul_program("bf16", k, m)
+    plain, checked = ([torch.full_like(t[name], SENTINEL) for name in ("values", "weights")] for _ in range(2))
+    for mode, (gv, gw) in (("validated", plain), ("checked", checked)):
+        dirty_allocator(torch, 1 << 20, 1 << 22)
+        report = program.run_backward(t["values"], t["weights"], t["offsets"], t["grad_out"], mode=mode,
+                                      grad_values=gv, grad_weights=gw)
+    assert report.mode == "checked" and report.kernel_names[:2] == ("offsets_init", "offsets_check")
+    assert all(torch.equal(a, b) for a, b in zip(plain, checked))
+    wrong = t["offsets"].clone()
+    wrong[-1] -= 1
+    with pytest.raises(ValidationError, match="offsets validation failed"):
+        program.run_backward(t["values"], t["weights"], wrong, t["grad_out"], mode="checked", grad_values=plain[0])
+    with pytest.raises(ValidationError, match="mode"):
+        program.run_backward(t["values"], t["weights"], t["offsets"], t["grad_out"], mode="unsafe", grad_values=plain[0])
+
+
+@pytest.mark.parametrize("route", ["run", "call", "operator"])
+@pytest.mark.parametrize("kind,k,m,lengths,kernel", [
+    ("grad_values", 72, 136, [300, 0, 41], "matmul_tensor"), ("grad_values", 1024, 1544, [9000, 0, 700], "matmul_pair"),
+    ("grad_weights", 72, 136, [300, 0, 41], "matmul_tensor"), ("grad_weights", 64, 64, [20_000], "matmul_tensor")])
+def test_a_wait_that_gave_up_in_a_gradient_is_reported(cuda, monkeypatch, kind, k, m, lengths, kernel, route):
+    """A launch that reports a wait that gave up (its words are written here, by
+    the host, after the launch: the last CTA's) raises in checked mode alone."""
+    torch = cuda
+    from ragged import _native, torch_adapter
+    case = make_case(lengths, k, m, "bf16")
+    t = device(torch, case, "bf16")
+    program = matmul_program("bf16", k, m)
+    scratch, empty, launch = [], torch.empty, _native.matmul
+
+    def remember(*args, **options):
+        made = empty(*args, **options)
+        if options.get("dtype") == torch.uint8:
+            scratch.append(made)
+        return made
+
+    def give_up(which, *args, **options):
+        report = _native.Report()
+        launch(which, *args[:-2], report, args[-1])
+        if args[-2] is not None:
+            import ctypes
+            ctypes.memmove(ctypes.byref(args[-2]), ctypes.byref(report), ctypes.sizeof(report))
+        if which == kind:
+            names = [_native.kernel_name(report.kernel_ids[i]) for i in range(report.num_launches)]
+            scratch[-1].view(torch.int64)[report.grid[names.index(kernel)][0] - 1] = 1
+
+    monkeypatch.setattr(torch, "empty", remember)
+    monkeypatch.setattr(_native, "matmul", give_up)
+    leaves = [t["values"].requires_grad_(), t["weights"].requires_grad_()]
+    names = ("grad_values", "grad_weights")
+
+    def gradients(mode):
+        if route == "run":
+            grads = {name: torch.empty_like(x) for name, x in zip(names, leaves) if name == kind}
+            program.run_backward(t["values"], t["weights"], t["offsets"], t["grad_out"], mode=mode, **grads)
+            return
+        if route == "call":
+            out = torch_adapter.segment_matmul(*leaves, t["offsets"], program=program, mode=mode)
+        else:
+            torch_adapter.register_torch_ops()
+            out = torch.ops.ragged_mlir.segment_matmul(*leaves, t["offsets"], torch_adapter.register_program(program), mode)
+        torch.autograd.grad(out, leaves[names.index(kind)], t["grad_out"])
+
+    gradients("validated")
+    with pytest.raises(RuntimeError, match="bounded wait"):
+        gradients("checked")

@@ -566,3 +566,25 @@ def test_padded_rows_of_results_are_zero(cuda, dtype, d, lengths, behind, initia
     grads = torch.autograd.grad((out, final), leaves, (t["grad_out"], t["grad_final"]))
     for got, name in zip((out, final, *grads), ("out", "final", "grad_values", "grad_gates", "grad_initial")):
         assert torch.equal(got, want[name]), name
+
+
+def test_checked_backward_validates_the_offsets(cuda):
+    torch = cuda
+    from ragged import ValidationError, torch_adapter
+    program = scan_program("f32", 8)
+    case = make_case([700, 0, 301], 8, "f32", False)
+    t = device(torch, case, "f32", "i64")
+    carries = torch.empty((program.carry_rows(1001), 8), device="cuda")
+    program.run(t["values"], t["gates"], t["offsets"], torch.empty_like(t["values"]), carries=carries)
+    grads = []
+    for mode in ("validated", "checked"):
+        grads.append(torch.empty_like(t["values"]))
+        report = program.run_backward(t["values"], t["gates"], t["offsets"], carries, t["grad_out"], mode=mode,
+                                      grad_values=grads[-1])
+    assert report.kernel_names[:2] == ("offsets_init", "offsets_check") and torch.equal(*grads)
+    for mode, wrong in (("checked", t["offsets"] + 1), ("unsafe", t["offsets"])):
+        with pytest.raises(ValidationError, match="offsets validation failed|mode"):
+            program.run_backward(t["values"], t["gates"], wrong, carries, t["grad_out"], mode=mode, grad_values=grads[0])
+    out, _ = torch_adapter.segment_scan(t["values"].requires_grad_(), t["gates"], t["offsets"], program=program,
+                                        mode="checked")
+    assert torch.equal(torch.autograd.grad(out, t["values"], t["grad_out"])[0], grads[0])
