@@ -15,7 +15,6 @@ from __future__ import annotations
 from contextlib import nullcontext
 from dataclasses import replace
 import importlib
-import sys
 import threading
 import time
 from typing import Any
@@ -37,16 +36,19 @@ THRESHOLDS = (32, 4096)
 _lock = threading.RLock()
 _checked_devices: set[int] = set()
 _device_l2_mib: dict[int, float | None] = {}
+_torch_module: Any = None
 
 
 def _torch():
-    loaded = sys.modules.get("torch")  # (import_module costs most of a microsecond a call)
-    if loaded is not None:
-        return loaded
-    try:
-        return importlib.import_module("torch")
-    except ImportError as exc:
-        raise RuntimeUnavailable("PyTorch is not installed; install the GPU environment to execute") from exc
+    """The torch module, once imported whole: while another thread imports it,
+    import_module waits for the end (and costs most of a microsecond a call)."""
+    global _torch_module
+    if _torch_module is None:
+        try:
+            _torch_module = importlib.import_module("torch")
+        except ImportError as exc:
+            raise RuntimeUnavailable("PyTorch is not installed; install the GPU environment to execute") from exc
+    return _torch_module
 
 
 def device_l2_mib(values) -> float | None:

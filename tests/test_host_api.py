@@ -237,3 +237,30 @@ def test_report_says_which_optimisation_controls_had_an_effect():
     every = set(effects["applied"]) | set(effects["no_effect"])
     assert every == {"classification", "online_fusion", "warp_mapping", "split_mapping", "shuffle",
                      "pointwise_fusion", "row_pipelining", "vectorize", "feature_tile"}
+
+
+_HALF_IMPORTED = """
+import sys, threading
+sys.path[:0] = {paths!r}
+from ragged.runtime import _torch
+assert "torch" not in sys.modules
+importer = threading.Thread(target=lambda: __import__("torch"))
+importer.start()
+while "torch" not in sys.modules:
+    pass
+assert _torch().ready and _torch() is sys.modules["torch"]
+importer.join()
+print("whole")
+"""
+
+
+def test_a_call_waits_for_another_threads_import_of_torch(tmp_path):
+    """No half-initialised module: the import (of a module that takes a while
+    after its entry in sys.modules is there) is waited for."""
+    import subprocess
+    import sys
+    from conftest import PACKAGE
+    (tmp_path / "torch.py").write_text("import time\ntime.sleep(0.5)\nready = True\n")
+    code = _HALF_IMPORTED.format(paths=[str(tmp_path), str(PACKAGE)])
+    result = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert result.returncode == 0 and "whole" in result.stdout, result.stderr[-2000:]
