@@ -31,6 +31,7 @@ from .runtime import CompiledProgram, _torch
 
 MODES = ("validated", "checked")
 REDUCTIONS = ("sum", "max")
+MISMATCH = "custom op does not match compiled program semantics"
 SCHEMAS = {
     "segment_reduce": 'segment_reduce(Tensor values, Tensor offsets, str kind, str program, '
                       'str mode="validated") -> Tensor',
@@ -50,6 +51,11 @@ SCHEMAS = {
                                'Tensor grad_out, str program, bool[2] wanted, str mode="validated") '
                                '-> (Tensor, Tensor)',
 }
+
+
+def _same_op(program, op: str) -> None:
+    if program.spec.op != op:
+        raise ValidationError(MISMATCH)
 
 
 class ProgramTable:
@@ -72,8 +78,7 @@ class ProgramTable:
             program = self._programs.get(token)
         if program is None:
             raise ValidationError("compiled program token is not registered in this process")
-        if program.spec.op != op:
-            raise ValidationError("custom op does not match compiled program semantics")
+        _same_op(program, op)
         return program
 
 
@@ -170,6 +175,8 @@ def output_shape(op: str, values, offsets) -> tuple:
 
 
 def _mask_presence(program, mask) -> None:
+    if not hasattr(program.spec, "mask"):  # a scan or a product
+        raise ValidationError(MISMATCH)
     if program.spec.mask != (mask is not None):
         raise ValidationError("mask presence must match the compiled specialization")
 
@@ -234,6 +241,10 @@ def _no_tangents(torch, *tensors) -> None:
     if forward._current_level >= 0 and any(t is not None and forward.unpack_dual(t).tangent is not None
                                            for t in tensors):
         raise ValidationError("forward-mode derivatives are not supported")
+
+
+def _records(torch, *tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _first_derivative(torch) -> None:
@@ -487,7 +498,8 @@ def segment_scan(values, gates, offsets, *, program: CompiledScan, initial=None,
     on the stream they were first used on, and the capture fails.  Take the
     gradients with ``torch.autograd.grad``, or drop earlier graphs first."""
     torch = _torch()
-    record = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (values, gates, initial))
+    _same_op(program, "scan")
+    record = _records(torch, values, gates, initial)
     _no_tangents(torch, values, gates, initial)
     if _plain(torch, values, gates, offsets, initial):
         if record:
@@ -505,9 +517,10 @@ def segment_matmul(values, weights, offsets, *, program: CompiledMatmul, mode: s
     are zero, as are the gradients of those values.  (On captured backward
     passes: see ``segment_scan``.)"""
     torch = _torch()
+    _same_op(program, "matmul")
     _no_tangents(torch, values, weights)
     if _plain(torch, values, weights, offsets):
-        if torch.is_grad_enabled() and (values.requires_grad or weights.requires_grad):
+        if _records(torch, values, weights):
             return _autograd_functions(torch)["matmul"].apply(values, weights, offsets, program, mode)
         return _matmul_call(values, weights, offsets, program, mode)
     register_torch_ops()
@@ -515,13 +528,26 @@ def segment_matmul(values, weights, offsets, *, program: CompiledMatmul, mode: s
 
 
 def bind(program: CompiledProgram, *, mode: str = "validated"):
-    """A callable ``f(values, offsets[, mask])`` that only invokes the opaque
-    operator with this program's token, so torch.compile can capture it in a
-    full graph.  The program is registered here, once."""
+    """A callable that only invokes the opaque operator with this program's
+    token, so torch.compile can capture it in a full graph: ``f(values,
+    offsets[, mask])``, for a scan ``f(values, gates, offsets[, initial])`` ->
+    (out, final) and for a product ``f(values, weights, offsets)``, both
+    differentiable.  The program is registered here, once."""
     if mode not in MODES:
         raise ValidationError("mode must be validated or checked")
+    torch = _torch()
     operators = register_torch_ops()
     token = register_program(program)
+    if program.spec.op == "scan":
+        scan_op = torch.ops.ragged_mlir.segment_scan
+
+        def scan(values, gates, offsets, initial=None):
+            return scan_op(values, gates, offsets, initial, token, mode, _records(torch, values, gates, initial))[:2]
+
+        return scan
+    if program.spec.op == "matmul":
+        matmul_op = torch.ops.ragged_mlir.segment_matmul
+        return lambda values, weights, offsets: matmul_op(values, weights, offsets, token, mode)
     if program.spec.op != "softmax":
         reduce_op, kind = operators["segment_reduce"], program.spec.op
         return lambda values, offsets: reduce_op(values, offsets, kind, token, mode)

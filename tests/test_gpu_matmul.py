@@ -748,3 +748,30 @@ def test_a_wait_that_gave_up_in_a_gradient_is_reported(cuda, monkeypatch, kind, 
     gradients("validated")
     with pytest.raises(RuntimeError, match="bounded wait"):
         gradients("checked")
+
+
+@pytest.mark.parametrize("compiled", [False, True])
+def test_bound_programs_give_what_the_calls_give(cuda, compiled):
+    torch = cuda
+    from ragged import ArtifactCache, Compiler, ScanSpec, torch_adapter
+    case = make_case([5, 0, 130, 2], 32, 48, "bf16")
+    t = device(torch, case, "bf16")
+    scan = Compiler().compile(ScanSpec("bf16", 48), ArtifactCache(_cache_dir(), max_specializations=4096))
+    product = matmul_program("bf16", 32, 48)
+    project, recur = torch_adapter.bind(product), torch_adapter.bind(scan)
+    leaves = [t["values"].requires_grad_(), t["weights"].requires_grad_(),
+              torch.rand_like(t["grad_out"]).requires_grad_(), torch.randn(4, 48, device="cuda", requires_grad=True)]
+
+    def model(values, weights, gates, initial, offsets):
+        out, final = recur(project(values, weights, offsets), gates, offsets, initial)
+        return recur(out, gates, offsets)[0], final
+
+    if compiled:
+        model = torch.compile(model, backend="aot_eager", fullgraph=True)
+    got = model(*leaves, t["offsets"])
+    x = torch_adapter.segment_matmul(*leaves[:2], t["offsets"], program=product)
+    out, final = torch_adapter.segment_scan(x, leaves[2], t["offsets"], program=scan, initial=leaves[3])
+    want = torch_adapter.segment_scan(out, leaves[2], t["offsets"], program=scan)[0], final
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    grads = [torch.autograd.grad((y.float().sum(), f.sum()), leaves) for y, f in (got, want)]
+    assert all(torch.equal(a, b) for a, b in zip(*grads))

@@ -207,3 +207,50 @@ def test_njt_mask_routes_the_dense_mask(monkeypatch):
     assert len(calls) == 1 and calls[0]["mask"] is mask and calls[0]["mode"] == "checked"
     with pytest.raises(ValidationError, match="mask presence"):
         torch_adapter.bind(program)(values, offsets)
+
+
+def _learned(spec, name):
+    return SimpleNamespace(spec=spec, artifact=SimpleNamespace(key=SimpleNamespace(digest=name)))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_bound_learned_programs_in_a_full_graph(monkeypatch, grad):
+    from ragged import MatmulSpec, ScanSpec, ValidationError, torch_adapter
+    monkeypatch.setattr(torch_adapter, "_table", torch_adapter.ProgramTable())
+    product = torch_adapter.bind(_learned(MatmulSpec("f32", 8, 4), "bound-product"))
+    scan = torch_adapter.bind(_learned(ScanSpec("f32", 4), "bound-scan"))
+
+    def model(values, weights, gates, offsets, initial):
+        out, final = scan(product(values * 2, weights, offsets), gates, offsets, initial)
+        free, _ = scan(out, gates, offsets)
+        return free + 1, final
+
+    meta = dict(device="meta", requires_grad=grad)
+    leaves = [torch.empty(shape, **meta) for shape in ((30, 8), (3, 8, 4), (30, 4))]
+    offsets, initial = torch.empty((4,), dtype=torch.int64, device="meta"), torch.empty((3, 4), **meta)
+    out, final = torch.compile(model, backend="aot_eager", fullgraph=True)(*leaves, offsets, initial)
+    assert out.shape == (30, 4) and final.shape == (3, 4) and final.dtype == torch.float32
+    assert out.requires_grad == grad
+    if grad:
+        (out.sum() + final.sum()).backward()
+        assert all(x.grad.shape == x.shape for x in (*leaves, initial))
+    for bad in ("checkd", None):
+        with pytest.raises(ValidationError, match="mode"):
+            torch_adapter.bind(_learned(ScanSpec("f32", 4), "bound-scan"), mode=bad)
+
+
+def test_programs_of_another_operator_are_refused(monkeypatch):
+    from ragged import MatmulSpec, ProgramSpec, ScanSpec, ValidationError, torch_adapter
+    monkeypatch.setattr(torch_adapter, "_table", torch_adapter.ProgramTable())
+    programs = {spec.op: _learned(spec, f"mismatch-{spec.op}") for spec in (
+        ProgramSpec("sum", "f32", 8), ProgramSpec("softmax", "f32", 8), ScanSpec("f32", 8), MatmulSpec("f32", 8, 8))}
+    values, weights, offsets = torch.ones((4, 8)), torch.ones((1, 8, 8)), torch.tensor([0, 4])
+    calls = dict(sum=lambda p: torch_adapter.segment_reduce(values, offsets, "sum", program=p),
+                 softmax=lambda p: torch_adapter.segment_softmax(values, offsets, program=p),
+                 scan=lambda p: torch_adapter.segment_scan(values, values, offsets, program=p),
+                 matmul=lambda p: torch_adapter.segment_matmul(values, weights, offsets, program=p))
+    for op, call in calls.items():
+        for other, program in programs.items():
+            if other != op:
+                with pytest.raises(ValidationError, match="does not match"):
+                    call(program)
