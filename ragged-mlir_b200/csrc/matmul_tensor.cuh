@@ -240,6 +240,7 @@ struct TensorStore {
             for (int i = 0; i < 64; ++i)
               if (col0 + i < p.cols) row[col0 + i] = __uint_as_float(v[i / 32][i % 32]);
           }
+          __syncwarp();  // the next load of tensor memory is one of all lanes
           continue;
         }
       }
