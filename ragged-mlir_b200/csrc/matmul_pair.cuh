@@ -138,7 +138,7 @@ matmul_pair_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps) 
   asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
   const uint32_t tmem = tmem_base;
   const TensorGate gate{&abandoned, p.status + blockIdx.x};
-  auto abandoned_now = [&]() { return *gate.abandoned != 0; };
+  auto abandoned_now = [&]() { return __any_sync(~0u, *gate.abandoned != 0) != 0; };
 
   MatmulWalk<OffT, KIND, kPairRows> walk(p.offsets, p.b);
   MatmulTile t;
@@ -259,7 +259,7 @@ matmul_pair_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps) 
       going = !abandoned_now();
       if (KIND == MATMUL_GRAD_WEIGHTS && going && whole < count) {
         const int stage = at.stage;
-        going = rank == 0 ? gate.wait(&full[stage], at.phase) : gate.wait(&tail[stage], (tails >> stage) & 1);
+        going = rank == 0 ? gate.wait_together(&full[stage], at.phase) : gate.wait_together(&tail[stage], (tails >> stage) & 1);
         if (!going) break;
         unsigned char *left = smem + stage * kStage, *right = left + kPairHalf;
         const int from = static_cast<int>(t.end - t.begin - int64_t{whole} * DEPTH), steps = (from + 15) / 16;
@@ -272,7 +272,7 @@ matmul_pair_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps) 
         fence_proxy_async_shared();
         __syncwarp();
         if (rank == 0) {
-          going = wait_cluster(&theirs[stage], (tails >> stage) & 1);
+          going = __all_sync(~0u, wait_cluster(&theirs[stage], (tails >> stage) & 1)) != 0;
           if (!going) break;
           if (elect_lane()) {
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
@@ -304,7 +304,7 @@ matmul_pair_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps) 
     for (int64_t index = first; going && walk.find(p, index, t); index += stride) {
       const bool nothing = KIND == MATMUL_GRAD_WEIGHTS && t.end == t.begin;
       if (!nothing) {
-        going = gate.wait(&ready[acc], acc_phase, slices(t));
+        going = gate.wait_together(&ready[acc], acc_phase, slices(t));
         if (!going) break;
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
       }

@@ -190,6 +190,11 @@ struct TensorGate {
     *status = 1;
     return false;
   }
+  // By all lanes of a warp, which go on, or give up, as one: what comes next
+  // (votes, tensor-memory loads) needs all of them.
+  __device__ __forceinline__ bool wait_together(uint64_t *bar, uint32_t parity, int64_t slices = 0) const {
+    return __all_sync(~0u, wait(bar, parity, slices)) != 0;
+  }
 };
 
 // Empties a warp's 32 rows (`quarter`: of the accumulator's 128, those this warp
@@ -324,7 +329,7 @@ matmul_tensor_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps
   asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
   const uint32_t tmem = tmem_base;
   const TensorGate gate{&abandoned, p.status + blockIdx.x};
-  auto abandoned_now = [&]() { return *gate.abandoned != 0; };
+  auto abandoned_now = [&]() { return __any_sync(~0u, *gate.abandoned != 0) != 0; };
 
   MatmulWalk<OffT, KIND, ROWS> walk(p.offsets, p.b);
   MatmulTile t;
@@ -425,7 +430,7 @@ matmul_tensor_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps
       at.skip(static_cast<uint32_t>(whole));
       going = !abandoned_now();
       if (KIND == MATMUL_GRAD_WEIGHTS && going && whole < count) {
-        going = gate.wait(&full[at.stage], at.phase);
+        going = gate.wait_together(&full[at.stage], at.phase);
         if (!going) break;
         unsigned char *left = smem + at.stage * kStage, *right = left + kLeftBytes;
         const int from = static_cast<int>(t.end - t.begin - int64_t{whole} * DEPTH), steps = (from + 15) / 16;
@@ -463,7 +468,7 @@ matmul_tensor_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps
     for (int64_t index = blockIdx.x; going && walk.find(p, index, t); index += gridDim.x) {
       const bool nothing = KIND == MATMUL_GRAD_WEIGHTS && t.end == t.begin;
       if (!nothing) {
-        going = gate.wait(&ready[acc], acc_phase, slices(t));
+        going = gate.wait_together(&ready[acc], acc_phase, slices(t));
         if (!going) break;
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
       }
