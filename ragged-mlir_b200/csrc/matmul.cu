@@ -207,7 +207,7 @@ int make_maps(TensorMaps &maps, const MatmulArgs &p, int right) {
   return RG_OK;
 }
 
-// After a pack launch the product may start before that ends (its copies wait).
+// After a pack launch the product may start before that ends (its roles wait).
 int launch_after_pack(void (*kernel)(MatmulArgs, TensorMaps), dim3 grid, int smem, const MatmulArgs &p,
                       const TensorMaps &maps, cudaStream_t stream) {
   cudaLaunchAttribute serial;

@@ -153,10 +153,12 @@ matmul_pair_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps) 
     return KIND == MATMUL_GRAD_WEIGHTS && tile.end - tile.begin - int64_t{k} * DEPTH < DEPTH;
   };
 
+  // On operands that are being packed, all roles: the waits below are bounded,
+  // and a pack launch may take longer than that.
+  grid_dependency_wait();
   if (warp == 0) {
     // ------------------------------------------------------------ copies --
-    grid_dependency_wait();  // on operands that are being packed
-    fence_proxy_async_global();
+    fence_proxy_async_global();  // (operands that a launch has packed)
     RingPlace<STAGES> at{0, 1};
     bool going = true;
     for (int64_t index = first; going && walk.find(p, index, t); index += stride) {
@@ -259,7 +261,9 @@ matmul_pair_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps) 
       going = !abandoned_now();
       if (KIND == MATMUL_GRAD_WEIGHTS && going && whole < count) {
         const int stage = at.stage;
-        going = rank == 0 ? gate.wait_together(&full[stage], at.phase) : gate.wait_together(&tail[stage], (tails >> stage) & 1);
+        // (the second CTA has not waited for the whole slices before this one)
+        going = rank == 0 ? gate.wait_together(&full[stage], at.phase)
+                          : gate.wait_together(&tail[stage], (tails >> stage) & 1, whole);
         if (!going) break;
         unsigned char *left = smem + stage * kStage, *right = left + kPairHalf;
         const int from = static_cast<int>(t.end - t.begin - int64_t{whole} * DEPTH), steps = (from + 15) / 16;

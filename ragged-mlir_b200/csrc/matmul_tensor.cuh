@@ -338,10 +338,12 @@ matmul_tensor_kernel(const MatmulArgs p, const __grid_constant__ TensorMaps maps
     return (depth + DEPTH - 1) / DEPTH;
   };
 
+  // On operands that are being packed, all roles: the waits below are bounded,
+  // and a pack launch may take longer than that.
+  grid_dependency_wait();
   if (warp == 0) {
     // ------------------------------------------------------------ copies --
-    grid_dependency_wait();  // on operands that are being packed
-    fence_proxy_async_global();
+    fence_proxy_async_global();  // (operands that a launch has packed)
     RingPlace<STAGES> at{0, 1};
     bool going = true;
     for (int64_t index = blockIdx.x; going && walk.find(p, index, t); index += gridDim.x) {
