@@ -275,8 +275,9 @@ int rg_run_noalloc(int op, int dtype, int index_dtype, int64_t d, int64_t n, int
  * rows it is initial[s], or 0.  values, gates and out are [N, D] of `dtype`
  * with 1 <= D <= 65536; states are f32 and are rounded to `dtype` only in out.
  * Gates must be finite, and products of the gates over neighbouring rows of a
- * segment must stay in f32's range where its states are not zero (|gate| <= 1
- * always does).
+ * segment must not overflow f32 where its states are not zero (with |gate| <= 1
+ * none does).  Where such a product underflows to zero, what is left of a finite
+ * state (under 2^-149 of it) is dropped, and an infinite one becomes NaN.
  *
  * rg_scan_workspace_bytes gives the scratch of either call (256-byte aligned;
  * 0: none).  carries (f32 [ceil(N / 8), D]) receives

@@ -344,7 +344,7 @@ __device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddep
 // cp.async.bulk moves a contiguous, 16-byte aligned block of global memory
 // (a multiple of 16 bytes) into this CTA's shared memory and signals an
 // mbarrier with the byte count: one instruction keeps tens of KB in flight.
-// No cluster multicast form is used anywhere in this library.
+// No copy or load of this library uses a cluster multicast form.
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

@@ -13,6 +13,8 @@ namespace rgb {
 
 namespace {
 
+// (The times beside the rules are of single launches between events, inputs cold:
+// they come in steps of 2 us, and a difference of one step decides nothing.)
 constexpr int64_t kMaxWidth = 65536;
 
 struct MatmulShape {

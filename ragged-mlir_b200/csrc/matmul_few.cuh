@@ -6,8 +6,10 @@
 // of the weights, 16 of them on their way into shared memory at a time (a
 // thread reads what it copied: no barrier), and keep f32 sums of all rows of
 // the tile; the sums meet in shared memory, in the order of the half-warps.
-// Bound: device memory (32 rows in 16 segments, 1024 x 2048, bf16: 25 us from a cold
-// L2, 50 MB, 17 without the first loads' way).  For bf16 tensor-core tiles read the
+// 32 rows in 16 segments, 1024 x 2048: bf16 21 us for the 50 MB of the 12 segments
+// with rows, f32 24 for 101 MB, from L2 as from device memory.  Bound: 192 tiles of
+// 256 KB on 148 SMs, so that a third of the SMs carries two (bf16), and the first
+// loads' way.  For bf16 tensor-core tiles read the
 // same bytes and start later, but take more rows at no cost; for f32 the other
 // kernel's tiles compute 64 rows where few are there.
 #pragma once

@@ -13,9 +13,10 @@
 // kind, a segment's last slice), each CTA has its own copies counted on its own
 // barrier and clears its rows, and the second one says so by a remote arrival.
 //
-// 65536 rows x 2048 x 2048 in 16 segments: 360 us forward, 358 and 363 for the
-// gradients of values and weights, 1.52 PFLOP/s (0.92 of a library's dense
-// product); on tiles of one SM 379, 385 and 404.  Bound: the tensor cores (74 %
+// 65536 rows x 2048 x 2048 in 16 segments: 357 to 365 us forward, 353 to 363 and 358
+// to 375 for the gradients of values and weights on several GPUs (single calls; 1.5
+// PFLOP/s, 0.92 of a library's dense product; 390 in a row, under the power limit);
+// on tiles of one SM 379, 385 and 404.  Bound: the tensor cores (74 %
 // busy at 16384 x 1024 x 2048, where the first and last tiles weigh more).  Copies
 // of a stage counted by relayed arrivals instead of on the first CTA's barrier
 // took 965 us; products issued behind a branch on the lane 430.

@@ -9,9 +9,10 @@
 // memory for 64 FMAs, so the pipes and not the loads set the pace.  Packed FMAs
 // (two columns at once) leave issue slots to the loads.
 //
-// 8192 rows x 512 x 512 in 8 segments: 104 us forward, 115 and 127 for the gradients
-// of values and weights: 41 TFLOP/s of the pipes' 74, the rest being rows past the
-// segments' ends and 288 tiles on 296 places.
+// 8192 rows x 512 x 512 in 8 segments: 98 us forward, 105 and 119 to 134 for the
+// gradients of values and weights: 32 to 44 TFLOP/s of the pipes' 74.  288 tiles on
+// 296 places are one wave, partly of rows past the segments' ends; within a tile the
+// FMA pipe is busy 38 % in packed FMAs (two each), the issue slots half.
 #pragma once
 
 #include "matmul.cuh"

@@ -23,10 +23,12 @@
 // Sums are f32 in tensor memory.  Every wait is bounded; one that gives up
 // sets the call's status word, and all roles leave.
 //
-// Bound: with some hundred rows a segment device memory and the last row tile
-// of each segment (16384 rows x 1024 x 1024 in 64 segments of unlike lengths:
-// 57 us, 600 TFLOP/s and 3.5 TB/s); with few rows the weights, read once (8192 rows
-// x 1024 x 64 in 256 segments: 18 us, 2.8 TB/s); in large products the operands
+// With some hundred rows a segment neither device memory nor the tensor cores are at
+// their limit (16384 rows x 1024 x 1024 in 64 segments of unlike lengths: 48 us, 53 %
+// of the tensor cores' cycles, a quarter of them for rows past a segment's end, 48 %
+// of the memory's); with few rows each CTA's way to its first tile, along the offsets,
+// counts (8192 rows x 1024 x 64 in 256 segments: 13 us, 17 with cold inputs, where
+// the bytes take 8); in large products the operands
 // that L2 delivers to an SM, which pairs of SMs halve (matmul_pair.cuh).
 #pragma once
 
@@ -505,9 +507,10 @@ struct PackArgs {
   int64_t rows, cols, pitch;
 };
 
-// One launch for both operands, 16 loads a lane at once; the product's launch may
-// start before it ends.  (5003 rows x 501 x 333 in 12 segments: 17 us a call in a
-// replayed graph, 19 with a launch each; 16001 rows x 1001 x 777 87 and 93.)
+// One launch for both operands, all weights among them, 16 loads a lane at once; the
+// product's launch may start before it ends.  (5003 rows x 501 x 333 in 12 segments:
+// 17 us a call in a replayed graph, 18 with cold inputs, 19 with a launch each; 16001
+// rows x 1001 x 777 87 and 93.)
 __global__ void __launch_bounds__(256) matmul_pack_kernel(const PackArgs left, const PackArgs right) {
   grid_dependents_launch();
   const int64_t stride = static_cast<int64_t>(gridDim.x) * 8;

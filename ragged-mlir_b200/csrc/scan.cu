@@ -27,7 +27,7 @@ bool walks_alone(int64_t n, int64_t b) { return n <= 128 || (n <= 512 && n <= 4 
 // 32 lanes, or as many as cover a row, of one vector each: 8 bytes where they
 // fill the lanes, else 4 (one element where D is odd).  8 bytes take two thirds
 // of the instructions: bf16 65536 x 1024 139 us (backward 186), 166 (227) with 4;
-// f32 262144 x 100 117 (158) and 131 (326).  A lane takes 64 rows of a slab, fewer
+// f32 262144 x 100 117 (158) and 131 (326), with a slower join than today's.  A lane takes 64 rows of a slab, fewer
 // where that would leave resident warps without a task: f32 262144 x 100 117 us,
 // 158 with 16; 4096 x 512 20 (23) with 16, 29 (35) with 64.  `align`: elements that
 // all tensors are aligned for.
@@ -39,7 +39,7 @@ ScanShape make_shape(int dtype, int64_t d, int64_t n, int64_t b, int align) {
   while ((int64_t{1} << s.shift) * s.vec < d && s.shift < 5) ++s.shift;
   s.tiles = static_cast<int>(ceil_div(d, (int64_t{1} << s.shift) * s.vec));
   const int groups = 32 >> s.shift;
-  constexpr int64_t warps = 148 * 24;
+  constexpr int64_t warps = 148 * 24;  // of a B200 (the workspace is asked for without a device)
   s.lane_rows = 64;
   while (s.lane_rows > 16 && (ceil_div(n, s.lane_rows * groups) * s.tiles < warps || s.lane_rows * groups > 512))
     s.lane_rows /= 2;

@@ -26,14 +26,20 @@
 // slabs, and walk goes through the slabs from the last one back (forward ones
 // in a backward pass), so that it meets first what fold left in L2.  The
 // arithmetic is one FMA an element, about 10 instructions an element in all.
-// bf16 65536 x 1024 in 16 segments: 140 us forward, 186 backward, 4.8 TB/s of 5
+// bf16 65536 x 1024 in 16 segments: 132 us forward, 176 backward, 5.1 TB/s of 5
 // and 7 passes over a tensor where 3 and 5 are the least; f32 262144 x 100 in 1024
-// segments 110 us.  What is left is the second reading, the join and each launch's
-// first loads; rows read once in a single launch, with waits for the slab before,
-// took 173 to 231 us.  Two halves of a batch in turn, one on its way, spill: 172.
+// segments 98 us and 142.  What is left is the second reading, the join and each
+// launch's first loads; rows read once in a single launch, with waits for the slab
+// before, took 173 to 231 us where this form took 140.  Two halves of a batch in
+// turn, one on its way, spill: 172.  (Times of this form: a graph of calls, inputs
+// larger than L2.  Times of the others, here and beside the rules in scan.cu, are of
+// single launches between events, which come in steps of 2 us.)
 //
 // For few rows walk is the only launch: a lane whose rows go on from earlier ones
-// runs the recurrence over those itself.
+// runs the recurrence over those itself.  Bound there: latency.  200 rows of 200
+// segments, bf16 x 1024, are 104 warps in 13 CTAs, each a chain of dependent reads
+// (the search in the offsets, rows, initial states, segments without rows): 8 us in
+// a graph of calls, 11 with cold inputs.
 //
 // The backward pass needs the states again.  It recomputes 8 rows at a time from
 // values and gates, from the state before them that forward records in f32 (4

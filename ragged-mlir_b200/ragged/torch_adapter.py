@@ -493,10 +493,10 @@ def segment_scan(values, gates, offsets, *, program: CompiledScan, initial=None,
     values, gates and initial.  Rows behind the last offset (a padded batch) are
     zero in out and in the gradients, whatever the inputs hold there.
 
-    Under a CUDA graph capture of a backward pass, autograd itself must not
-    have an eager graph of the same leaves alive: its accumulation nodes stay
-    on the stream they were first used on, and the capture fails.  Take the
-    gradients with ``torch.autograd.grad``, or drop earlier graphs first."""
+    Under a CUDA graph capture of a backward pass (``torch.autograd.grad``
+    included) autograd must not have an eager graph of the same leaves alive:
+    its accumulation nodes stay on the stream they were first used on, and the
+    capture fails, as with torch's own operations.  Drop earlier graphs first."""
     torch = _torch()
     _same_op(program, "scan")
     record = _records(torch, values, gates, initial)

@@ -139,3 +139,23 @@ def test_forward_mode_is_refused(native_library, tmp_path):
             torch_adapter.segment_scan(x, dual, offsets, program=scan)
         with pytest.raises(ValidationError, match="forward-mode"):
             torch_adapter.segment_matmul(dual, w, offsets, program=product)
+
+
+def test_clear_rest_is_a_flag_of_the_calls_alone(native_library):
+    """RG_CLEAR_REST goes with a dtype of rg_scan, rg_scan_backward and rg_matmul,
+    changes no check of theirs, and is none of a size's."""
+    from conftest import REPO
+    from ragged import _native
+    lib, one, flag = native_library, ctypes.c_int64(), _native.CLEAR_REST
+    assert f"RG_CLEAR_REST = {flag} " in (REPO / "include" / "ragged_b200.h").read_text()
+    for dtype in (0, 1):
+        assert lib.rg_matmul(0, dtype | flag, 1, 8, 8, 0, 0, *[None] * 5, 0, None, None) == 0
+        assert lib.rg_scan(dtype | flag, 1, 8, 0, 0, *[None] * 8, 0, None, None) == 0
+        assert lib.rg_scan_backward(dtype | flag, 1, 8, 0, 0, *[None] * 11, 0, None, None) == 0
+        assert lib.rg_matmul(0, dtype | flag, 1, 8, 8, 4, 1, *[None] * 5, 0, None, None) == _native.RG_ERR_INVALID_ARGUMENT
+        assert lib.rg_matmul_workspace_bytes(0, dtype | flag, 1, 8, 8, 4, 1, None, None,
+                                             ctypes.byref(one)) == _native.RG_ERR_INVALID_ARGUMENT
+        assert lib.rg_scan_workspace_bytes(dtype | flag, 1, 8, 4, 1, ctypes.byref(one)) == _native.RG_ERR_INVALID_ARGUMENT
+    for dtype in (2 | flag, flag * 2, -1):
+        assert lib.rg_scan(dtype, 1, 8, 0, 0, *[None] * 8, 0, None, None) == _native.RG_ERR_INVALID_ARGUMENT, dtype
+        assert lib.rg_matmul(0, dtype, 1, 8, 8, 0, 0, *[None] * 5, 0, None, None) == _native.RG_ERR_INVALID_ARGUMENT, dtype
