@@ -362,8 +362,8 @@ def scan(dtype: str, index: str, d: int, n: int, b: int, pointers: tuple, worksp
          stream: int, report: Report | None, clear_rest: bool = False) -> None:
     """``pointers``: values, gates, offsets, initial, out, final, carries (0: none).
     ``clear_rest``: rows behind the last segment are set to zero."""
-    status = library().rg_scan(_rest(dtype, clear_rest), INDEX[index], d, n, b, *pointers, workspace_ptr, workspace_bytes, stream,
-                               report)
+    status = library().rg_scan(_rest(dtype, clear_rest), INDEX[index], d, n, b, *pointers, workspace_ptr,
+                               workspace_bytes, stream, report)
     if status:
         raise_for(status, "rg_scan")
 
